@@ -135,6 +135,34 @@ class AttnDecodeArgs(C.Structure):
     ]
 
 
+class Kv8StoreArgs(C.Structure):
+    _fields_ = [
+        ("qkv", C.c_void_p), ("ld", C.c_long),
+        ("n", C.c_int), ("hq", C.c_int), ("hkv", C.c_int),
+        ("inv_freq", C.c_void_p), ("tok_pos", C.c_void_p), ("rope_pos", C.c_void_p), ("rope_pos3", C.c_void_p), ("pair_axis", C.c_void_p),
+        ("tok_seq", C.c_void_p), ("n_seq", C.c_int),
+        ("block_table", C.c_void_p), ("bt_ld", C.c_int), ("bt_cols", C.c_int),
+        ("pool", C.c_void_p), ("n_pages", C.c_int),
+        ("q_out", C.c_void_p), ("ldq", C.c_long),
+        ("status", C.c_void_p),
+    ]
+
+
+class Kv8AttnArgs(C.Structure):
+    _fields_ = [
+        ("q", C.c_void_p), ("ldq", C.c_long),
+        ("pool", C.c_void_p), ("n_pages", C.c_int),
+        ("block_table", C.c_void_p), ("bt_ld", C.c_int), ("bt_cols", C.c_int), ("n_seq", C.c_int),
+        ("grp_tok0", C.c_void_p), ("grp_cnt", C.c_void_p), ("n_groups", C.c_int),
+        ("tok_pos", C.c_void_p), ("tok_seq", C.c_void_p), ("n_tok", C.c_int),
+        ("tree_mask", C.c_void_p),
+        ("hq", C.c_int), ("hkv", C.c_int),
+        ("scale_log2", C.c_float),
+        ("out", C.c_void_p), ("ldo", C.c_long),
+        ("status", C.c_void_p),
+    ]
+
+
 class WqMmArgs(C.Structure):
     _fields_ = [
         ("wq", C.c_void_p), ("n", C.c_int), ("k", C.c_int), ("m", C.c_int),
@@ -189,6 +217,9 @@ def _declare(lib: C.CDLL):
         "b2_fill_u32": ([vp, C.c_uint32, l, vp], i),
         "b2_attn_decode": ([C.POINTER(AttnDecodeArgs), i, vp], i),
         "b2_attn_decode_smem_bytes": ([i], i),
+        "b2_kv8_store": ([C.POINTER(Kv8StoreArgs), i, i, vp], i),
+        "b2_kv8_attn": ([C.POINTER(Kv8AttnArgs), i, i, vp], i),
+        "b2_kv8_read": ([vp, i, i, i, i, vp, i, l, vp, vp, vp], i),
         "b2_ipc_alloc": ([C.c_size_t, C.POINTER(vp), C.c_char_p], i),
         "b2_ipc_open": ([C.c_char_p, C.POINTER(vp)], i),
         "b2_ipc_close": ([vp], i),

@@ -160,6 +160,8 @@ class Kv8AttnArgs(C.Structure):
         ("scale_log2", C.c_float),
         ("out", C.c_void_p), ("ldo", C.c_long),
         ("status", C.c_void_p),
+        ("split_keys", C.c_int), ("max_splits", C.c_int),
+        ("part_o", C.c_void_p), ("part_ml", C.c_void_p),
     ]
 
 

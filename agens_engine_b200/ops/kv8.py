@@ -24,6 +24,7 @@ from .._lib import Kv8AttnArgs, Kv8StoreArgs, check, ptr
 PAGE = 16
 FORMATS = {"int8": 0, "fp8": 1}
 GROUP_ROWS = 32                    # most rows of one attention group (bits of a tree mask)
+MAX_SPLIT = 2048                   # most keys of one split
 
 
 def block_bytes(hd: int) -> int:
@@ -36,6 +37,22 @@ def make_pool(n_pages: int, hkv: int, hd: int, device) -> torch.Tensor:
     if hd not in (64, 128):
         raise ValueError(f"8-bit KV pages: head_dim 64 or 128, got {hd}")
     return torch.zeros(n_pages, hkv, block_bytes(hd), dtype=torch.uint8, device=device)
+
+
+def split_keys_for(max_ctx: int) -> int:
+    """Keys of one attention split for contexts of up to ``max_ctx`` tokens: 256, doubled while more than 64 splits were needed.  A
+    constant of the engine, since a row's bits depend on it."""
+    s = 256
+    while s < MAX_SPLIT and s * 64 < max_ctx:
+        s *= 2
+    return s
+
+
+def part_floats(n_tok: int, hq: int, hd: int, max_ctx: int, split_keys: Optional[int] = None) -> int:
+    """fp32 entries of the workspace that :func:`attn_decode8` needs for ``n_tok`` rows (0: none).  One workspace serves any number
+    of calls one after the other; calls that may run at the same time need one each, captured ones too."""
+    splits = -(-max_ctx // (split_keys or split_keys_for(max_ctx)))
+    return n_tok * hq * splits * (hd + 2) if splits > 1 else 0
 
 
 def _format(fmt: str) -> int:
@@ -128,13 +145,19 @@ def rope_kvstore8(qkv: torch.Tensor, hq: int, hkv: int, hd: int, inv_freq: torch
 
 
 def attn_decode8(q: torch.Tensor, pool: torch.Tensor, fmt: str, block_table: torch.Tensor, grp_tok0: torch.Tensor, grp_cnt: torch.Tensor,
-                 tok_pos: torch.Tensor, tok_seq: torch.Tensor, hq: int, hkv: int, hd: int, tree_mask: Optional[torch.Tensor] = None,
+                 tok_pos: torch.Tensor, tok_seq: torch.Tensor, hq: int, hkv: int, hd: int, split_keys: Optional[int] = None,
+                 max_ctx: Optional[int] = None, part: Optional[torch.Tensor] = None, tree_mask: Optional[torch.Tensor] = None,
                  status: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Attention of new rows over 8-bit pages: ``attention.attn_decode`` for a pool of this module.  ``q``: bf16
     ``[n_tok, hq * hd]`` (RoPE applied).  Group ``g`` is the ``grp_cnt[g]`` (at most 32) rows from ``grp_tok0[g]`` on, all of one
-    sequence, whose K and V are in the pool already; row i sees the slots up to ``tok_pos[i]``, of the group's own slots those
-    whose bit its ``tree_mask`` (int32 ``[n_tok]``) has.  A row that sees nothing (``tok_pos`` -1, an empty mask) gives zeros; rows
-    of no group are left as they were in ``out``.  Returns bf16 ``[n_tok, hq * hd]``."""
+    sequence in ascending order of ``tok_pos``, whose K and V are in the pool already; row i sees the slots up to ``tok_pos[i]``, of
+    the slots from the group's first on those whose bit its ``tree_mask`` (int32 ``[n_tok]``) has.  A row that sees nothing
+    (``tok_pos`` -1 in a group of its own, an empty mask) gives zeros; rows of no group are left as they were in ``out``.
+
+    ``split_keys`` (a multiple of 16, at most 2048; default :func:`split_keys_for` the table's length) cuts every sequence into
+    splits that are joined at the end; a row's bits depend on its own position and on ``split_keys`` only.  ``max_ctx`` (default:
+    the table's length) bounds the positions, ``part`` is a workspace of :func:`part_floats` entries (default: allocated for the
+    call).  Returns bf16 ``[n_tok, hq * hd]``."""
     f, dev = _format(fmt), q.device
     n = q.shape[0]
     _need(hq > 0 and hkv > 0 and hq % hkv == 0, "hq is a multiple of hkv")
@@ -148,12 +171,24 @@ def attn_decode8(q: torch.Tensor, pool: torch.Tensor, fmt: str, block_table: tor
         out = torch.empty(n, hq * hd, dtype=torch.bfloat16, device=dev)
     else:
         _check_rows(out, n, hq * hd, dev, "out", 8)
+    max_ctx = block_table.shape[1] * PAGE if max_ctx is None else int(max_ctx)
+    _need(0 < max_ctx <= block_table.shape[1] * PAGE, f"max_ctx: 1 .. {block_table.shape[1] * PAGE}, what the block table holds")
+    split_keys = split_keys_for(max_ctx) if split_keys is None else int(split_keys)
+    _need(PAGE <= split_keys <= MAX_SPLIT and split_keys % PAGE == 0, f"split_keys: a multiple of {PAGE} up to {MAX_SPLIT}")
+    splits = -(-max_ctx // split_keys)
+    slots = n * hq * splits if splits > 1 else 0
+    if part is not None:
+        _need(part.dtype is torch.float32 and part.is_contiguous() and part.numel() >= slots * (hd + 2) and part.device == dev and part.data_ptr() % 16 == 0,
+              f"part: contiguous fp32 with at least {slots * (hd + 2)} entries on {dev}")
     status = _status(status, dev)
     if n == 0 or n_groups == 0:
         return out
+    if part is None and slots:
+        part = torch.empty(slots * (hd + 2), dtype=torch.float32, device=dev)
+    at = ptr(part)
     a = Kv8AttnArgs(ptr(q), q.stride(0), ptr(pool), pool.shape[0], ptr(block_table), block_table.stride(0), block_table.shape[1], block_table.shape[0],
                     ptr(grp_tok0), ptr(grp_cnt), n_groups, ptr(tok_pos), ptr(tok_seq), n, ptr(tree_mask), hq, hkv,
-                    math.log2(math.e) / math.sqrt(hd), ptr(out), out.stride(0), ptr(status))
+                    math.log2(math.e) / math.sqrt(hd), ptr(out), out.stride(0), ptr(status), split_keys, splits, at, at + 4 * slots * hd)
     with _on(dev):
         check(_lib.cuda_lib().b2_kv8_attn(C.byref(a), hd, f, torch.cuda.current_stream().cuda_stream), "b2_kv8_attn")
     return out

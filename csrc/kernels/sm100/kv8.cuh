@@ -7,7 +7,7 @@
 // with 128 added, so that one byte permute makes the fp16 number 1024 + byte) or max(amax / 448, 2^-64) for e4m3 codes.
 // code = round-to-nearest-even(x / scale); the row stands for code * scale.  The lower limit keeps 1 / scale finite and lets
 // a row of zeros count as one that adds nothing (the attention weighs rows by their scale's exponent).  A row with an
-// infinity or a NaN gets the scale NaN: it reads back as NaN instead of as a number that hides the fault.
+// infinity or a NaN gets the scale NaN and the codes of zeros: it reads back as NaN instead of as a number that hides the fault.
 #pragma once
 #include <cuda_fp8.h>
 

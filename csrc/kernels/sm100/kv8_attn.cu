@@ -2,7 +2,28 @@
 // and short prefill chunks.  Counterpart in the reference: the INT8 KV of its dense layers, which expands tiles to bf16 and
 // attends to those (kernels/m1/m1_dense8.cu:65-126); here the codes go straight into the products.
 //
-// o = sum_j p_j vs_j vc_j / sum_j p_j,  p_j = exp(q . kc_j ks_j / sqrt(hd) - m)   over the keys that the row sees.
+//     o = sum_j p_j vs_j vc_j / sum_j p_j,    p_j = 2^(s_j - m),    s_j = log2(e) / sqrt(hd) * ks_j * (q . kc_j)
+//
+// over the keys j that the row sees.  One pass with a running reference m; the codes kc, vc become fp16 numbers (exactly: both
+// formats fit), their scales stay in fp32: ks multiplies the finished product, vs the weight before it is rounded.
+//
+// Split.  A sequence's keys are cut every split_keys keys, a constant of the engine; one CTA of four warps takes the keys of one
+// (group, KV head, columns, split), page i of them on warp i % 4, and joins its warps in shared memory.  Rows with one split are
+// finished there, the others leave (o, m, l) per split to kv8_join_kernel.  What a row adds up and in which order depends on its
+// own position alone, so a row has the same bits in a decode step, a verify block or any batch.
+//
+// Products.  The group's rows times the q heads of a KV head are the columns ("N" of the MMA, eight to a tile), keys are the rows
+// of K q^T and head channels the rows of V^T p^T, so a single decode row with eight q heads fills its tiles.  The order of
+// channels inside a product and of keys inside a page is free, and chosen so that every lane loads sixteen bytes of a row at a
+// time straight from global memory into its fragments; shared memory is not used on the way.  Only the weights need a
+// transposition between the products (movmatrix).
+//
+// Range.  The weights reach the second product as fp16 numbers p_j vs_j.  m follows the largest s_j + log2 of vs_j's power of two,
+// so what is rounded is each key's contribution relative to the largest one, whatever the size of V; a key that has weight but no
+// V (a row of zeros has the least scale) cannot push the others out of fp16's range.  m is raised only when a column's largest
+// value has grown by 2^8 (fp16 has room for that), which leaves the accumulators alone for nearly all pages.
+#include <algorithm>
+
 #include "kv8.cuh"
 
 namespace b2 {
@@ -18,55 +39,448 @@ struct Kv8AttnArgs {
   float scale_log2;                         // log2(e) / sqrt(hd)
   bf16* out; long ldo;
   int* status;
+  int split_keys, max_splits;
+  float* part_o;                            // [n_tok][hq][max_splits][hd]; unused when max_splits is 1
+  float* part_ml;                           // [n_tok][hq][max_splits][2]
 };
 
 namespace {
 
-// One warp per (group, q head): row by row, key by key.
-template <int HD, int FMT>
-__global__ void __launch_bounds__(128) kv8_attn_kernel(const Kv8AttnArgs a) {
-  constexpr int PER = HD / 32;
+constexpr int kWarps = 4;
+constexpr float kNoRef = -3.4028234e38f;    // m before the first key
+constexpr float kGrow = 8.f;                // log2 of what a column may grow before m follows
+// l sums 2^(s - m) * 2^30 and the weights carry vs * 2^-30: with V of any size between 2^-64 and 2^121 neither leaves fp32
+constexpr float kUp = 30.f, kDown = 9.313225746154785e-10f;
+
+__device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+// two bytes with 128 added -> two fp16 numbers: 0x64xx is 1024 + xx, then minus 1152
+__device__ __forceinline__ uint32_t biased_pair(uint32_t magic) {
+  const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&magic), __half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480)));
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ uint32_t e4m3_pair(uint32_t two) {
+  uint32_t y;
+  asm("{ .reg .b16 lo, hi; mov.b32 {lo, hi}, %1; cvt.rn.f16x2.e4m3x2 %0, lo; }" : "=r"(y) : "r"(two));
+  return y;
+}
+// Fragment pairs of a word of four codes of one row: channels (0, 2) and (1, 3) for int8, (0, 1) and (2, 3) for e4m3
+template <int FMT>
+__device__ __forceinline__ void row_pairs(uint32_t w, uint32_t& x, uint32_t& y) {
+  if (FMT == KV8_INT8) {
+    x = biased_pair(lop3_and_or(w, 0x00ff00ffu, 0x64006400u));
+    y = biased_pair(__byte_perm(w, 0x64646464u, 0x4341));
+  } else {
+    x = e4m3_pair(w);
+    y = e4m3_pair(w >> 16);
+  }
+}
+// Of two rows' words: pairs (row a, row b) of bytes 2 * HI and 2 * HI + 1
+template <int FMT, int HI>
+__device__ __forceinline__ void cross_pairs(uint32_t wa, uint32_t wb, uint32_t& x, uint32_t& y) {
+  if (FMT == KV8_INT8) {
+    const uint32_t z = __byte_perm(wa, wb, HI ? 0x7632 : 0x5410);
+    x = biased_pair(lop3_and_or(z, 0x00ff00ffu, 0x64006400u));
+    y = biased_pair(__byte_perm(z, 0x64646464u, 0x4341));
+  } else {
+    const uint32_t z = __byte_perm(wa, wb, HI ? 0x7362 : 0x5140);
+    x = e4m3_pair(z);
+    y = e4m3_pair(z >> 16);
+  }
+}
+
+struct Group { int tok0, cnt, first, last, seq; bool ok; };
+
+// A group and whether everything it names is there; `last` is the last slot that its rows may see.
+__device__ __forceinline__ Group group_at(const Kv8AttnArgs& a, int g) {
+  Group r = {0, 0, 0, -1, 0, true};
+  if (g >= a.n_groups) return r;
+  r.tok0 = a.grp_tok0[g]; r.cnt = a.grp_cnt[g];
+  if (r.cnt < 1) { r.cnt = 0; return r; }
+  r.ok = r.cnt <= 32 && r.tok0 >= 0 && r.tok0 <= a.n_tok - r.cnt;
+  if (!r.ok) return r;
+  r.seq = a.tok_seq[r.tok0]; r.first = a.tok_pos[r.tok0];
+  r.last = r.cnt == 1 ? r.first : a.tok_pos[r.tok0 + r.cnt - 1];
+  r.ok = r.seq >= 0 && r.seq < a.n_seq && r.last < a.bt_cols * kKv8Page && r.last / a.split_keys < a.max_splits;
+  return r;
+}
+__device__ __forceinline__ int splits_of(int last_key, int split_keys) { return last_key < 0 ? 1 : last_key / split_keys + 1; }
+
+template <int HD, int FMT, int NT>
+__global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 2) kv8_attn_kernel(const Kv8AttnArgs a) {
+  constexpr int KC = HD / 64;            // 16-byte chunks of a K row per lane
+  constexpr int KS = HD / 16;            // k-steps of K q^T
+  constexpr int VW = HD / 32;            // words of a V row per lane
+  constexpr int MT = HD / 16;            // channel tiles of V^T p^T
+  constexpr int COLS = NT * 8;
+  constexpr int LDO = HD + 4;
+  __shared__ __align__(16) float sh_o[kWarps][COLS][LDO];
+  __shared__ float sh_m[kWarps][COLS], sh_l[kWarps][COLS];
   pdl_wait();
   pdl_launch_dependents();
-  const long item = (long)blockIdx.x * 4 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  const int grp = (int)(item / a.hq), head = (int)(item % a.hq), kvh = head / (a.hq / a.hkv);
-  if (grp >= a.n_groups) return;
-  const int tok0 = a.grp_tok0[grp], cnt = a.grp_cnt[grp];
-  if (cnt < 1) return;
-  bool ok = cnt <= 32 && tok0 >= 0 && tok0 <= a.n_tok - cnt;
-  const int seq = ok ? a.tok_seq[tok0] : -1;
-  ok = ok && seq >= 0 && seq < a.n_seq;
-  const int first = ok ? a.tok_pos[tok0] : 0, last = ok ? a.tok_pos[tok0 + cnt - 1] : 0;
-  ok = ok && last < a.bt_cols * kKv8Page;
-  if (!ok) { if (lane == 0) atomicExch(a.status, (int)B2_ERR_BOUNDS); return; }
-  for (int r = 0; r < cnt; ++r) {
-    const int tok = tok0 + r, pos = min(a.tok_pos[tok], last);
-    const unsigned mask = a.tree_mask ? a.tree_mask[tok] : 0u;
-    float qv[PER], o[PER], m = -INFINITY, l = 0.f;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int gq = a.hq / a.hkv;
+
+  // Items are numbered group after group; every lane holds one group of a run of 32 and the sum of items up to it.
+  int run = -32, base = 0, total = 0, incl = 0, mine = 0;
+  Group grp = {0, 0, 0, -1, 0, true};
+  bool joined = false;                   // shared memory of the item before may still be read
+  for (int item = blockIdx.x;; item += gridDim.x) {
+    while (item - base >= total) {
+      base += total;
+      run += 32;
+      if (run >= a.n_groups) return;
+      grp = group_at(a, run + lane);
+      if (!grp.ok && blockIdx.x == 0 && warp == 0) atomicExch(a.status, (int)B2_ERR_BOUNDS);
+      mine = grp.ok && grp.cnt > 0 ? splits_of(grp.last, a.split_keys) * a.hkv * ((grp.cnt * gq + COLS - 1) / COLS) : 0;
+      incl = mine;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) { qv[i] = __bfloat162float(a.q[(size_t)tok * a.ldq + (size_t)head * HD + lane * PER + i]); o[i] = 0.f; }
-    for (int key = 0; key <= pos; ++key) {
-      if (a.tree_mask && key >= first && (key - first > 31 || !((mask >> (key - first)) & 1u))) continue;
-      const int page = a.block_table[(size_t)seq * a.bt_ld + key / kKv8Page], slot = key % kKv8Page;
-      if (page < 0 || page >= a.n_pages) { if (lane == 0) atomicExch(a.status, (int)B2_ERR_BOUNDS); continue; }
-      const uint8_t* blk = a.pool + ((size_t)page * a.hkv + kvh) * kv8_block_bytes(HD);
-      const float2 sc = reinterpret_cast<const float2*>(blk + 2 * kKv8Page * HD)[slot];
-      const uint8_t* kp = blk + slot * HD + lane * PER;
-      float s = 0.f;
-#pragma unroll
-      for (int i = 0; i < PER; ++i) s = fmaf(qv[i], kv8_value<FMT>(kp[i]), s);
-      s = warp_sum(s) * sc.x * a.scale_log2;
-      const float mn = fmaxf(m, s), corr = exp2f(m - mn), p = exp2f(s - mn);
-      l = l * corr + p;
-#pragma unroll
-      for (int i = 0; i < PER; ++i) o[i] = o[i] * corr + p * (kv8_value<FMT>(kp[kKv8Page * HD + i]) * sc.y);
-      m = mn;
+      for (int o = 1; o < 32; o <<= 1) { const int v = __shfl_up_sync(0xffffffffu, incl, o); if (lane >= o) incl += v; }
+      total = __shfl_sync(0xffffffffu, incl, 31);
     }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const int src = __ffs(__ballot_sync(0xffffffffu, incl > item - base)) - 1;
+    int at = item - base - (__shfl_sync(0xffffffffu, incl, src) - __shfl_sync(0xffffffffu, mine, src));
+    const int tok0 = __shfl_sync(0xffffffffu, grp.tok0, src), cnt = __shfl_sync(0xffffffffu, grp.cnt, src);
+    const int first = __shfl_sync(0xffffffffu, grp.first, src), last = __shfl_sync(0xffffffffu, grp.last, src);
+    const int seq = __shfl_sync(0xffffffffu, grp.seq, src);
+    const int ctiles = (cnt * gq + COLS - 1) / COLS;
+    const int col0 = at % ctiles * COLS; at /= ctiles;
+    const int kvh = at % a.hkv, split = at / a.hkv;
+    const int k_begin = split * a.split_keys, k_end = min(last + 1, k_begin + a.split_keys);
+    const int n_pg = (k_end - k_begin + kKv8Page - 1) / kKv8Page;           // 0 for a group without keys
+    const int n_my = (n_pg - warp + kWarps - 1) / kWarps;
+
+    // this warp's page numbers, one to a lane (split_keys is at most 2048)
+    int my_page = -1;
+    if (lane < n_my) {
+      my_page = a.block_table[(size_t)seq * a.bt_ld + k_begin / kKv8Page + warp + kWarps * lane];
+      if (my_page < 0 || my_page >= a.n_pages) { atomicExch(a.status, (int)B2_ERR_BOUNDS); my_page = -1; }
+    }
+    __syncwarp();
+
+    uint4 kw[2][KC];
+    uint32_t vw[4][VW];
+    float4 sc;
+    auto block_of = [&](int i) {
+      const int p = __shfl_sync(0xffffffffu, my_page, i);
+      return a.pool + ((size_t)max(p, 0) * a.hkv + kvh) * kv8_block_bytes(HD);
+    };
+    auto load_k = [&](const uint8_t* blk) {        // keys 2g, 2g + 1: chunks t, t + 4 of their rows, and their scales
 #pragma unroll
-    for (int i = 0; i < PER; ++i) a.out[(size_t)tok * a.ldo + (size_t)head * HD + lane * PER + i] = __float2bfloat16_rn(o[i] * inv);
+      for (int r = 0; r < 2; ++r)
+#pragma unroll
+        for (int c = 0; c < KC; ++c) kw[r][c] = ld_nc_v4(blk + (2 * g + r) * HD + (t + 4 * c) * 16);
+      const uint4 u = ld_nc_v4(blk + 2 * kKv8Page * HD + g * 16);
+      sc = make_float4(__uint_as_float(u.x), __uint_as_float(u.y), __uint_as_float(u.z), __uint_as_float(u.w));
+    };
+    auto load_v = [&](const uint8_t* blk) {        // keys 4t .. 4t + 3: channels g * HD / 8 and on
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const uint8_t* p = blk + kKv8Page * HD + (4 * t + r) * HD + g * (HD / 8);
+        if constexpr (VW == 4) {
+          const uint4 u = ld_nc_v4(p);
+          vw[r][0] = u.x; vw[r][1] = u.y; vw[r][2] = u.z; vw[r][3] = u.w;
+        } else {
+          const uint2 u = ld_nc_v2(p);
+          vw[r][0] = u.x; vw[r][1] = u.y;
+        }
+      }
+    };
+    const uint8_t* blk = nullptr;
+    if (n_my > 0) { blk = block_of(0); load_k(blk); load_v(blk); }
+
+    // q as fp16, every column scaled by a power of two of its own so that its largest value lies in [2^10, 2^11): a bf16 number
+    // stays exact down to 2^-24 of that.  qs undoes it on the scores and brings the softmax scale.
+    uint32_t qb[NT][KS][2];
+    float qs[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int col = col0 + n * 8 + g;
+      const bool live = col < cnt * gq;
+      uint4 raw[KC][2];
+      uint32_t top = 0;
+#pragma unroll
+      for (int c = 0; c < KC; ++c)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          raw[c][h] = make_uint4(0u, 0u, 0u, 0u);
+          if (live) raw[c][h] = *reinterpret_cast<const uint4*>(a.q + (size_t)(tok0 + col / gq) * a.ldq + (size_t)(kvh * gq + col % gq) * HD + (t + 4 * c) * 16 + h * 8);
+          const uint32_t* w = &raw[c][h].x;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) top = max(top, max((w[i] & 0x7fffu) << 16, w[i] & 0x7fff0000u));
+        }
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      const uint32_t e = min(264u - (top >> 23), 253u);
+      const float up = __uint_as_float(e << 23), down = __uint_as_float((254u - e) << 23) * a.scale_log2;
+      qs[n][0] = __shfl_sync(0xffffffffu, down, 8 * t);
+      qs[n][1] = __shfl_sync(0xffffffffu, down, 8 * t + 4);
+#pragma unroll
+      for (int c = 0; c < KC; ++c)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {                // four channels of a K word
+          const uint32_t a0 = (&raw[c][w >> 1].x)[2 * (w & 1)], a1 = (&raw[c][w >> 1].x)[2 * (w & 1) + 1];
+          const float f0 = __uint_as_float(a0 << 16) * up, f1 = __uint_as_float(a0 & 0xffff0000u) * up;
+          const float f2 = __uint_as_float(a1 << 16) * up, f3 = __uint_as_float(a1 & 0xffff0000u) * up;
+          qb[n][c * 4 + w][0] = FMT == KV8_INT8 ? pack_half(f0, f2) : pack_half(f0, f1);
+          qb[n][c * 4 + w][1] = FMT == KV8_INT8 ? pack_half(f1, f3) : pack_half(f2, f3);
+        }
+    }
+
+    float o[NT][MT][4], m[NT][2], l[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      m[n][0] = m[n][1] = kNoRef; l[n][0] = l[n][1] = 0.f;
+#pragma unroll
+      for (int i = 0; i < MT; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
+    }
+
+    for (int i = 0; i < n_my; ++i) {
+      // s: keys 2g (0, 1) and 2g + 1 (2, 3), columns 2t (0, 2) and 2t + 1 (1, 3)
+      float s[NT][4];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+#pragma unroll
+      for (int c = 0; c < KC; ++c)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          uint32_t f[4];
+          row_pairs<FMT>((&kw[0][c].x)[w], f[0], f[2]);
+          row_pairs<FMT>((&kw[1][c].x)[w], f[1], f[3]);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) mma_f16_16816(s[n], f, qb[n][c * 4 + w][0], qb[n][c * 4 + w][1]);
+        }
+      const float4 scale = sc;
+      const bool there = __shfl_sync(0xffffffffu, my_page, i) >= 0;
+      const uint8_t* nxt = blk;
+      if (i + 1 < n_my) { nxt = block_of(i + 1); load_k(nxt); }
+
+      const float e0 = __uint_as_float(0x4b000000u | (__float_as_uint(scale.y) >> 23)) - 8388735.f;      // log2 of vs's power of two
+      const float e1 = __uint_as_float(0x4b000000u | (__float_as_uint(scale.w) >> 23)) - 8388735.f;
+      bool grows = false;
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[n][j] = __fmul_rn(__fmul_rn(s[n][j], j < 2 ? scale.x : scale.z), qs[n][j & 1]);
+      const int kb = k_begin + (warp + kWarps * i) * kKv8Page;
+      const bool partly = kb + kKv8Page > min(first, k_end) || !there;      // from the group's first slot on keys are looked at one by one
+      if (partly) {
+        const int end = there ? k_end : 0;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const int col = col0 + n * 8 + 2 * t + j, row = min(col / gq, cnt - 1);
+            const int pos = cnt == 1 ? last : min(a.tok_pos[tok0 + row], last);
+            const unsigned mask = a.tree_mask ? a.tree_mask[tok0 + row] : 0u;
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              const int key = kb + 2 * g + r, in = key - first;
+              const bool seen = key <= pos && key < end && (!a.tree_mask || in < 0 || (in < 32 && ((mask >> (in & 31)) & 1u)));
+              if (!seen) s[n][2 * r + j] = -INFINITY;
+            }
+          }
+        if (FMT == KV8_FP8) {          // bytes past the end may be e4m3's NaN, which a weight of zero does not silence
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (kb + 4 * t + r >= end)
+#pragma unroll
+              for (int w = 0; w < VW; ++w) vw[r][w] = 0u;
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) grows |= fmaxf(__fadd_rn(s[n][j], e0), __fadd_rn(s[n][2 + j], e1)) > __fadd_rn(m[n][j], kGrow);
+      if (__any_sync(0xffffffffu, grows)) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            float mx = fmaxf(__fadd_rn(s[n][j], e0), __fadd_rn(s[n][2 + j], e1));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+            if (mx > __fadd_rn(m[n][j], kGrow)) {
+              const float f = ex2(__fadd_rn(m[n][j], -mx));
+              m[n][j] = mx;
+              l[n][j] = __fmul_rn(l[n][j], f);
+#pragma unroll
+              for (int k = 0; k < MT; ++k) { o[n][k][j] = __fmul_rn(o[n][k][j], f); o[n][k][2 + j] = __fmul_rn(o[n][k][2 + j], f); }
+            }
+          }
+        __syncwarp();
+      }
+      const float v0 = scale.y * kDown, v1 = scale.w * kDown;
+      uint32_t pb[NT][2];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        float w[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float p = ex2(__fadd_rn(__fadd_rn(s[n][j], -m[n][j & 1]), kUp));
+          l[n][j & 1] = __fadd_rn(l[n][j & 1], p);
+          w[j] = __fmul_rn(p, j < 2 ? v0 : v1);
+          if (partly && s[n][j] == -INFINITY) w[j] = 0.f;       // a row that is not seen may have the scale NaN
+        }
+        pb[n][0] = transpose8x8(pack_half(w[0], w[1]));
+        pb[n][1] = transpose8x8(pack_half(w[2], w[3]));
+      }
+#pragma unroll
+      for (int w = 0; w < VW; ++w) {
+        uint32_t f[4];
+        cross_pairs<FMT, 0>(vw[0][w], vw[2][w], f[0], f[1]);
+        cross_pairs<FMT, 0>(vw[1][w], vw[3][w], f[2], f[3]);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) mma_f16_16816(o[n][2 * w], f, pb[n][0], pb[n][1]);
+        cross_pairs<FMT, 1>(vw[0][w], vw[2][w], f[0], f[1]);
+        cross_pairs<FMT, 1>(vw[1][w], vw[3][w], f[2], f[3]);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) mma_f16_16816(o[n][2 * w + 1], f, pb[n][0], pb[n][1]);
+      }
+      blk = nxt;
+      if (i + 1 < n_my) load_v(blk);
+    }
+
+    if (joined) __syncthreads();
+    joined = true;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        float x = l[n][j];
+        x = __fadd_rn(x, __shfl_xor_sync(0xffffffffu, x, 4));
+        x = __fadd_rn(x, __shfl_xor_sync(0xffffffffu, x, 8));
+        x = __fadd_rn(x, __shfl_xor_sync(0xffffffffu, x, 16));
+        const int c = n * 8 + 2 * t + j;
+        if (g == 0) { sh_m[warp][c] = m[n][j]; sh_l[warp][c] = __fmul_rn(x, kDown); }
+#pragma unroll
+        for (int k = 0; k < MT; k += 2)
+          *reinterpret_cast<float4*>(&sh_o[warp][c][g * (HD / 8) + 2 * k]) = make_float4(o[n][k][j], o[n][k][2 + j], o[n][k + 1][j], o[n][k + 1][2 + j]);
+      }
+    __syncthreads();
+    for (int i = threadIdx.x; i < COLS * (HD / 4); i += kWarps * 32) {
+      const int c = i / (HD / 4), d = i % (HD / 4) * 4, col = col0 + c;
+      if (col >= cnt * gq) continue;
+      const int tok = tok0 + col / gq, head = kvh * gq + col % gq;
+      const int ns = splits_of(cnt == 1 ? last : min(a.tok_pos[tok], last), a.split_keys);
+      if (split >= ns) continue;
+      float M = sh_m[0][c];
+#pragma unroll
+      for (int w = 1; w < kWarps; ++w) M = fmaxf(M, sh_m[w][c]);
+      float L = 0.f;
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const float f = ex2(__fadd_rn(sh_m[w][c], -M));
+        const float4 y = *reinterpret_cast<const float4*>(&sh_o[w][c][d]);
+        L = __fmaf_rn(sh_l[w][c], f, L);
+        x.x = __fmaf_rn(y.x, f, x.x); x.y = __fmaf_rn(y.y, f, x.y); x.z = __fmaf_rn(y.z, f, x.z); x.w = __fmaf_rn(y.w, f, x.w);
+      }
+      if (ns == 1) {
+        const float inv = L == 0.f ? 0.f : __fdiv_rn(1.f, L);
+        uint2 v;
+        *reinterpret_cast<__nv_bfloat162*>(&v.x) = __floats2bfloat162_rn(__fmul_rn(x.x, inv), __fmul_rn(x.y, inv));
+        *reinterpret_cast<__nv_bfloat162*>(&v.y) = __floats2bfloat162_rn(__fmul_rn(x.z, inv), __fmul_rn(x.w, inv));
+        *reinterpret_cast<uint2*>(a.out + (size_t)tok * a.ldo + (size_t)head * HD + d) = v;
+      } else {
+        const size_t slot = ((size_t)tok * a.hq + head) * a.max_splits + split;
+        *reinterpret_cast<float4*>(a.part_o + slot * HD + d) = x;
+        if (d == 0) *reinterpret_cast<float2*>(a.part_ml + slot * 2) = make_float2(M, L);
+      }
+    }
   }
+}
+
+// Joins the splits of rows that have more than one: a CTA per (group, row, q head), warp w adds the splits w, w + 4, ... in
+// order, the four sums are added in order of w.
+template <int HD>
+__global__ void __launch_bounds__(kWarps * 32) kv8_join_kernel(const Kv8AttnArgs a, int rows_at_once) {
+  constexpr int PER = HD / 32, AHEAD = 4;
+  __shared__ float sh[kWarps][HD + 1];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  pdl_wait();
+  pdl_launch_dependents();
+  const int head = blockIdx.x % a.hq, r0 = blockIdx.x / a.hq % rows_at_once;
+  const Group grp = group_at(a, blockIdx.x / a.hq / rows_at_once);
+  if (!grp.ok) return;
+  for (int r = r0; r < grp.cnt; r += rows_at_once) {
+    const int tok = grp.tok0 + r;
+    const int ns = splits_of(grp.cnt == 1 ? grp.last : min(a.tok_pos[tok], grp.last), a.split_keys);
+    if (ns == 1) continue;
+    const size_t slot = ((size_t)tok * a.hq + head) * a.max_splits;
+    const float* po = a.part_o + slot * HD + lane * PER;
+    const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + slot;
+    float M = kNoRef;
+    for (int s = lane; s < ns; s += 32) M = fmaxf(M, ml[s].x);
+    M = warp_max(M);
+    float L = 0.f, x[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) x[i] = 0.f;
+    for (int s0 = warp; s0 < ns; s0 += AHEAD * kWarps) {
+      float2 w[AHEAD];
+      float y[AHEAD][PER];
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j) {
+        const int s = s0 + j * kWarps;
+        w[j] = s < ns ? ml[s] : make_float2(kNoRef, 0.f);
+#pragma unroll
+        for (int i = 0; i < PER; ++i) y[j][i] = s < ns ? po[(size_t)s * HD + i] : 0.f;
+      }
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j) {
+        const float f = ex2(__fadd_rn(w[j].x, -M));
+        L = __fmaf_rn(w[j].y, f, L);
+#pragma unroll
+        for (int i = 0; i < PER; ++i) x[i] = __fmaf_rn(y[j][i], f, x[i]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < PER; ++i) sh[warp][lane * PER + i] = x[i];
+    if (lane == 0) sh[warp][HD] = L;
+    __syncthreads();
+    for (int d = threadIdx.x; d < HD; d += kWarps * 32) {
+      float sum = sh[0][d], Ls = sh[0][HD];
+#pragma unroll
+      for (int w = 1; w < kWarps; ++w) { sum = __fadd_rn(sum, sh[w][d]); Ls = __fadd_rn(Ls, sh[w][HD]); }
+      a.out[(size_t)tok * a.ldo + (size_t)head * HD + d] = __float2bfloat16_rn(Ls == 0.f ? 0.f : __fmul_rn(sum, __fdiv_rn(1.f, Ls)));
+    }
+    __syncthreads();
+  }
+}
+
+template <class K, class... A>
+cudaError_t launch(K kernel, unsigned blocks, cudaStream_t st, A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(blocks); cfg.blockDim = dim3(kWarps * 32); cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at; cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+template <int HD, int FMT>
+int run(const Kv8AttnArgs& a, cudaStream_t st) {
+  const long rows = ((long)a.n_tok + a.n_groups - 1) / a.n_groups;           // of a group, on average
+  const int gq = a.hq / a.hkv;
+  // columns of one item: eight where a group fills no more (a decode step of up to eight q heads per KV head), else sixteen,
+  // which halves the loads and conversions of K and V
+  const bool wide = rows * gq > 8;
+  const long items = (long)a.n_groups * a.hkv * a.max_splits * ((rows * gq + (wide ? 15 : 7)) / (wide ? 16 : 8));
+  const unsigned grid = (unsigned)std::min<long>(items, 148 * (wide ? 2 : 4));
+  cudaError_t e = wide ? launch(kv8_attn_kernel<HD, FMT, 2>, grid, st, a) : launch(kv8_attn_kernel<HD, FMT, 1>, grid, st, a);
+  if (e == cudaSuccess && a.max_splits > 1)
+    e = launch(kv8_join_kernel<HD>, (unsigned)(a.n_groups * rows * a.hq), st, a, (int)rows);
+  return e == cudaSuccess ? B2_OK : B2_ERR_LAUNCH;
 }
 
 }  // namespace
@@ -78,15 +492,10 @@ B2_API int b2_kv8_attn(const Kv8AttnArgs* args, int hd, int fmt, cudaStream_t st
   const Kv8AttnArgs& a = *args;
   if (a.n_groups < 1 || a.n_tok < 1 || a.hkv < 1 || a.hq < 1 || a.hq % a.hkv || a.n_seq < 1 || a.bt_cols < 1 || a.n_pages < 1) return B2_ERR_ARG;
   if ((hd != 64 && hd != 128) || (fmt != KV8_INT8 && fmt != KV8_FP8) || a.ldq % 8 || a.ldo % 8) return B2_ERR_ARG;
-  const long blocks = ((long)a.n_groups * a.hq + 3) / 4;
-  if (blocks > 0x7fffffffl || a.bt_cols > (1 << 26)) return B2_ERR_ARG;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)blocks); cfg.blockDim = dim3(128); cfg.stream = st;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = at; cfg.numAttrs = 1;
-  auto k = hd == 128 ? (fmt == KV8_INT8 ? kv8_attn_kernel<128, KV8_INT8> : kv8_attn_kernel<128, KV8_FP8>)
-                     : (fmt == KV8_INT8 ? kv8_attn_kernel<64, KV8_INT8> : kv8_attn_kernel<64, KV8_FP8>);
-  return cudaLaunchKernelEx(&cfg, k, a) == cudaSuccess ? B2_OK : B2_ERR_LAUNCH;
+  if (a.split_keys < kKv8Page || a.split_keys > 2048 || a.split_keys % kKv8Page || a.max_splits < 1) return B2_ERR_ARG;
+  if (a.max_splits > 1 && (!a.part_o || !a.part_ml)) return B2_ERR_ARG;
+  // item and block numbers are 32-bit
+  if (a.bt_cols > (1 << 26) || (long)a.n_groups * a.hq * 32 * a.max_splits > 0x7fff0000l || ((long)a.n_tok + a.n_groups) * a.hq > 0x7fffffffl) return B2_ERR_ARG;
+  if (hd == 128) return fmt == KV8_INT8 ? run<128, KV8_INT8>(a, st) : run<128, KV8_FP8>(a, st);
+  return fmt == KV8_INT8 ? run<64, KV8_INT8>(a, st) : run<64, KV8_FP8>(a, st);
 }

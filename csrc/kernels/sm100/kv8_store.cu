@@ -101,11 +101,12 @@ __global__ void __launch_bounds__(256) kv8_store_kernel(const Kv8StoreArgs a, in
     if (!live || head < a.hq || !stored) continue;
     const bool is_v = head >= a.hq + a.hkv;
     const int kvh = head - a.hq - (is_v ? a.hkv : 0), slot = pos % kKv8Page;
-    float scale = fmaxf(__fdiv_rn(__uint_as_float(mx), FMT == KV8_INT8 ? 127.f : 448.f), kKv8MinScale);
-    if (mx >= 0x7f800000u) scale = __uint_as_float(0x7fffffffu);
+    const float scale = fmaxf(__fdiv_rn(__uint_as_float(mx), FMT == KV8_INT8 ? 127.f : 448.f), kKv8MinScale);
+    const bool finite = mx < 0x7f800000u;
     uint32_t clo = 0, chi = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
+      if (!finite) lo[i] = hi[i] = 0.f;            // codes stay numbers: what tells of the row is its scale
       clo |= kv8_code<FMT>(__fdiv_rn(lo[i], scale)) << (8 * i);
       chi |= kv8_code<FMT>(__fdiv_rn(hi[i], scale)) << (8 * i);
     }
@@ -113,7 +114,7 @@ __global__ void __launch_bounds__(256) kv8_store_kernel(const Kv8StoreArgs a, in
     uint8_t* row = blk + (is_v ? kKv8Page * HD : 0) + slot * HD + l * 4;
     *reinterpret_cast<uint32_t*>(row) = clo;
     *reinterpret_cast<uint32_t*>(row + HALF) = chi;
-    if (l == 0) reinterpret_cast<float*>(blk + 2 * kKv8Page * HD)[slot * 2 + is_v] = scale;
+    if (l == 0) reinterpret_cast<float*>(blk + 2 * kKv8Page * HD)[slot * 2 + is_v] = finite ? scale : __uint_as_float(0x7fffffffu);
   }
 }
 

@@ -49,7 +49,10 @@ BAD_ATTN = [
     (dict(q=torch.zeros(3, HQ * HD + 4, dtype=torch.bfloat16)[:, :HQ * HD]), "boundaries"), (dict(out=torch.zeros(3, HQ * HD)), "out"),
     (dict(out=torch.zeros(2, HQ * HD, dtype=torch.bfloat16)), "out"), (dict(grp_cnt=torch.zeros(0, dtype=torch.int32)), "grp_cnt"),
     (dict(tok_pos=torch.zeros(2, dtype=torch.int32)), "tok_pos"), (dict(tree_mask=torch.zeros(3, dtype=torch.int64)), "tree_mask"),
-    (dict(tree_mask=torch.zeros(2, dtype=torch.int32)), "tree_mask"), (dict(block_table=torch.zeros(1, 4)), "block_table"), (dict(), "CUDA device"),
+    (dict(tree_mask=torch.zeros(2, dtype=torch.int32)), "tree_mask"), (dict(block_table=torch.zeros(1, 4)), "block_table"),
+    (dict(split_keys=40), "split_keys"), (dict(split_keys=4096), "split_keys"), (dict(split_keys=0), "split_keys"), (dict(max_ctx=65), "max_ctx"), (dict(max_ctx=0), "max_ctx"),
+    (dict(split_keys=16, part=torch.zeros(3 * HQ * 4 * (HD + 2) - 1)), "part"), (dict(part=torch.zeros(9999, dtype=torch.float64)), "part"),
+    (dict(split_keys=16, part=torch.zeros(3 * HQ * 4 * (HD + 2))), "CUDA device"), (dict(), "CUDA device"),
 ]
 
 
@@ -82,14 +85,21 @@ def test_the_library_refuses_what_the_launchers_would_not_pass_on():
         for k, v in kw.items():
             setattr(b, k, v)
         assert lib.b2_kv8_store(C.byref(b), hd, fmt, None) == 1
-    for hd, fmt, kw in ((32, 0, {}), (64, -1, {}), (64, 0, dict(hq=3, hkv=2)), (64, 0, dict(n_groups=0)), (64, 0, dict(ldq=4)), (64, 0, dict(bt_cols=0))):
-        b = _lib.Kv8AttnArgs(n_pages=1, bt_cols=1, n_seq=1, n_groups=1, n_tok=1, hq=1, hkv=1)
+    for hd, fmt, kw in ((32, 0, {}), (64, -1, {}), (64, 0, dict(hq=3, hkv=2)), (64, 0, dict(n_groups=0)), (64, 0, dict(ldq=4)), (64, 0, dict(bt_cols=0)),
+                        (64, 0, dict(split_keys=24)), (64, 0, dict(split_keys=4096)), (64, 0, dict(max_splits=0)), (64, 0, dict(max_splits=2)),
+                        (64, 0, dict(n_tok=2 ** 31 - 1)), (64, 0, dict(n_groups=2 ** 26))):
+        b = _lib.Kv8AttnArgs(n_pages=1, bt_cols=1, n_seq=1, n_groups=1, n_tok=1, hq=1, hkv=1, split_keys=256, max_splits=1)
         for k, v in kw.items():
             setattr(b, k, v)
         assert lib.b2_kv8_attn(C.byref(b), hd, fmt, None) == 1
     for bad in ((0, 1, 64, 0, 1, 0), (1, 0, 64, 0, 1, 0), (1, 1, 80, 0, 1, 0), (1, 1, 64, 5, 1, 0), (1, 1, 64, 0, 0, 0), (1, 1, 64, 0, 1, -1)):
         n_pages, hkv, hd, fmt, n_out, n_tok = bad
         assert lib.b2_kv8_read(None, n_pages, hkv, hd, fmt, None, n_out, n_tok, None, None, None) == 1
+
+
+def test_splits_for_a_context():
+    assert [K.split_keys_for(n) for n in (1, 256, 16384, 16385, 32769, 131072, 1 << 20)] == [256, 256, 256, 512, 1024, 2048, 2048]
+    assert K.part_floats(3, 8, 128, 256) == 0 and K.part_floats(3, 8, 128, 257) == 3 * 8 * 2 * 130 and K.part_floats(1, 2, 64, 100, 16) == 2 * 7 * 66
 
 
 @pytest.mark.parametrize("fmt", FMTS)

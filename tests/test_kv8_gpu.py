@@ -263,6 +263,57 @@ def test_attend_rows_without_keys_padding_and_strides():
         assert bool(((rows[t].view(hq, hd).double() - ref).abs() <= tol).all())
 
 
+@pytest.mark.parametrize("split", [16, 48, 64, 2048])
+def test_attend_split_sizes_and_a_workspace_of_the_caller(split):
+    """Any split gives the result within the bound; what lies in the workspace before or behind its part does not matter."""
+    hq, hkv, hd = 16, 2, 64
+    lens, new = [1, 47, 49, 1003], [1, 1, 2, 7]
+    c = Cache(lens, hkv, hd, "fp8", seed=split)
+    pos, seq, g0, gc = _groups(lens, new)
+    q = bf(torch.randn(len(pos), hq * hd))
+    need = K.part_floats(len(pos), hq, hd, c.bt.shape[1] * PAGE, split)
+    part = torch.full((need + 64,), float("nan"), device=DEV)
+    out = _attend(c, q, hq, pos, seq, g0, gc, split_keys=split, part=part)
+    _check_attend(c, q, hq, out, pos, seq, g0, gc)
+    assert bool(torch.isnan(part[need:]).all())
+    # groups in another order, one group a call, and more groups than a warp has lanes
+    order = [3, 1, 0, 2]
+    again = _attend(c, q, hq, pos, seq, [g0[i] for i in order], [gc[i] for i in order], split_keys=split)
+    assert torch.equal(again, out)
+    many = _attend(c, q, hq, pos, seq, g0 * 17 + list(range(len(pos))), gc * 17 + [1] * len(pos), split_keys=split)
+    assert torch.equal(many, out)
+
+
+def test_attend_refuses_positions_past_max_ctx():
+    hq, hkv, hd = 4, 2, 64
+    c = Cache([600, 600], hkv, hd, "int8")
+    q = bf(torch.randn(2, hq * hd)).to(DEV)
+    out = torch.full((2, hq * hd), 9.0, dtype=torch.bfloat16, device=DEV)
+    st = torch.zeros(1, dtype=torch.int32, device=DEV)
+    K.attn_decode8(q, c.pool.to(DEV), "int8", c.bt.to(DEV), i32([0, 1]), i32([1, 1]), i32([599, 255]), i32([0, 1]), hq, hkv, hd, split_keys=256, max_ctx=512,
+                   status=st, out=out)
+    assert int(st.item()) == 4 and bool((out[0] == 9).all())
+    k, v = c.rows(1)
+    ref, tol = attend(q[1].cpu().view(hq, hd), k, v, seen_keys(600, 255), hq, hkv)
+    assert bool(((out[1].cpu().view(hq, hd).double() - ref).abs() <= tol).all())
+
+
+def test_attend_rows_that_others_see_may_be_nan():
+    """A row of the group whose V is NaN: rows whose mask leaves it out do not notice."""
+    hq, hkv, hd = 8, 1, 64
+    for fmt in FMTS:
+        c = Cache([40], hkv, hd, fmt, seed=2)
+        fields(c.pool, hd)[2][int(c.bt[0, 2]), 0, 5, :] = float("nan")       # token 37
+        pos, seq, g0, gc = _groups([40], [4])                                  # rows 36 .. 39
+        q = bf(torch.randn(4, hq * hd))
+        out = _attend(c, q, hq, pos, seq, g0, gc, [1, 3, 5, 0b1010])
+        assert bool(torch.isfinite(out[[0, 2]]).all()) and bool(torch.isnan(out[[1, 3]]).all())
+        k, v = c.rows(0)
+        for t, m in ((0, 1), (2, 5)):
+            ref, tol = attend(q[t].view(hq, hd), k, v, seen_keys(40, pos[t], 36, m), hq, hkv)
+            assert bool(((out[t].view(hq, hd).double() - ref).abs() <= tol).all())
+
+
 @pytest.mark.parametrize("fmt", FMTS)
 def test_attend_scales_of_every_size(fmt):
     """V rows of very different sizes, a heavy key whose V is zero (it takes weight and adds nothing), tiny and huge V, large scores."""

@@ -11,15 +11,13 @@ What a kernel finds out of range (a page, a position past the block table) sets 
 """
 from __future__ import annotations
 
-import contextlib
-import ctypes as C
 import math
 from typing import Optional
 
 import torch
 
 from .. import _lib
-from .._lib import Kv8AttnArgs, Kv8StoreArgs, check, ptr
+from .._lib import Kv8AttnArgs, Kv8StoreArgs, check
 
 PAGE = 16
 FORMATS = {"int8": 0, "fp8": 1}
@@ -55,58 +53,87 @@ def part_floats(n_tok: int, hq: int, hd: int, max_ctx: int, split_keys: Optional
     return n_tok * hq * splits * (hd + 2) if splits > 1 else 0
 
 
+# Launches of a step follow one another every few microseconds, so the checks are written to cost little when they pass: one
+# expression per argument, the message made only when it fails.
+def _fail(what: str):
+    raise ValueError("8-bit KV cache: " + what)
+
+
 def _format(fmt: str) -> int:
-    try:
-        return FORMATS[fmt]
-    except (KeyError, TypeError):
-        raise ValueError(f"8-bit KV format: one of {', '.join(FORMATS)}, got {fmt!r}") from None
+    f = FORMATS.get(fmt) if type(fmt) is str else None
+    if f is None:
+        raise ValueError(f"8-bit KV format: one of {', '.join(FORMATS)}, got {fmt!r}")
+    return f
 
 
-def _need(ok: bool, what: str):
-    if not ok:
-        raise ValueError("8-bit KV cache: " + what)
+def _check_pool(pool: torch.Tensor, dev: int) -> int:
+    """Head size of a pool's pages."""
+    if not (pool.dtype is _U8 and pool.dim() == 3 and pool.is_contiguous() and pool.data_ptr() % 16 == 0):
+        _fail("the pool is a contiguous uint8 tensor [pages, hkv, 32 * hd + 128]")
+    pages, _, size = pool.shape
+    hd = _HD_OF.get(size)
+    if hd is None or pages == 0:
+        _fail(f"a pool of {tuple(pool.shape)} holds no pages of head_dim 64 or 128")
+    if pool.get_device() != dev:
+        _fail("all tensors on one device")
+    return hd
 
 
-def _check_pool(pool: torch.Tensor, dev, hkv: Optional[int] = None, hd: Optional[int] = None):
-    _need(pool.dtype is torch.uint8 and pool.dim() == 3 and pool.is_contiguous() and pool.data_ptr() % 16 == 0,
-          "the pool is a contiguous uint8 tensor [pages, hkv, 32 * hd + 128]")
-    got = (pool.shape[2] - 8 * PAGE) // (2 * PAGE)
-    _need(got in (64, 128) and pool.shape[2] == block_bytes(got) and pool.shape[0] > 0, f"a pool of {tuple(pool.shape)} holds no pages of head_dim 64 or 128")
-    _need((hkv is None or pool.shape[1] == hkv) and (hd is None or got == hd), f"the pool's pages are of {pool.shape[1]} KV heads of {got}")
-    _need(pool.device == dev, "all tensors on one device")
-    return got
+def _check_heads(pool: torch.Tensor, dev: int, hkv: int, hd: int):
+    got = _check_pool(pool, dev)
+    if got != hd or pool.shape[1] != hkv:
+        _fail(f"the pool's pages are of {pool.shape[1]} KV heads of {got}")
 
 
-def _check_index(t: Optional[torch.Tensor], n: int, dev, name: str):
-    if t is not None:
-        _need(t.dtype is torch.int32 and t.numel() >= n and t.is_contiguous() and t.device == dev, f"{name}: contiguous int32 with at least {n} entries on {dev}")
+def _check_index(t: torch.Tensor, n: int, dev: int, name: str) -> int:
+    if not (t.dtype is _I32 and t.numel() >= n and t.is_contiguous() and t.get_device() == dev):
+        _fail(f"{name}: contiguous int32 with at least {n} entries on the device of the rows")
+    return t.data_ptr()
 
 
-def _check_rows(t: torch.Tensor, n: int, width: int, dev, name: str, align: int):
-    _need(t.dtype is torch.bfloat16 and t.dim() == 2 and t.shape[0] == n and t.shape[1] == width and t.device == dev, f"{name}: bf16 [{n}, {width}] on {dev}")
-    _need((width == 1 or t.stride(1) == 1) and t.stride(0) % align == 0 and t.data_ptr() % (2 * align) == 0,
-          f"{name}: rows of unit stride that start on {2 * align}-byte boundaries")
+def _check_rows(t: torch.Tensor, n: int, width: int, dev: int, name: str, align: int) -> int:
+    """Distance of two rows of a bf16 [n, width] tensor."""
+    if not (t.dtype is _BF16 and t.shape == (n, width) and t.get_device() == dev):
+        _fail(f"{name}: bf16 [{n}, {width}] on the device of the rows")
+    if t.is_contiguous():
+        ld = width
+    else:
+        ld, unit = t.stride()
+        if unit != 1:
+            ld = 1
+    if ld % align or t.data_ptr() % (2 * align):
+        _fail(f"{name}: rows of unit stride that start on {2 * align}-byte boundaries")
+    return ld
 
 
-def _check_table(bt: torch.Tensor, dev):
-    _need(bt.dtype is torch.int32 and bt.dim() == 2 and bt.shape[1] > 0 and bt.stride(1) == 1 and bt.device == dev, f"block_table: int32 [sequences, pages] on {dev}")
+def _check_table(bt: torch.Tensor, dev: int):
+    """Sequences, pages of a sequence and distance of two rows of a block table."""
+    if not (bt.dtype is _I32 and bt.dim() == 2 and bt.get_device() == dev):
+        _fail("block_table: int32 [sequences, pages] on the device of the rows")
+    seqs, cols = bt.shape
+    ld, unit = (cols, 1) if bt.is_contiguous() else bt.stride()
+    if cols == 0 or unit != 1:
+        _fail("block_table: rows of unit stride, at least one page each")
+    return seqs, cols, ld
 
 
-_HERE = contextlib.nullcontext()
+_BF16, _I32, _U8, _F32 = torch.bfloat16, torch.int32, torch.uint8, torch.float32
+_LOG2E = math.log2(math.e)
+_HD_OF = {block_bytes(hd): hd for hd in (64, 128)}
 
 
-def _on(dev):
-    """Makes the tensors' device the current one for the launch."""
-    if dev.type != "cuda":
-        raise ValueError("8-bit KV cache: tensors on a CUDA device")
-    return _HERE if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
-
-
-def _status(status: Optional[torch.Tensor], dev) -> torch.Tensor:
-    if status is None:
-        return torch.zeros(1, dtype=torch.int32, device=dev)
-    _check_index(status, 1, dev, "status")
-    return status
+def _launch(name: str, dev: int, *args):
+    """Calls an entry of the library with the current stream of the tensors' device appended."""
+    if dev < 0:
+        _fail("tensors on a CUDA device")
+    fn = getattr(_lib.cuda_lib(), name)
+    if torch.cuda.current_device() == dev:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    if rc:
+        check(rc, name)
 
 
 def rope_kvstore8(qkv: torch.Tensor, hq: int, hkv: int, hd: int, inv_freq: torch.Tensor, tok_pos: torch.Tensor, tok_seq: torch.Tensor,
@@ -117,30 +144,33 @@ def rope_kvstore8(qkv: torch.Tensor, hq: int, hkv: int, hd: int, inv_freq: torch
     quantises k and v into slot ``tok_pos[i]`` of sequence ``tok_seq[i]``.  The 8-bit form of ``basic.rope_kvstore`` and, with
     ``rope_pos3`` (int32 ``[3, n]``) and ``pair_axis`` (uint8 ``[hd / 2]``), of ``basic.rope_kvstore_m``; angles are taken in
     64 bits.  Two rows of a call must not name the same slot.  Returns the status word."""
-    f, dev = _format(fmt), qkv.device
+    f, dev = _format(fmt), qkv.get_device()
     n = qkv.shape[0]
-    _need(hq > 0 and hkv > 0, "hq and hkv are positive")
-    _check_pool(pool, dev, hkv, hd)
-    _check_rows(qkv, n, (hq + 2 * hkv) * hd, dev, "qkv", 4)
-    _check_rows(q_out, n, hq * hd, dev, "q_out", 4)
-    _check_table(block_table, dev)
-    for t, name in ((tok_pos, "tok_pos"), (tok_seq, "tok_seq"), (rope_pos, "rope_pos")):
-        _check_index(t, n, dev, name)
-    _need(inv_freq.dtype is torch.float32 and inv_freq.numel() == hd // 2 and inv_freq.is_contiguous() and inv_freq.device == dev
-          and inv_freq.data_ptr() % 16 == 0, f"inv_freq: fp32 [{hd // 2}]")
+    if hq < 1 or hkv < 1:
+        _fail("hq and hkv are positive")
+    _check_heads(pool, dev, hkv, hd)
+    ld = _check_rows(qkv, n, (hq + 2 * hkv) * hd, dev, "qkv", 4)
+    ldq = _check_rows(q_out, n, hq * hd, dev, "q_out", 4)
+    seqs, cols, bt_ld = _check_table(block_table, dev)
+    at_pos, at_seq = _check_index(tok_pos, n, dev, "tok_pos"), _check_index(tok_seq, n, dev, "tok_seq")
+    at_rope = 0 if rope_pos is None else _check_index(rope_pos, n, dev, "rope_pos")
+    if not (inv_freq.dtype is _F32 and inv_freq.numel() == hd // 2 and inv_freq.is_contiguous() and inv_freq.get_device() == dev
+            and inv_freq.data_ptr() % 16 == 0):
+        _fail(f"inv_freq: contiguous fp32 [{hd // 2}] on the device of the rows")
+    at_rope3 = at_axis = 0
     if rope_pos3 is not None:
-        _need(pair_axis is not None and pair_axis.dtype is torch.uint8 and pair_axis.numel() == hd // 2 and pair_axis.is_contiguous() and pair_axis.device == dev,
-              f"rope_pos3 goes with pair_axis, uint8 [{hd // 2}]")
-        _need(tuple(rope_pos3.shape) == (3, n) and rope_pos is None, f"rope_pos3: int32 [3, {n}], without rope_pos")
-        _check_index(rope_pos3, 3 * n, dev, "rope_pos3")
-    status = _status(status, dev)
-    if n == 0:
-        return status
-    a = Kv8StoreArgs(ptr(qkv), qkv.stride(0), n, hq, hkv, ptr(inv_freq), ptr(tok_pos), ptr(rope_pos), ptr(rope_pos3), ptr(pair_axis), ptr(tok_seq),
-                     block_table.shape[0], ptr(block_table), block_table.stride(0), block_table.shape[1], ptr(pool), pool.shape[0], ptr(q_out),
-                     q_out.stride(0), ptr(status))
-    with _on(dev):
-        check(_lib.cuda_lib().b2_kv8_store(C.byref(a), hd, f, torch.cuda.current_stream().cuda_stream), "b2_kv8_store")
+        if pair_axis is None or not (pair_axis.dtype is _U8 and pair_axis.numel() == hd // 2 and pair_axis.is_contiguous() and pair_axis.get_device() == dev):
+            _fail(f"rope_pos3 goes with pair_axis, uint8 [{hd // 2}]")
+        if rope_pos3.shape != (3, n) or rope_pos is not None:
+            _fail(f"rope_pos3: int32 [3, {n}], without rope_pos")
+        at_rope3, at_axis = _check_index(rope_pos3, 3 * n, dev, "rope_pos3"), pair_axis.data_ptr()
+    if status is None:
+        status = torch.zeros(1, dtype=_I32, device=qkv.device)
+    at_status = _check_index(status, 1, dev, "status")
+    if n:
+        a = Kv8StoreArgs(qkv.data_ptr(), ld, n, hq, hkv, inv_freq.data_ptr(), at_pos, at_rope, at_rope3, at_axis, at_seq, seqs, block_table.data_ptr(), bt_ld,
+                         cols, pool.data_ptr(), pool.shape[0], q_out.data_ptr(), ldq, at_status)
+        _launch("b2_kv8_store", dev, a, hd, f)
     return status
 
 
@@ -158,39 +188,44 @@ def attn_decode8(q: torch.Tensor, pool: torch.Tensor, fmt: str, block_table: tor
     splits that are joined at the end; a row's bits depend on its own position and on ``split_keys`` only.  ``max_ctx`` (default:
     the table's length) bounds the positions, ``part`` is a workspace of :func:`part_floats` entries (default: allocated for the
     call).  Returns bf16 ``[n_tok, hq * hd]``."""
-    f, dev = _format(fmt), q.device
+    f, dev = _format(fmt), q.get_device()
     n = q.shape[0]
-    _need(hq > 0 and hkv > 0 and hq % hkv == 0, "hq is a multiple of hkv")
-    _check_pool(pool, dev, hkv, hd)
-    _check_rows(q, n, hq * hd, dev, "q", 8)
-    _check_table(block_table, dev)
+    if hkv < 1 or hq < 1 or hq % hkv:
+        _fail("hq is a multiple of hkv")
+    _check_heads(pool, dev, hkv, hd)
+    ldq = _check_rows(q, n, hq * hd, dev, "q", 8)
+    seqs, cols, bt_ld = _check_table(block_table, dev)
     n_groups = grp_tok0.numel()
-    for t, m, name in ((grp_tok0, n_groups, "grp_tok0"), (grp_cnt, n_groups, "grp_cnt"), (tok_pos, n, "tok_pos"), (tok_seq, n, "tok_seq"), (tree_mask, n, "tree_mask")):
-        _check_index(t, m, dev, name)
+    at_tok0, at_cnt = _check_index(grp_tok0, n_groups, dev, "grp_tok0"), _check_index(grp_cnt, n_groups, dev, "grp_cnt")
+    at_pos, at_seq = _check_index(tok_pos, n, dev, "tok_pos"), _check_index(tok_seq, n, dev, "tok_seq")
+    at_mask = 0 if tree_mask is None else _check_index(tree_mask, n, dev, "tree_mask")
     if out is None:
-        out = torch.empty(n, hq * hd, dtype=torch.bfloat16, device=dev)
+        out, ldo = torch.empty(n, hq * hd, dtype=_BF16, device=q.device), hq * hd
     else:
-        _check_rows(out, n, hq * hd, dev, "out", 8)
-    max_ctx = block_table.shape[1] * PAGE if max_ctx is None else int(max_ctx)
-    _need(0 < max_ctx <= block_table.shape[1] * PAGE, f"max_ctx: 1 .. {block_table.shape[1] * PAGE}, what the block table holds")
-    split_keys = split_keys_for(max_ctx) if split_keys is None else int(split_keys)
-    _need(PAGE <= split_keys <= MAX_SPLIT and split_keys % PAGE == 0, f"split_keys: a multiple of {PAGE} up to {MAX_SPLIT}")
+        ldo = _check_rows(out, n, hq * hd, dev, "out", 8)
+    if max_ctx is None:
+        max_ctx = cols * PAGE
+    elif not 0 < max_ctx <= cols * PAGE:
+        _fail(f"max_ctx: 1 .. {cols * PAGE}, what the block table holds")
+    if split_keys is None:
+        split_keys = split_keys_for(max_ctx)
+    elif not PAGE <= split_keys <= MAX_SPLIT or split_keys % PAGE:
+        _fail(f"split_keys: a multiple of {PAGE} up to {MAX_SPLIT}")
     splits = -(-max_ctx // split_keys)
     slots = n * hq * splits if splits > 1 else 0
-    if part is not None:
-        _need(part.dtype is torch.float32 and part.is_contiguous() and part.numel() >= slots * (hd + 2) and part.device == dev and part.data_ptr() % 16 == 0,
-              f"part: contiguous fp32 with at least {slots * (hd + 2)} entries on {dev}")
-    status = _status(status, dev)
-    if n == 0 or n_groups == 0:
-        return out
-    if part is None and slots:
-        part = torch.empty(slots * (hd + 2), dtype=torch.float32, device=dev)
-    at = ptr(part)
-    a = Kv8AttnArgs(ptr(q), q.stride(0), ptr(pool), pool.shape[0], ptr(block_table), block_table.stride(0), block_table.shape[1], block_table.shape[0],
-                    ptr(grp_tok0), ptr(grp_cnt), n_groups, ptr(tok_pos), ptr(tok_seq), n, ptr(tree_mask), hq, hkv,
-                    math.log2(math.e) / math.sqrt(hd), ptr(out), out.stride(0), ptr(status), split_keys, splits, at, at + 4 * slots * hd)
-    with _on(dev):
-        check(_lib.cuda_lib().b2_kv8_attn(C.byref(a), hd, f, torch.cuda.current_stream().cuda_stream), "b2_kv8_attn")
+    if part is not None and not (part.dtype is _F32 and part.is_contiguous() and part.numel() >= slots * (hd + 2) and part.get_device() == dev
+                                 and part.data_ptr() % 16 == 0):
+        _fail(f"part: contiguous fp32 with at least {slots * (hd + 2)} entries on the device of the rows")
+    if status is None:
+        status = torch.zeros(1, dtype=_I32, device=q.device)
+    at_status = _check_index(status, 1, dev, "status")
+    if n and n_groups:
+        if part is None and slots:
+            part = torch.empty(slots * (hd + 2), dtype=_F32, device=q.device)
+        at_o = part.data_ptr() if slots else 0
+        a = Kv8AttnArgs(q.data_ptr(), ldq, pool.data_ptr(), pool.shape[0], block_table.data_ptr(), bt_ld, cols, seqs, at_tok0, at_cnt, n_groups, at_pos, at_seq, n,
+                        at_mask, hq, hkv, _LOG2E / math.sqrt(hd), out.data_ptr(), ldo, at_status, split_keys, splits, at_o, at_o + 4 * slots * hd)
+        _launch("b2_kv8_attn", dev, a, hd, f)
     return out
 
 
@@ -198,21 +233,21 @@ def kv_read8(pool: torch.Tensor, fmt: str, pages: torch.Tensor, n_tokens: Option
              status: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The named pages (int32 ``[n]``, a row of a block table or any list) as bf16 pages ``[n, 2, hkv, 16, hd]``, the layout of the
     bf16 pool.  Slots from ``n_tokens`` on (counted over the list) are zeros and are not read; default: every slot."""
-    f, dev = _format(fmt), pool.device
+    f, dev = _format(fmt), pool.get_device()
     hd = _check_pool(pool, dev)
     n, hkv = pages.numel(), pool.shape[1]
-    _check_index(pages, n, dev, "pages")
-    n_tokens = n * PAGE if n_tokens is None else int(n_tokens)
-    _need(0 <= n_tokens <= n * PAGE, f"n_tokens: 0 .. {n * PAGE}")
-    shape = (n, 2, hkv, PAGE, hd)
+    at_pages = _check_index(pages, n, dev, "pages")
+    if n_tokens is None:
+        n_tokens = n * PAGE
+    elif not 0 <= n_tokens <= n * PAGE:
+        _fail(f"n_tokens: 0 .. {n * PAGE}")
     if out is None:
-        out = torch.empty(shape, dtype=torch.bfloat16, device=dev)
-    else:
-        _need(out.dtype is torch.bfloat16 and tuple(out.shape) == shape and out.is_contiguous() and out.device == dev and out.data_ptr() % 16 == 0, f"out: contiguous bf16 {list(shape)}")
-    status = _status(status, dev)
-    if n == 0:
-        return out
-    with _on(dev):
-        check(_lib.cuda_lib().b2_kv8_read(ptr(pool), pool.shape[0], hkv, hd, f, ptr(pages), n, n_tokens, ptr(out), ptr(status),
-                                          torch.cuda.current_stream().cuda_stream), "b2_kv8_read")
+        out = torch.empty(n, 2, hkv, PAGE, hd, dtype=_BF16, device=pool.device)
+    elif not (out.dtype is _BF16 and out.shape == (n, 2, hkv, PAGE, hd) and out.is_contiguous() and out.get_device() == dev and out.data_ptr() % 16 == 0):
+        _fail(f"out: contiguous bf16 {[n, 2, hkv, PAGE, hd]} on the device of the pool")
+    if status is None:
+        status = torch.zeros(1, dtype=_I32, device=pool.device)
+    at_status = _check_index(status, 1, dev, "status")
+    if n:
+        _launch("b2_kv8_read", dev, pool.data_ptr(), pool.shape[0], hkv, hd, f, at_pages, n, n_tokens, out.data_ptr(), at_status)
     return out

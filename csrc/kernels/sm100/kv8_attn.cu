@@ -47,6 +47,7 @@ struct Kv8AttnArgs {
 namespace {
 
 constexpr int kWarps = 4;
+constexpr int kStages = 3;                  // pages that a warp has in shared memory or under way
 constexpr float kNoRef = -3.4028234e38f;    // m before the first key
 constexpr float kGrow = 8.f;                // log2 of what a column may grow before m follows
 // l sums 2^(s - m) * 2^30 and the weights carry vs * 2^-30: with V of any size between 2^-64 and 2^121 neither leaves fp32
@@ -97,6 +98,22 @@ __device__ __forceinline__ void cross_pairs(uint32_t wa, uint32_t wb, uint32_t& 
   }
 }
 
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ uint4 lds128(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint2 lds64(uint32_t addr) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr) : "memory");
+  return v;
+}
+
 struct Group { int tok0, cnt, first, last, seq; bool ok; };
 
 // A group and whether everything it names is there; `last` is the last slot that its rows may see.
@@ -114,30 +131,80 @@ __device__ __forceinline__ Group group_at(const Kv8AttnArgs& a, int g) {
 }
 __device__ __forceinline__ int splits_of(int last_key, int split_keys) { return last_key < 0 ? 1 : last_key / split_keys + 1; }
 
+// Copies of blocks into the ring and where a lane finds its bytes there.  A block is looked at as 128-byte lines (one row of 128
+// channels, two of 64); the 16-byte pieces of a line are permuted so that the eight lanes of a load's phase hit different banks:
+// for K these are two rows times four neighbouring pieces, for V four rows times two.
+template <int HD>
+struct Ring {
+  static constexpr int kSlab = kKv8Page * HD;
+  uint32_t src, dst_k, dst_v[kSlab / 512];           // a lane's copies: 512 bytes a turn
+  uint32_t rd_k, rd_v;
+  __device__ __forceinline__ Ring(int lane) {
+    const int g = lane >> 2, t = lane & 3, l4 = lane >> 3, c = lane & 7;
+    src = lane * 16;
+    // lines 4k + l4: K by the line's parity in units of two rows, V by fours of rows
+    dst_k = l4 * 128 + ((c ^ ((HD == 128 ? l4 >> 1 : l4) & 1) * 4) << 4);
+#pragma unroll
+    for (int k = 0; k < kSlab / 512; ++k) dst_v[k] = kSlab + (4 * k + l4) * 128 + ((c ^ ((HD == 128 ? k : 2 * k + (l4 >> 1)) * 2)) << 4);
+    rd_k = HD == 128 ? 2 * g * 128 + ((t ^ (g & 1) * 4) << 4) : g * 128 + ((t ^ (g & 1) * 4) << 4);
+    rd_v = kSlab + (HD == 128 ? 4 * t * 128 + ((g ^ t * 2) << 4) : 2 * t * 128 + (((g >> 1) ^ t * 2) << 4) + (g & 1) * 8);
+  }
+  __device__ __forceinline__ void copy(uint32_t stage, const uint8_t* blk, int lane) const {
+#pragma unroll
+    for (int k = 0; k < kSlab / 512; ++k) {
+      cp_async16(stage + dst_k + k * 512, blk + src + k * 512);
+      cp_async16(stage + dst_v[k], blk + kSlab + src + k * 512);
+    }
+    if (lane < 8) cp_async16(stage + 2 * kSlab + src, blk + 2 * kSlab + src);
+  }
+  __device__ __forceinline__ uint4 k(uint32_t stage, int r, int c) const {      // row 2g + r, piece t + 4c
+    if (HD == 128) return lds128(stage + ((rd_k + r * 128) ^ (c * 64)));
+    return lds128(stage + (rd_k ^ (r * 64)));
+  }
+  __device__ __forceinline__ void v(uint32_t stage, int r, uint32_t (&w)[HD / 32]) const {     // row 4t + r, channels g * HD / 8 and on
+    if constexpr (HD == 128) {
+      const uint4 u = lds128(stage + rd_v + r * 128);
+      w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
+    } else {
+      const uint2 u = lds64(stage + ((rd_v + (r >> 1) * 128) ^ ((r & 1) * 64)));
+      w[0] = u.x; w[1] = u.y;
+    }
+  }
+};
+
+struct Item { int tok0, cnt, first, last, col0, kvh, split, n_my, page; };      // page: lane i's page i of this warp
+
+template <int HD, int NT>
+constexpr size_t attn_smem() { return (size_t)kWarps * (kStages * kv8_block_bytes(HD) + NT * 8 * (HD + 4) * 4 + 2 * NT * 8 * 4); }
+
 template <int HD, int FMT, int NT>
-__global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 2) kv8_attn_kernel(const Kv8AttnArgs a) {
+__global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_attn_kernel(const Kv8AttnArgs a) {
   constexpr int KC = HD / 64;            // 16-byte chunks of a K row per lane
   constexpr int KS = HD / 16;            // k-steps of K q^T
   constexpr int VW = HD / 32;            // words of a V row per lane
   constexpr int MT = HD / 16;            // channel tiles of V^T p^T
   constexpr int COLS = NT * 8;
   constexpr int LDO = HD + 4;
-  __shared__ __align__(16) float sh_o[kWarps][COLS][LDO];
-  __shared__ float sh_m[kWarps][COLS], sh_l[kWarps][COLS];
+  constexpr int BLK = kv8_block_bytes(HD);
+  extern __shared__ __align__(128) uint8_t smem[];
+  float (*sh_o)[COLS][LDO] = reinterpret_cast<float (*)[COLS][LDO]>(smem + kWarps * kStages * BLK);
+  float (*sh_m)[COLS] = reinterpret_cast<float (*)[COLS]>(sh_o + kWarps);
+  float (*sh_l)[COLS] = sh_m + kWarps;
   pdl_wait();
   pdl_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int gq = a.hq / a.hkv;
+  const Ring<HD> ring(lane);
+  const uint32_t mem = smem_u32(smem) + warp * kStages * BLK;
 
   // Items are numbered group after group; every lane holds one group of a run of 32 and the sum of items up to it.
   int run = -32, base = 0, total = 0, incl = 0, mine = 0;
   Group grp = {0, 0, 0, -1, 0, true};
-  bool joined = false;                   // shared memory of the item before may still be read
-  for (int item = blockIdx.x;; item += gridDim.x) {
+  auto fetch = [&](int item, Item& it) -> bool {
     while (item - base >= total) {
       base += total;
       run += 32;
-      if (run >= a.n_groups) return;
+      if (run >= a.n_groups) return false;
       grp = group_at(a, run + lane);
       if (!grp.ok && blockIdx.x == 0 && warp == 0) atomicExch(a.status, (int)B2_ERR_BOUNDS);
       mine = grp.ok && grp.cnt > 0 ? splits_of(grp.last, a.split_keys) * a.hkv * ((grp.cnt * gq + COLS - 1) / COLS) : 0;
@@ -148,54 +215,48 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 2) kv8_attn_kernel(
     }
     const int src = __ffs(__ballot_sync(0xffffffffu, incl > item - base)) - 1;
     int at = item - base - (__shfl_sync(0xffffffffu, incl, src) - __shfl_sync(0xffffffffu, mine, src));
-    const int tok0 = __shfl_sync(0xffffffffu, grp.tok0, src), cnt = __shfl_sync(0xffffffffu, grp.cnt, src);
-    const int first = __shfl_sync(0xffffffffu, grp.first, src), last = __shfl_sync(0xffffffffu, grp.last, src);
+    it.tok0 = __shfl_sync(0xffffffffu, grp.tok0, src); it.cnt = __shfl_sync(0xffffffffu, grp.cnt, src);
+    it.first = __shfl_sync(0xffffffffu, grp.first, src); it.last = __shfl_sync(0xffffffffu, grp.last, src);
     const int seq = __shfl_sync(0xffffffffu, grp.seq, src);
-    const int ctiles = (cnt * gq + COLS - 1) / COLS;
-    const int col0 = at % ctiles * COLS; at /= ctiles;
-    const int kvh = at % a.hkv, split = at / a.hkv;
-    const int k_begin = split * a.split_keys, k_end = min(last + 1, k_begin + a.split_keys);
+    const int ctiles = (it.cnt * gq + COLS - 1) / COLS;
+    it.col0 = at % ctiles * COLS; at /= ctiles;
+    it.kvh = at % a.hkv; it.split = at / a.hkv;
+    const int k_begin = it.split * a.split_keys, k_end = min(it.last + 1, k_begin + a.split_keys);
     const int n_pg = (k_end - k_begin + kKv8Page - 1) / kKv8Page;           // 0 for a group without keys
-    const int n_my = (n_pg - warp + kWarps - 1) / kWarps;
-
-    // this warp's page numbers, one to a lane (split_keys is at most 2048)
-    int my_page = -1;
-    if (lane < n_my) {
-      my_page = a.block_table[(size_t)seq * a.bt_ld + k_begin / kKv8Page + warp + kWarps * lane];
-      if (my_page < 0 || my_page >= a.n_pages) { atomicExch(a.status, (int)B2_ERR_BOUNDS); my_page = -1; }
-    }
+    it.n_my = (n_pg - warp + kWarps - 1) / kWarps;                          // at most 32: split_keys is at most 2048
+    it.page = -1;
+    if (lane < it.n_my) it.page = a.block_table[(size_t)seq * a.bt_ld + k_begin / kKv8Page + warp + kWarps * lane];
     __syncwarp();
-
-    uint4 kw[2][KC];
-    uint32_t vw[4][VW];
-    float4 sc;
-    auto block_of = [&](int i) {
-      const int p = __shfl_sync(0xffffffffu, my_page, i);
-      return a.pool + ((size_t)max(p, 0) * a.hkv + kvh) * kv8_block_bytes(HD);
-    };
-    auto load_k = [&](const uint8_t* blk) {        // keys 2g, 2g + 1: chunks t, t + 4 of their rows, and their scales
-#pragma unroll
-      for (int r = 0; r < 2; ++r)
-#pragma unroll
-        for (int c = 0; c < KC; ++c) kw[r][c] = ld_nc_v4(blk + (2 * g + r) * HD + (t + 4 * c) * 16);
-      const uint4 u = ld_nc_v4(blk + 2 * kKv8Page * HD + g * 16);
-      sc = make_float4(__uint_as_float(u.x), __uint_as_float(u.y), __uint_as_float(u.z), __uint_as_float(u.w));
-    };
-    auto load_v = [&](const uint8_t* blk) {        // keys 4t .. 4t + 3: channels g * HD / 8 and on
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const uint8_t* p = blk + kKv8Page * HD + (4 * t + r) * HD + g * (HD / 8);
-        if constexpr (VW == 4) {
-          const uint4 u = ld_nc_v4(p);
-          vw[r][0] = u.x; vw[r][1] = u.y; vw[r][2] = u.z; vw[r][3] = u.w;
-        } else {
-          const uint2 u = ld_nc_v2(p);
-          vw[r][0] = u.x; vw[r][1] = u.y;
+    return true;
+  };
+  Item cur, nxt;
+  bool more = fetch(blockIdx.x, nxt);
+  // pages that this warp has sent for and has used; where it fetches (cur or nxt) and which page comes next
+  int made = 0, used = 0, at_page = 0;
+  bool ahead = false, joined = false;
+  for (int item = blockIdx.x; more; item += gridDim.x) {
+    cur = nxt;
+    at_page = ahead ? at_page : 0;
+    ahead = false;
+    more = fetch(item + gridDim.x, nxt);
+    const int tok0 = cur.tok0, cnt = cur.cnt, first = cur.first, last = cur.last, col0 = cur.col0, kvh = cur.kvh, split = cur.split, n_my = cur.n_my;
+    const int k_begin = split * a.split_keys, k_end = min(last + 1, k_begin + a.split_keys);
+    auto top_up = [&]() {
+      while (made - used < kStages) {
+        if (!ahead && at_page >= n_my) { ahead = true; at_page = 0; }
+        if (ahead && (!more || at_page >= nxt.n_my)) return;
+        int p = __shfl_sync(0xffffffffu, ahead ? nxt.page : cur.page, at_page);
+        if (p < 0 || p >= a.n_pages) {               // its keys are masked below; something there is copied in their place
+          if (lane == 0) atomicExch(a.status, (int)B2_ERR_BOUNDS);
+          p = 0;
         }
+        ring.copy(mem + made % kStages * BLK, a.pool + ((size_t)p * a.hkv + (ahead ? nxt.kvh : kvh)) * BLK, lane);
+        cp_async_commit();
+        ++made;
+        ++at_page;
       }
     };
-    const uint8_t* blk = nullptr;
-    if (n_my > 0) { blk = block_of(0); load_k(blk); load_v(blk); }
+    top_up();
 
     // q as fp16, every column scaled by a power of two of its own so that its largest value lies in [2^10, 2^11): a bf16 number
     // stays exact down to 2^-24 of that.  qs undoes it on the scores and brings the softmax scale.
@@ -244,24 +305,30 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 2) kv8_attn_kernel(
     }
 
     for (int i = 0; i < n_my; ++i) {
+      // this page has arrived once no more copies are under way than were sent for after it
+      if (made - used >= 3) cp_async_wait<2>(); else if (made - used == 2) cp_async_wait<1>(); else cp_async_wait<0>();
+      __syncwarp();
+      const uint32_t stage = mem + used % kStages * BLK;
       // s: keys 2g (0, 1) and 2g + 1 (2, 3), columns 2t (0, 2) and 2t + 1 (1, 3)
       float s[NT][4];
 #pragma unroll
       for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
 #pragma unroll
-      for (int c = 0; c < KC; ++c)
+      for (int c = 0; c < KC; ++c) {
+        const uint4 k0 = ring.k(stage, 0, c), k1 = ring.k(stage, 1, c);
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
           uint32_t f[4];
-          row_pairs<FMT>((&kw[0][c].x)[w], f[0], f[2]);
-          row_pairs<FMT>((&kw[1][c].x)[w], f[1], f[3]);
+          row_pairs<FMT>((&k0.x)[w], f[0], f[2]);
+          row_pairs<FMT>((&k1.x)[w], f[1], f[3]);
 #pragma unroll
           for (int n = 0; n < NT; ++n) mma_f16_16816(s[n], f, qb[n][c * 4 + w][0], qb[n][c * 4 + w][1]);
         }
-      const float4 scale = sc;
-      const bool there = __shfl_sync(0xffffffffu, my_page, i) >= 0;
-      const uint8_t* nxt = blk;
-      if (i + 1 < n_my) { nxt = block_of(i + 1); load_k(nxt); }
+      }
+      uint4 su = lds128(stage + 2 * kKv8Page * HD + g * 16);        // K and V scales of keys 2g, 2g + 1
+      const float4 scale = make_float4(__uint_as_float(su.x), __uint_as_float(su.y), __uint_as_float(su.z), __uint_as_float(su.w));
+      const int page = __shfl_sync(0xffffffffu, cur.page, i);
+      const bool there = page >= 0 && page < a.n_pages;
 
       const float e0 = __uint_as_float(0x4b000000u | (__float_as_uint(scale.y) >> 23)) - 8388735.f;      // log2 of vs's power of two
       const float e1 = __uint_as_float(0x4b000000u | (__float_as_uint(scale.w) >> 23)) - 8388735.f;
@@ -288,13 +355,6 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 2) kv8_attn_kernel(
               if (!seen) s[n][2 * r + j] = -INFINITY;
             }
           }
-        if (FMT == KV8_FP8) {          // bytes past the end may be e4m3's NaN, which a weight of zero does not silence
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (kb + 4 * t + r >= end)
-#pragma unroll
-              for (int w = 0; w < VW; ++w) vw[r][w] = 0u;
-        }
       }
 #pragma unroll
       for (int n = 0; n < NT; ++n)
@@ -334,6 +394,18 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 2) kv8_attn_kernel(
         pb[n][0] = transpose8x8(pack_half(w[0], w[1]));
         pb[n][1] = transpose8x8(pack_half(w[2], w[3]));
       }
+      uint32_t vw[4][VW];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        ring.v(stage, r, vw[r]);
+        // bytes past the end may be e4m3's NaN, which a weight of zero does not silence
+        if (FMT == KV8_FP8 && partly && kb + 4 * t + r >= (there ? k_end : 0))
+#pragma unroll
+          for (int w = 0; w < VW; ++w) vw[r][w] = 0u;
+      }
+      __syncwarp();                                 // the block has been read
+      ++used;
+      top_up();
 #pragma unroll
       for (int w = 0; w < VW; ++w) {
         uint32_t f[4];
@@ -346,8 +418,6 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 2) kv8_attn_kernel(
 #pragma unroll
         for (int n = 0; n < NT; ++n) mma_f16_16816(o[n][2 * w + 1], f, pb[n][0], pb[n][1]);
       }
-      blk = nxt;
-      if (i + 1 < n_my) load_v(blk);
     }
 
     if (joined) __syncthreads();
@@ -458,9 +528,9 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_join_kernel(const Kv8AttnArgs
 }
 
 template <class K, class... A>
-cudaError_t launch(K kernel, unsigned blocks, cudaStream_t st, A... args) {
+cudaError_t launch(K kernel, unsigned blocks, size_t smem, cudaStream_t st, A... args) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(blocks); cfg.blockDim = dim3(kWarps * 32); cfg.stream = st;
+  cfg.gridDim = dim3(blocks); cfg.blockDim = dim3(kWarps * 32); cfg.dynamicSmemBytes = smem; cfg.stream = st;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[0].val.programmaticStreamSerializationAllowed = 1;
@@ -476,10 +546,13 @@ int run(const Kv8AttnArgs& a, cudaStream_t st) {
   // which halves the loads and conversions of K and V
   const bool wide = rows * gq > 8;
   const long items = (long)a.n_groups * a.hkv * a.max_splits * ((rows * gq + (wide ? 15 : 7)) / (wide ? 16 : 8));
-  const unsigned grid = (unsigned)std::min<long>(items, 148 * (wide ? 2 : 4));
-  cudaError_t e = wide ? launch(kv8_attn_kernel<HD, FMT, 2>, grid, st, a) : launch(kv8_attn_kernel<HD, FMT, 1>, grid, st, a);
+  const unsigned grid = (unsigned)std::min<long>(items, 148 * (wide ? 2 : 3));
+  auto kernel = wide ? kv8_attn_kernel<HD, FMT, 2> : kv8_attn_kernel<HD, FMT, 1>;
+  const size_t smem = wide ? attn_smem<HD, 2>() : attn_smem<HD, 1>();
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);     // of the current device
+  if (e == cudaSuccess) e = launch(kernel, grid, smem, st, a);
   if (e == cudaSuccess && a.max_splits > 1)
-    e = launch(kv8_join_kernel<HD>, (unsigned)(a.n_groups * rows * a.hq), st, a, (int)rows);
+    e = launch(kv8_join_kernel<HD>, (unsigned)(a.n_groups * rows * a.hq), 0, st, a, (int)rows);
   return e == cudaSuccess ? B2_OK : B2_ERR_LAUNCH;
 }
 

@@ -4,8 +4,9 @@
 //
 //     o = sum_j p_j vs_j vc_j / sum_j p_j,    p_j = 2^(s_j - m),    s_j = log2(e) / sqrt(hd) * ks_j * (q . kc_j)
 //
-// over the keys j that the row sees.  One pass with a running reference m; the codes kc, vc become fp16 numbers (exactly: both
-// formats fit), their scales stay in fp32: ks multiplies the finished product, vs the weight before it is rounded.
+// over the keys j that the row sees.  One pass with a running reference m.  The int8 codes kc go into an integer product with q in
+// sixteen bits; e4m3's, and all vc, become fp16 numbers (exactly: both formats fit).  The scales stay in fp32: ks multiplies the
+// finished product, vs the weight before it is rounded.
 //
 // Split.  A sequence's keys are cut every split_keys keys, a constant of the engine; one CTA of four warps takes the keys of one
 // (group, KV head, columns, split), page i of them on warp i % 4, and joins its warps in shared memory.  Rows with one split are
@@ -23,6 +24,7 @@
 // V (a row of zeros has the least scale) cannot push the others out of fp16's range.  m is raised only when a column's largest
 // value has grown by 2^8 (fp16 has room for that), which leaves the accumulators alone for nearly all pages.
 #include <algorithm>
+#include <type_traits>
 
 #include "kv8.cuh"
 
@@ -68,21 +70,19 @@ __device__ __forceinline__ uint32_t biased_pair(uint32_t magic) {
   const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&magic), __half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480)));
   return *reinterpret_cast<const uint32_t*>(&v);
 }
-__device__ __forceinline__ uint32_t e4m3_pair(uint32_t two) {
-  uint32_t y;
-  asm("{ .reg .b16 lo, hi; mov.b32 {lo, hi}, %1; cvt.rn.f16x2.e4m3x2 %0, lo; }" : "=r"(y) : "r"(two));
-  return y;
+// four e4m3 numbers -> fp16 pairs (0, 1) and (2, 3)
+__device__ __forceinline__ void e4m3_pairs(uint32_t w, uint32_t& x, uint32_t& y) {
+  asm("{ .reg .b16 lo, hi; mov.b32 {lo, hi}, %2; cvt.rn.f16x2.e4m3x2 %0, lo; cvt.rn.f16x2.e4m3x2 %1, hi; }" : "=r"(x), "=r"(y) : "r"(w));
 }
-// Fragment pairs of a word of four codes of one row: channels (0, 2) and (1, 3) for int8, (0, 1) and (2, 3) for e4m3
-template <int FMT>
-__device__ __forceinline__ void row_pairs(uint32_t w, uint32_t& x, uint32_t& y) {
-  if (FMT == KV8_INT8) {
-    x = biased_pair(lop3_and_or(w, 0x00ff00ffu, 0x64006400u));
-    y = biased_pair(__byte_perm(w, 0x64646464u, 0x4341));
-  } else {
-    x = e4m3_pair(w);
-    y = e4m3_pair(w >> 16);
-  }
+// D(16x8, s32) += A(16x32, u8, row) * B(32x8, s8 or u8, col)
+template <bool SIGNED>
+__device__ __forceinline__ void mma_u8(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (SIGNED)
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.u8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 // Of two rows' words: pairs (row a, row b) of bytes 2 * HI and 2 * HI + 1
 template <int FMT, int HI>
@@ -92,9 +92,7 @@ __device__ __forceinline__ void cross_pairs(uint32_t wa, uint32_t wb, uint32_t& 
     x = biased_pair(lop3_and_or(z, 0x00ff00ffu, 0x64006400u));
     y = biased_pair(__byte_perm(z, 0x64646464u, 0x4341));
   } else {
-    const uint32_t z = __byte_perm(wa, wb, HI ? 0x7362 : 0x5140);
-    x = e4m3_pair(z);
-    y = e4m3_pair(z >> 16);
+    e4m3_pairs(__byte_perm(wa, wb, HI ? 0x7362 : 0x5140), x, y);
   }
 }
 
@@ -172,15 +170,19 @@ struct Ring {
   }
 };
 
-struct Item { int tok0, cnt, first, last, col0, kvh, split, n_my, page; };      // page: lane i's page i of this warp
+// One CTA's share of a group: keys of one split for eight or sixteen columns.
+struct Item {
+  int tok0, cnt, first, last, col0, kvh, split;
+  int n_my, page;                        // pages of this warp; lane i holds the number of page i
+};
 
 template <int HD, int NT>
 constexpr size_t attn_smem() { return (size_t)kWarps * (kStages * kv8_block_bytes(HD) + NT * 8 * (HD + 4) * 4 + 2 * NT * 8 * 4); }
 
 template <int HD, int FMT, int NT>
 __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_attn_kernel(const Kv8AttnArgs a) {
-  constexpr int KC = HD / 64;            // 16-byte chunks of a K row per lane
-  constexpr int KS = HD / 16;            // k-steps of K q^T
+  constexpr int KC = HD / 64;            // 16-byte pieces of a K row per lane
+  constexpr int KW = HD / 16;            // words of a K row per lane
   constexpr int VW = HD / 32;            // words of a V row per lane
   constexpr int MT = HD / 16;            // channel tiles of V^T p^T
   constexpr int COLS = NT * 8;
@@ -197,52 +199,76 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_attn_kernel(
   const Ring<HD> ring(lane);
   const uint32_t mem = smem_u32(smem) + warp * kStages * BLK;
 
-  // Items are numbered group after group; every lane holds one group of a run of 32 and the sum of items up to it.
-  int run = -32, base = 0, total = 0, incl = 0, mine = 0;
+  // Items are numbered group after group and cut evenly over the CTAs; neighbours differ in the split first, so a CTA keeps its
+  // q for most of them.  Every lane holds one group of a run of 32 and the number of items up to it.
+  int run = -1, base = 0, total = 0, incl = 0, mine = 0;
   Group grp = {0, 0, 0, -1, 0, true};
-  auto fetch = [&](int item, Item& it) -> bool {
-    while (item - base >= total) {
-      base += total;
-      run += 32;
-      if (run >= a.n_groups) return false;
-      grp = group_at(a, run + lane);
-      if (!grp.ok && blockIdx.x == 0 && warp == 0) atomicExch(a.status, (int)B2_ERR_BOUNDS);
-      mine = grp.ok && grp.cnt > 0 ? splits_of(grp.last, a.split_keys) * a.hkv * ((grp.cnt * gq + COLS - 1) / COLS) : 0;
-      incl = mine;
+  auto load_run = [&](int r) {
+    run = r;
+    grp = group_at(a, r * 32 + lane);
+    mine = grp.ok && grp.cnt > 0 ? splits_of(grp.last, a.split_keys) * a.hkv * ((grp.cnt * gq + COLS - 1) / COLS) : 0;
+    incl = mine;
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) { const int v = __shfl_up_sync(0xffffffffu, incl, o); if (lane >= o) incl += v; }
-      total = __shfl_sync(0xffffffffu, incl, 31);
-    }
-    const int src = __ffs(__ballot_sync(0xffffffffu, incl > item - base)) - 1;
-    int at = item - base - (__shfl_sync(0xffffffffu, incl, src) - __shfl_sync(0xffffffffu, mine, src));
+    for (int o = 1; o < 32; o <<= 1) { const int v = __shfl_up_sync(0xffffffffu, incl, o); if (lane >= o) incl += v; }
+    total = __shfl_sync(0xffffffffu, incl, 31);
+  };
+  int all = 0;
+  for (int r = 0; r * 32 < a.n_groups; ++r) {
+    load_run(r);
+    if (!grp.ok && blockIdx.x == 0 && warp == 0) atomicExch(a.status, (int)B2_ERR_BOUNDS);
+    all += total;
+  }
+  const int share = all / (int)gridDim.x, rest = all % (int)gridDim.x, id = blockIdx.x;
+  int item = id * share + min(id, rest);
+  const int item_end = item + share + (id < rest ? 1 : 0);
+  if (item >= item_end) return;
+  if (run != 0) load_run(0);
+  auto fetch = [&](int at, Item& it) {
+    while (at - base >= total) { base += total; load_run(run + 1); }
+    at -= base;
+    const int src = __ffs(__ballot_sync(0xffffffffu, incl > at)) - 1;
+    at -= __shfl_sync(0xffffffffu, incl, src) - __shfl_sync(0xffffffffu, mine, src);
     it.tok0 = __shfl_sync(0xffffffffu, grp.tok0, src); it.cnt = __shfl_sync(0xffffffffu, grp.cnt, src);
     it.first = __shfl_sync(0xffffffffu, grp.first, src); it.last = __shfl_sync(0xffffffffu, grp.last, src);
-    const int seq = __shfl_sync(0xffffffffu, grp.seq, src);
+    const int seq = __shfl_sync(0xffffffffu, grp.seq, src), ns = splits_of(it.last, a.split_keys);
     const int ctiles = (it.cnt * gq + COLS - 1) / COLS;
-    it.col0 = at % ctiles * COLS; at /= ctiles;
-    it.kvh = at % a.hkv; it.split = at / a.hkv;
+    it.split = at % ns; at /= ns;
+    it.col0 = at % ctiles * COLS; it.kvh = at / ctiles;
     const int k_begin = it.split * a.split_keys, k_end = min(it.last + 1, k_begin + a.split_keys);
     const int n_pg = (k_end - k_begin + kKv8Page - 1) / kKv8Page;           // 0 for a group without keys
     it.n_my = (n_pg - warp + kWarps - 1) / kWarps;                          // at most 32: split_keys is at most 2048
     it.page = -1;
     if (lane < it.n_my) it.page = a.block_table[(size_t)seq * a.bt_ld + k_begin / kKv8Page + warp + kWarps * lane];
     __syncwarp();
-    return true;
   };
   Item cur, nxt;
-  bool more = fetch(blockIdx.x, nxt);
-  // pages that this warp has sent for and has used; where it fetches (cur or nxt) and which page comes next
-  int made = 0, used = 0, at_page = 0;
-  bool ahead = false, joined = false;
-  for (int item = blockIdx.x; more; item += gridDim.x) {
+  fetch(item, nxt);
+  cur = nxt;
+  cur.tok0 = -1;                         // no q yet
+  int wr = 0, rd = 0, pending = 0;       // stages to fill and to read next; copies sent for and not yet used
+  int at_page = 0;                       // next page to send for, of nxt (ahead) or cur
+  bool ahead = true, joined = false;
+
+  // q, every column scaled by a power of two; qs undoes it on the scores and brings the softmax scale.
+  // int8: sixteen bits of fixed point, the largest value in [2^14, 2^15), as a signed and an unsigned byte (hi * 256 + lo): K's bytes
+  // then feed the product as they are, and the sums are exact.  What is lost is at most 2^-15 of the column's largest value, as much as
+  // a weight in fp16 loses.  The 128 in K's bytes comes off again with the accumulators' start, -128 * sum(q).
+  // e4m3: fp16 with the largest value in [2^10, 2^11), where a bf16 number stays exact down to 2^-24 of that.
+  uint32_t qb[NT][KW][2];
+  float qs[NT][2];
+  int q0[NT][2];
+
+  for (; item < item_end; ++item) {
+    const bool same_q = nxt.tok0 == cur.tok0 && nxt.cnt == cur.cnt && nxt.col0 == cur.col0 && nxt.kvh == cur.kvh;
     cur = nxt;
-    at_page = ahead ? at_page : 0;
+    if (!ahead) at_page = 0;
     ahead = false;
-    more = fetch(item + gridDim.x, nxt);
+    const bool more = item + 1 < item_end;
+    if (more) fetch(item + 1, nxt);
     const int tok0 = cur.tok0, cnt = cur.cnt, first = cur.first, last = cur.last, col0 = cur.col0, kvh = cur.kvh, split = cur.split, n_my = cur.n_my;
     const int k_begin = split * a.split_keys, k_end = min(last + 1, k_begin + a.split_keys);
     auto top_up = [&]() {
-      while (made - used < kStages) {
+      while (pending < kStages) {
         if (!ahead && at_page >= n_my) { ahead = true; at_page = 0; }
         if (ahead && (!more || at_page >= nxt.n_my)) return;
         int p = __shfl_sync(0xffffffffu, ahead ? nxt.page : cur.page, at_page);
@@ -250,52 +276,69 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_attn_kernel(
           if (lane == 0) atomicExch(a.status, (int)B2_ERR_BOUNDS);
           p = 0;
         }
-        ring.copy(mem + made % kStages * BLK, a.pool + ((size_t)p * a.hkv + (ahead ? nxt.kvh : kvh)) * BLK, lane);
+        ring.copy(mem + wr, a.pool + ((size_t)p * a.hkv + (ahead ? nxt.kvh : kvh)) * BLK, lane);
         cp_async_commit();
-        ++made;
+        wr = wr == (kStages - 1) * BLK ? 0 : wr + BLK;
+        ++pending;
         ++at_page;
       }
     };
     top_up();
 
-    // q as fp16, every column scaled by a power of two of its own so that its largest value lies in [2^10, 2^11): a bf16 number
-    // stays exact down to 2^-24 of that.  qs undoes it on the scores and brings the softmax scale.
-    uint32_t qb[NT][KS][2];
-    float qs[NT][2];
+    if (!same_q) {
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const int col = col0 + n * 8 + g;
-      const bool live = col < cnt * gq;
-      uint4 raw[KC][2];
-      uint32_t top = 0;
+      for (int n = 0; n < NT; ++n) {
+        const int col = col0 + n * 8 + g;
+        const bool live = col < cnt * gq;
+        uint4 raw[KC][2];
+        uint32_t top = 0;
 #pragma unroll
-      for (int c = 0; c < KC; ++c)
+        for (int c = 0; c < KC; ++c)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          raw[c][h] = make_uint4(0u, 0u, 0u, 0u);
-          if (live) raw[c][h] = *reinterpret_cast<const uint4*>(a.q + (size_t)(tok0 + col / gq) * a.ldq + (size_t)(kvh * gq + col % gq) * HD + (t + 4 * c) * 16 + h * 8);
-          const uint32_t* w = &raw[c][h].x;
+          for (int h = 0; h < 2; ++h) {
+            raw[c][h] = make_uint4(0u, 0u, 0u, 0u);
+            if (live) raw[c][h] = *reinterpret_cast<const uint4*>(a.q + (size_t)(tok0 + col / gq) * a.ldq + (size_t)(kvh * gq + col % gq) * HD + (t + 4 * c) * 16 + h * 8);
+            const uint32_t* w = &raw[c][h].x;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) top = max(top, max((w[i] & 0x7fffu) << 16, w[i] & 0x7fff0000u));
+            for (int i = 0; i < 4; ++i) top = max(top, max((w[i] & 0x7fffu) << 16, w[i] & 0x7fff0000u));
+          }
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const uint32_t e = min((FMT == KV8_INT8 ? 268u : 264u) - (top >> 23), 253u);
+        const float up = __uint_as_float(e << 23);
+        float down = __uint_as_float((254u - e) << 23) * a.scale_log2;
+        if (top >= 0x7f800000u) down = __uint_as_float(0x7fffffffu);           // an infinity or a NaN in q: a column of NaN
+        int sum = 0;
+#pragma unroll
+        for (int c = 0; c < KC; ++c)
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {                // four channels of a K word
+            const uint32_t a0 = (&raw[c][w >> 1].x)[2 * (w & 1)], a1 = (&raw[c][w >> 1].x)[2 * (w & 1) + 1];
+            const float f0 = __uint_as_float(a0 << 16) * up, f1 = __uint_as_float(a0 & 0xffff0000u) * up;
+            const float f2 = __uint_as_float(a1 << 16) * up, f3 = __uint_as_float(a1 & 0xffff0000u) * up;
+            if constexpr (FMT == KV8_INT8) {
+              const int i0 = __float2int_rn(f0), i1 = __float2int_rn(f1), i2 = __float2int_rn(f2), i3 = __float2int_rn(f3);
+              sum += i0 + i1 + i2 + i3;
+              const uint32_t p01 = __byte_perm(i0, i1, 0x5140), p23 = __byte_perm(i2, i3, 0x5140);      // lo, lo, hi, hi
+              qb[n][c * 4 + w][0] = __byte_perm(p01, p23, 0x7632);
+              qb[n][c * 4 + w][1] = __byte_perm(p01, p23, 0x5410);
+            } else {
+              qb[n][c * 4 + w][0] = pack_half(f0, f1);
+              qb[n][c * 4 + w][1] = pack_half(f2, f3);
+            }
+          }
+        qs[n][0] = __shfl_sync(0xffffffffu, down, 8 * t);
+        qs[n][1] = __shfl_sync(0xffffffffu, down, 8 * t + 4);
+        if constexpr (FMT == KV8_INT8) {
+          sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+          sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+          q0[n][0] = -128 * __shfl_sync(0xffffffffu, sum, 8 * t);
+          q0[n][1] = -128 * __shfl_sync(0xffffffffu, sum, 8 * t + 4);
         }
-      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      const uint32_t e = min(264u - (top >> 23), 253u);
-      const float up = __uint_as_float(e << 23), down = __uint_as_float((254u - e) << 23) * a.scale_log2;
-      qs[n][0] = __shfl_sync(0xffffffffu, down, 8 * t);
-      qs[n][1] = __shfl_sync(0xffffffffu, down, 8 * t + 4);
-#pragma unroll
-      for (int c = 0; c < KC; ++c)
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {                // four channels of a K word
-          const uint32_t a0 = (&raw[c][w >> 1].x)[2 * (w & 1)], a1 = (&raw[c][w >> 1].x)[2 * (w & 1) + 1];
-          const float f0 = __uint_as_float(a0 << 16) * up, f1 = __uint_as_float(a0 & 0xffff0000u) * up;
-          const float f2 = __uint_as_float(a1 << 16) * up, f3 = __uint_as_float(a1 & 0xffff0000u) * up;
-          qb[n][c * 4 + w][0] = FMT == KV8_INT8 ? pack_half(f0, f2) : pack_half(f0, f1);
-          qb[n][c * 4 + w][1] = FMT == KV8_INT8 ? pack_half(f1, f3) : pack_half(f2, f3);
-        }
+      }
     }
 
+    // m is the reference less kUp, so that 2^(s - m) carries the 2^30
     float o[NT][MT][4], m[NT][2], l[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -306,33 +349,57 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_attn_kernel(
 
     for (int i = 0; i < n_my; ++i) {
       // this page has arrived once no more copies are under way than were sent for after it
-      if (made - used >= 3) cp_async_wait<2>(); else if (made - used == 2) cp_async_wait<1>(); else cp_async_wait<0>();
+      if (pending >= 3) cp_async_wait<2>(); else if (pending == 2) cp_async_wait<1>(); else cp_async_wait<0>();
       __syncwarp();
-      const uint32_t stage = mem + used % kStages * BLK;
+      const uint32_t stage = mem + rd;
       // s: keys 2g (0, 1) and 2g + 1 (2, 3), columns 2t (0, 2) and 2t + 1 (1, 3)
       float s[NT][4];
+      if constexpr (FMT == KV8_INT8) {
+        int hi[NT][4], lo[NT][4];
 #pragma unroll
-      for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int c = 0; c < KC; ++c) {
-        const uint4 k0 = ring.k(stage, 0, c), k1 = ring.k(stage, 1, c);
+          for (int j = 0; j < 4; ++j) { hi[n][j] = 0; lo[n][j] = q0[n][j & 1]; }
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          uint32_t f[4];
-          row_pairs<FMT>((&k0.x)[w], f[0], f[2]);
-          row_pairs<FMT>((&k1.x)[w], f[1], f[3]);
+        for (int c = 0; c < KC; ++c) {
+          const uint4 k0 = ring.k(stage, 0, c), k1 = ring.k(stage, 1, c);
 #pragma unroll
-          for (int n = 0; n < NT; ++n) mma_f16_16816(s[n], f, qb[n][c * 4 + w][0], qb[n][c * 4 + w][1]);
+          for (int w = 0; w < 4; w += 2) {
+            const uint32_t f[4] = {(&k0.x)[w], (&k1.x)[w], (&k0.x)[w + 1], (&k1.x)[w + 1]};
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              mma_u8<true>(hi[n], f, qb[n][c * 4 + w][0], qb[n][c * 4 + w + 1][0]);
+              mma_u8<false>(lo[n], f, qb[n][c * 4 + w][1], qb[n][c * 4 + w + 1][1]);
+            }
+          }
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) s[n][j] = __int2float_rn(hi[n][j] * 256 + lo[n][j]);
+      } else {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+#pragma unroll
+        for (int c = 0; c < KC; ++c) {
+          const uint4 k0 = ring.k(stage, 0, c), k1 = ring.k(stage, 1, c);
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            uint32_t f[4];
+            e4m3_pairs((&k0.x)[w], f[0], f[2]);
+            e4m3_pairs((&k1.x)[w], f[1], f[3]);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) mma_f16_16816(s[n], f, qb[n][c * 4 + w][0], qb[n][c * 4 + w][1]);
+          }
         }
       }
-      uint4 su = lds128(stage + 2 * kKv8Page * HD + g * 16);        // K and V scales of keys 2g, 2g + 1
+      const uint4 su = lds128(stage + 2 * kKv8Page * HD + g * 16);        // K and V scales of keys 2g, 2g + 1
       const float4 scale = make_float4(__uint_as_float(su.x), __uint_as_float(su.y), __uint_as_float(su.z), __uint_as_float(su.w));
       const int page = __shfl_sync(0xffffffffu, cur.page, i);
       const bool there = page >= 0 && page < a.n_pages;
 
-      const float e0 = __uint_as_float(0x4b000000u | (__float_as_uint(scale.y) >> 23)) - 8388735.f;      // log2 of vs's power of two
-      const float e1 = __uint_as_float(0x4b000000u | (__float_as_uint(scale.w) >> 23)) - 8388735.f;
-      bool grows = false;
+      const float e0 = __uint_as_float(0x4b000000u | (su.y >> 23)) - 8388735.f;       // log2 of vs's power of two
+      const float e1 = __uint_as_float(0x4b000000u | (su.w >> 23)) - 8388735.f;
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -356,10 +423,11 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_attn_kernel(
             }
           }
       }
+      bool grows = false;
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) grows |= fmaxf(__fadd_rn(s[n][j], e0), __fadd_rn(s[n][2 + j], e1)) > __fadd_rn(m[n][j], kGrow);
+        for (int j = 0; j < 2; ++j) grows |= fmaxf(__fadd_rn(s[n][j], e0), __fadd_rn(s[n][2 + j], e1)) > __fadd_rn(m[n][j], kUp + kGrow);
       if (__any_sync(0xffffffffu, grows)) {
 #pragma unroll
         for (int n = 0; n < NT; ++n)
@@ -369,9 +437,9 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_attn_kernel(
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-            if (mx > __fadd_rn(m[n][j], kGrow)) {
-              const float f = ex2(__fadd_rn(m[n][j], -mx));
-              m[n][j] = mx;
+            if (mx > __fadd_rn(m[n][j], kUp + kGrow)) {
+              const float f = ex2(__fadd_rn(m[n][j], kUp - mx));
+              m[n][j] = __fadd_rn(mx, -kUp);
               l[n][j] = __fmul_rn(l[n][j], f);
 #pragma unroll
               for (int k = 0; k < MT; ++k) { o[n][k][j] = __fmul_rn(o[n][k][j], f); o[n][k][2 + j] = __fmul_rn(o[n][k][2 + j], f); }
@@ -379,14 +447,14 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_attn_kernel(
           }
         __syncwarp();
       }
-      const float v0 = scale.y * kDown, v1 = scale.w * kDown;
+      const float v0 = __fmul_rn(scale.y, kDown), v1 = __fmul_rn(scale.w, kDown);
       uint32_t pb[NT][2];
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         float w[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const float p = ex2(__fadd_rn(__fadd_rn(s[n][j], -m[n][j & 1]), kUp));
+          const float p = ex2(__fadd_rn(s[n][j], -m[n][j & 1]));
           l[n][j & 1] = __fadd_rn(l[n][j & 1], p);
           w[j] = __fmul_rn(p, j < 2 ? v0 : v1);
           if (partly && s[n][j] == -INFINITY) w[j] = 0.f;       // a row that is not seen may have the scale NaN
@@ -404,7 +472,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_attn_kernel(
           for (int w = 0; w < VW; ++w) vw[r][w] = 0u;
       }
       __syncwarp();                                 // the block has been read
-      ++used;
+      rd = rd == (kStages - 1) * BLK ? 0 : rd + BLK;
+      --pending;
       top_up();
 #pragma unroll
       for (int w = 0; w < VW; ++w) {
@@ -420,7 +489,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_attn_kernel(
       }
     }
 
-    if (joined) __syncthreads();
+    if (joined) __syncthreads();                    // the item before has been read
     joined = true;
 #pragma unroll
     for (int n = 0; n < NT; ++n)
@@ -470,12 +539,13 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_attn_kernel(
   }
 }
 
-// Joins the splits of rows that have more than one: a CTA per (group, row, q head), warp w adds the splits w, w + 4, ... in
-// order, the four sums are added in order of w.
-template <int HD>
-__global__ void __launch_bounds__(kWarps * 32) kv8_join_kernel(const Kv8AttnArgs a, int rows_at_once) {
-  constexpr int PER = HD / 32, AHEAD = 4;
-  __shared__ float sh[kWarps][HD + 1];
+// Joins the splits of rows that have more than one: a CTA per (group, row, q head).  Sixteen sums, sum j of the splits j, j + 16, ...
+// in order, are added in order of j.  WARPS warps take 16 / WARPS sums each, side by side; both variants give the same bits.
+template <int HD, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32) kv8_join_kernel(const Kv8AttnArgs a, int rows_at_once) {
+  constexpr int PER = HD / 32, SETS = 16, MY = SETS / WARPS, AHEAD = 8 / MY;
+  using Vec = std::conditional_t<PER == 4, float4, float2>;
+  __shared__ float sh[SETS][HD + 1];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_wait();
   pdl_launch_dependents();
@@ -487,40 +557,50 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_join_kernel(const Kv8AttnArgs
     const int ns = splits_of(grp.cnt == 1 ? grp.last : min(a.tok_pos[tok], grp.last), a.split_keys);
     if (ns == 1) continue;
     const size_t slot = ((size_t)tok * a.hq + head) * a.max_splits;
-    const float* po = a.part_o + slot * HD + lane * PER;
+    const Vec* po = reinterpret_cast<const Vec*>(a.part_o + slot * HD) + lane;
     const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + slot;
     float M = kNoRef;
     for (int s = lane; s < ns; s += 32) M = fmaxf(M, ml[s].x);
     M = warp_max(M);
-    float L = 0.f, x[PER];
+    float L[MY], x[MY][PER];
 #pragma unroll
-    for (int i = 0; i < PER; ++i) x[i] = 0.f;
-    for (int s0 = warp; s0 < ns; s0 += AHEAD * kWarps) {
-      float2 w[AHEAD];
-      float y[AHEAD][PER];
+    for (int k = 0; k < MY; ++k) {
+      L[k] = 0.f;
 #pragma unroll
-      for (int j = 0; j < AHEAD; ++j) {
-        const int s = s0 + j * kWarps;
-        w[j] = s < ns ? ml[s] : make_float2(kNoRef, 0.f);
+      for (int i = 0; i < PER; ++i) x[k][i] = 0.f;
+    }
+    for (int s0 = warp * MY; s0 < ns; s0 += AHEAD * SETS) {
+      float2 w[AHEAD][MY];
+      Vec y[AHEAD][MY];
 #pragma unroll
-        for (int i = 0; i < PER; ++i) y[j][i] = s < ns ? po[(size_t)s * HD + i] : 0.f;
-      }
+      for (int j = 0; j < AHEAD; ++j)
 #pragma unroll
-      for (int j = 0; j < AHEAD; ++j) {
-        const float f = ex2(__fadd_rn(w[j].x, -M));
-        L = __fmaf_rn(w[j].y, f, L);
+        for (int k = 0; k < MY; ++k) {                 // past the end: the last split again, with the weight zero
+          const int s = min(s0 + j * SETS + k, ns - 1);
+          w[j][k] = ml[s];
+          y[j][k] = po[(size_t)s * 32];
+        }
 #pragma unroll
-        for (int i = 0; i < PER; ++i) x[i] = __fmaf_rn(y[j][i], f, x[i]);
-      }
+      for (int j = 0; j < AHEAD; ++j)
+#pragma unroll
+        for (int k = 0; k < MY; ++k) {
+          const float f = s0 + j * SETS + k < ns ? ex2(__fadd_rn(w[j][k].x, -M)) : 0.f;
+          L[k] = __fmaf_rn(w[j][k].y, f, L[k]);
+#pragma unroll
+          for (int i = 0; i < PER; ++i) x[k][i] = __fmaf_rn((&y[j][k].x)[i], f, x[k][i]);
+        }
     }
 #pragma unroll
-    for (int i = 0; i < PER; ++i) sh[warp][lane * PER + i] = x[i];
-    if (lane == 0) sh[warp][HD] = L;
+    for (int k = 0; k < MY; ++k) {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) sh[warp * MY + k][lane * PER + i] = x[k][i];
+      if (lane == 0) sh[warp * MY + k][HD] = L[k];
+    }
     __syncthreads();
-    for (int d = threadIdx.x; d < HD; d += kWarps * 32) {
+    for (int d = threadIdx.x; d < HD; d += WARPS * 32) {
       float sum = sh[0][d], Ls = sh[0][HD];
 #pragma unroll
-      for (int w = 1; w < kWarps; ++w) { sum = __fadd_rn(sum, sh[w][d]); Ls = __fadd_rn(Ls, sh[w][HD]); }
+      for (int w = 1; w < SETS; ++w) { sum = __fadd_rn(sum, sh[w][d]); Ls = __fadd_rn(Ls, sh[w][HD]); }
       a.out[(size_t)tok * a.ldo + (size_t)head * HD + d] = __float2bfloat16_rn(Ls == 0.f ? 0.f : __fmul_rn(sum, __fdiv_rn(1.f, Ls)));
     }
     __syncthreads();
@@ -528,9 +608,9 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_join_kernel(const Kv8AttnArgs
 }
 
 template <class K, class... A>
-cudaError_t launch(K kernel, unsigned blocks, size_t smem, cudaStream_t st, A... args) {
+cudaError_t launch(K kernel, unsigned blocks, int threads, size_t smem, cudaStream_t st, A... args) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(blocks); cfg.blockDim = dim3(kWarps * 32); cfg.dynamicSmemBytes = smem; cfg.stream = st;
+  cfg.gridDim = dim3(blocks); cfg.blockDim = dim3(threads); cfg.dynamicSmemBytes = smem; cfg.stream = st;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[0].val.programmaticStreamSerializationAllowed = 1;
@@ -550,9 +630,13 @@ int run(const Kv8AttnArgs& a, cudaStream_t st) {
   auto kernel = wide ? kv8_attn_kernel<HD, FMT, 2> : kv8_attn_kernel<HD, FMT, 1>;
   const size_t smem = wide ? attn_smem<HD, 2>() : attn_smem<HD, 1>();
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);     // of the current device
-  if (e == cudaSuccess) e = launch(kernel, grid, smem, st, a);
-  if (e == cudaSuccess && a.max_splits > 1)
-    e = launch(kv8_join_kernel<HD>, (unsigned)(a.n_groups * rows * a.hq), 0, st, a, (int)rows);
+  if (e == cudaSuccess) e = launch(kernel, grid, kWarps * 32, smem, st, a);
+  if (e == cudaSuccess && a.max_splits > 1) {
+    // few rows with many splits: sixteen warps a CTA keep enough loads under way
+    const unsigned blocks = (unsigned)(a.n_groups * rows * a.hq);
+    e = a.max_splits > 16 && blocks <= 148 * 4 ? launch(kv8_join_kernel<HD, 16>, blocks, 512, 0, st, a, (int)rows)
+                                               : launch(kv8_join_kernel<HD, 4>, blocks, 128, 0, st, a, (int)rows);
+  }
   return e == cudaSuccess ? B2_OK : B2_ERR_LAUNCH;
 }
 

@@ -49,7 +49,7 @@ struct Kv8AttnArgs {
 namespace {
 
 constexpr int kWarps = 4;
-constexpr int kStages = 3;                  // pages that a warp has in shared memory or under way
+constexpr int kStages = 2;                  // pairs of pages that a warp has in shared memory or under way
 constexpr float kNoRef = -3.4028234e38f;    // m before the first key
 constexpr float kGrow = 8.f;                // log2 of what a column may grow before m follows
 // l sums 2^(s - m) * 2^30 and the weights carry vs * 2^-30: with V of any size between 2^-64 and 2^121 neither leaves fp32
@@ -63,11 +63,6 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
 }
 __device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
   const __half2 v = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&v);
-}
-// two bytes with 128 added -> two fp16 numbers: 0x64xx is 1024 + xx, then minus 1152
-__device__ __forceinline__ uint32_t biased_pair(uint32_t magic) {
-  const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&magic), __half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480)));
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 // four e4m3 numbers -> fp16 pairs (0, 1) and (2, 3)
@@ -89,8 +84,8 @@ template <int FMT, int HI>
 __device__ __forceinline__ void cross_pairs(uint32_t wa, uint32_t wb, uint32_t& x, uint32_t& y) {
   if (FMT == KV8_INT8) {
     const uint32_t z = __byte_perm(wa, wb, HI ? 0x7632 : 0x5410);
-    x = biased_pair(lop3_and_or(z, 0x00ff00ffu, 0x64006400u));
-    y = biased_pair(__byte_perm(z, 0x64646464u, 0x4341));
+    x = lop3_and_or(z, 0x00ff00ffu, 0x64006400u);          // 0x64xx is 1024 + xx, 1152 above the code
+    y = __byte_perm(z, 0x64646464u, 0x4341);
   } else {
     e4m3_pairs(__byte_perm(wa, wb, HI ? 0x7362 : 0x5140), x, y);
   }
@@ -176,8 +171,8 @@ struct Item {
   int n_my, page;                        // pages of this warp; lane i holds the number of page i
 };
 
-template <int HD, int NT>
-constexpr size_t attn_smem() { return (size_t)kWarps * (kStages * kv8_block_bytes(HD) + NT * 8 * (HD + 4) * 4 + 2 * NT * 8 * 4); }
+template <int HD>
+constexpr int attn_smem() { return kWarps * kStages * 2 * kv8_block_bytes(HD); }
 
 template <int HD, int FMT, int NT>
 __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_attn_kernel(const Kv8AttnArgs a) {
@@ -188,16 +183,18 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_attn_kernel(
   constexpr int COLS = NT * 8;
   constexpr int LDO = HD + 4;
   constexpr int BLK = kv8_block_bytes(HD);
+  constexpr int PAIR = 2 * BLK;
+  // a warp's results of an item go over the pair of pages that it used last, which is not refilled before they have been read
+  static_assert(COLS * LDO * 4 <= PAIR, "a tile of results fits a pair of pages");
   extern __shared__ __align__(128) uint8_t smem[];
-  float (*sh_o)[COLS][LDO] = reinterpret_cast<float (*)[COLS][LDO]>(smem + kWarps * kStages * BLK);
-  float (*sh_m)[COLS] = reinterpret_cast<float (*)[COLS]>(sh_o + kWarps);
-  float (*sh_l)[COLS] = sh_m + kWarps;
+  __shared__ float sh_m[kWarps][COLS], sh_l[kWarps][COLS];
+  __shared__ int sh_at[kWarps];
   pdl_wait();
   pdl_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int gq = a.hq / a.hkv;
   const Ring<HD> ring(lane);
-  const uint32_t mem = smem_u32(smem) + warp * kStages * BLK;
+  const uint32_t mem = smem_u32(smem) + warp * kStages * PAIR;
 
   // Items are numbered group after group and cut evenly over the CTAs; neighbours differ in the split first, so a CTA keeps its
   // q for most of them.  Every lane holds one group of a run of 32 and the number of items up to it.
@@ -245,9 +242,10 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_attn_kernel(
   fetch(item, nxt);
   cur = nxt;
   cur.tok0 = -1;                         // no q yet
-  int wr = 0, rd = 0, pending = 0;       // stages to fill and to read next; copies sent for and not yet used
-  int at_page = 0;                       // next page to send for, of nxt (ahead) or cur
-  bool ahead = true, joined = false;
+  int wr = 0, rd = 0, pending = 0;       // stages to fill and to read next; pairs sent for and not yet used
+  // where this warp fetches (nxt once it is ahead of cur): pages left to send for and which come next
+  int f_i = 0, f_n = 0, f_page = 0, f_kvh = 0;
+  bool ahead = false, more = true;
 
   // q, every column scaled by a power of two; qs undoes it on the scores and brings the softmax scale.
   // int8: sixteen bits of fixed point, the largest value in [2^14, 2^15), as a signed and an unsigned byte (hi * 256 + lo): K's bytes
@@ -261,26 +259,35 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_attn_kernel(
   for (; item < item_end; ++item) {
     const bool same_q = nxt.tok0 == cur.tok0 && nxt.cnt == cur.cnt && nxt.col0 == cur.col0 && nxt.kvh == cur.kvh;
     cur = nxt;
-    if (!ahead) at_page = 0;
+    if (!ahead) { f_i = 0; f_n = cur.n_my; f_page = cur.page; f_kvh = cur.kvh; }
     ahead = false;
-    const bool more = item + 1 < item_end;
+    more = item + 1 < item_end;
     if (more) fetch(item + 1, nxt);
     const int tok0 = cur.tok0, cnt = cur.cnt, first = cur.first, last = cur.last, col0 = cur.col0, kvh = cur.kvh, split = cur.split, n_my = cur.n_my;
     const int k_begin = split * a.split_keys, k_end = min(last + 1, k_begin + a.split_keys);
+    const unsigned valid = __ballot_sync(0xffffffffu, lane < n_my && (unsigned)cur.page < (unsigned)a.n_pages);
     auto top_up = [&]() {
       while (pending < kStages) {
-        if (!ahead && at_page >= n_my) { ahead = true; at_page = 0; }
-        if (ahead && (!more || at_page >= nxt.n_my)) return;
-        int p = __shfl_sync(0xffffffffu, ahead ? nxt.page : cur.page, at_page);
-        if (p < 0 || p >= a.n_pages) {               // its keys are masked below; something there is copied in their place
-          if (lane == 0) atomicExch(a.status, (int)B2_ERR_BOUNDS);
-          p = 0;
+        if (f_i >= f_n) {
+          if (ahead || !more) return;
+          ahead = true;
+          f_i = 0; f_n = nxt.n_my; f_page = nxt.page; f_kvh = nxt.kvh;
+          continue;
         }
-        ring.copy(mem + wr, a.pool + ((size_t)p * a.hkv + (ahead ? nxt.kvh : kvh)) * BLK, lane);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if (h == 1 && f_i + 1 >= f_n) break;
+          int p = __shfl_sync(0xffffffffu, f_page, f_i + h);
+          if ((unsigned)p >= (unsigned)a.n_pages) {       // its keys are masked below; something there is copied in their place
+            if (lane == 0) atomicExch(a.status, (int)B2_ERR_BOUNDS);
+            p = 0;
+          }
+          ring.copy(mem + wr + h * BLK, a.pool + ((size_t)p * a.hkv + f_kvh) * BLK, lane);
+        }
         cp_async_commit();
-        wr = wr == (kStages - 1) * BLK ? 0 : wr + BLK;
+        wr ^= PAIR;
         ++pending;
-        ++at_page;
+        f_i += 2;
       }
     };
     top_up();
@@ -340,74 +347,84 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_attn_kernel(
 
     // m is the reference less kUp, so that 2^(s - m) carries the 2^30
     float o[NT][MT][4], m[NT][2], l[NT][2];
+    // int8: V's fp16 numbers are 1152 above the codes; the same sums of 1152 alone are taken off at the end.  Both lose alike to
+    // the accumulators' truncation, 2^-23 of 1152 a step, so that what is left of it is a random part below 2^-10 of a code.
+    float bias[NT][4];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       m[n][0] = m[n][1] = kNoRef; l[n][0] = l[n][1] = 0.f;
+      bias[n][0] = bias[n][1] = bias[n][2] = bias[n][3] = 0.f;
 #pragma unroll
       for (int i = 0; i < MT; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
     }
 
-    for (int i = 0; i < n_my; ++i) {
-      // this page has arrived once no more copies are under way than were sent for after it
-      if (pending >= 3) cp_async_wait<2>(); else if (pending == 2) cp_async_wait<1>(); else cp_async_wait<0>();
+    for (int i = 0; i < n_my; i += 2) {
+      // this pair has arrived once no more copies are under way than were sent for after it
+      if (pending >= 2) cp_async_wait<1>(); else cp_async_wait<0>();
       __syncwarp();
       const uint32_t stage = mem + rd;
-      // s: keys 2g (0, 1) and 2g + 1 (2, 3), columns 2t (0, 2) and 2t + 1 (1, 3)
-      float s[NT][4];
-      if constexpr (FMT == KV8_INT8) {
-        int hi[NT][4], lo[NT][4];
+      // s[h]: page i + h, keys 2g (0, 1) and 2g + 1 (2, 3), columns 2t (0, 2) and 2t + 1 (1, 3)
+      float s[2][NT][4];
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+      for (int h = 0; h < 2; ++h) {
+        if constexpr (FMT == KV8_INT8) {
+          int hi[NT][4], lo[NT][4];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) { hi[n][j] = 0; lo[n][j] = q0[n][j & 1]; }
+          for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int c = 0; c < KC; ++c) {
-          const uint4 k0 = ring.k(stage, 0, c), k1 = ring.k(stage, 1, c);
+            for (int j = 0; j < 4; ++j) { hi[n][j] = 0; lo[n][j] = q0[n][j & 1]; }
 #pragma unroll
-          for (int w = 0; w < 4; w += 2) {
-            const uint32_t f[4] = {(&k0.x)[w], (&k1.x)[w], (&k0.x)[w + 1], (&k1.x)[w + 1]};
+          for (int c = 0; c < KC; ++c) {
+            const uint4 k0 = ring.k(stage + h * BLK, 0, c), k1 = ring.k(stage + h * BLK, 1, c);
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-              mma_u8<true>(hi[n], f, qb[n][c * 4 + w][0], qb[n][c * 4 + w + 1][0]);
-              mma_u8<false>(lo[n], f, qb[n][c * 4 + w][1], qb[n][c * 4 + w + 1][1]);
+            for (int w = 0; w < 4; w += 2) {
+              const uint32_t f[4] = {(&k0.x)[w], (&k1.x)[w], (&k0.x)[w + 1], (&k1.x)[w + 1]};
+#pragma unroll
+              for (int n = 0; n < NT; ++n) {
+                mma_u8<true>(hi[n], f, qb[n][c * 4 + w][0], qb[n][c * 4 + w + 1][0]);
+                mma_u8<false>(lo[n], f, qb[n][c * 4 + w][1], qb[n][c * 4 + w + 1][1]);
+              }
+            }
+          }
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s[h][n][j] = __int2float_rn(hi[n][j] * 256 + lo[n][j]);
+        } else {
+#pragma unroll
+          for (int n = 0; n < NT; ++n) s[h][n][0] = s[h][n][1] = s[h][n][2] = s[h][n][3] = 0.f;
+#pragma unroll
+          for (int c = 0; c < KC; ++c) {
+            const uint4 k0 = ring.k(stage + h * BLK, 0, c), k1 = ring.k(stage + h * BLK, 1, c);
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+              uint32_t f[4];
+              e4m3_pairs((&k0.x)[w], f[0], f[2]);
+              e4m3_pairs((&k1.x)[w], f[1], f[3]);
+#pragma unroll
+              for (int n = 0; n < NT; ++n) mma_f16_16816(s[h][n], f, qb[n][c * 4 + w][0], qb[n][c * 4 + w][1]);
             }
           }
         }
+      }
+      float e[2][2], vs[2][2];                      // of keys 2g, 2g + 1: log2 of V scale's power of two; V scale 2^-30
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint4 su = lds128(stage + h * BLK + 2 * kKv8Page * HD + g * 16);        // (K, V) scales of keys 2g, 2g + 1
+        e[h][0] = __uint_as_float(0x4b000000u | (su.y >> 23)) - 8388735.f;
+        e[h][1] = __uint_as_float(0x4b000000u | (su.w >> 23)) - 8388735.f;
+        vs[h][0] = __fmul_rn(__uint_as_float(su.y), kDown);
+        vs[h][1] = __fmul_rn(__uint_as_float(su.w), kDown);
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) s[n][j] = __int2float_rn(hi[n][j] * 256 + lo[n][j]);
-      } else {
-#pragma unroll
-        for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
-#pragma unroll
-        for (int c = 0; c < KC; ++c) {
-          const uint4 k0 = ring.k(stage, 0, c), k1 = ring.k(stage, 1, c);
-#pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            uint32_t f[4];
-            e4m3_pairs((&k0.x)[w], f[0], f[2]);
-            e4m3_pairs((&k1.x)[w], f[1], f[3]);
-#pragma unroll
-            for (int n = 0; n < NT; ++n) mma_f16_16816(s[n], f, qb[n][c * 4 + w][0], qb[n][c * 4 + w][1]);
-          }
-        }
+          for (int j = 0; j < 4; ++j) s[h][n][j] = __fmul_rn(__fmul_rn(s[h][n][j], __uint_as_float(j < 2 ? su.x : su.z)), qs[n][j & 1]);
       }
-      const uint4 su = lds128(stage + 2 * kKv8Page * HD + g * 16);        // K and V scales of keys 2g, 2g + 1
-      const float4 scale = make_float4(__uint_as_float(su.x), __uint_as_float(su.y), __uint_as_float(su.z), __uint_as_float(su.w));
-      const int page = __shfl_sync(0xffffffffu, cur.page, i);
-      const bool there = page >= 0 && page < a.n_pages;
-
-      const float e0 = __uint_as_float(0x4b000000u | (su.y >> 23)) - 8388735.f;       // log2 of vs's power of two
-      const float e1 = __uint_as_float(0x4b000000u | (su.w >> 23)) - 8388735.f;
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) s[n][j] = __fmul_rn(__fmul_rn(s[n][j], j < 2 ? scale.x : scale.z), qs[n][j & 1]);
-      const int kb = k_begin + (warp + kWarps * i) * kKv8Page;
-      const bool partly = kb + kKv8Page > min(first, k_end) || !there;      // from the group's first slot on keys are looked at one by one
+      const int kb = k_begin + (warp + kWarps * i) * kKv8Page;              // the pair's second page begins 64 keys later
+      const unsigned have = valid >> i & 3u;
+      // from the group's first slot on, at the split's end and where a page is missing, keys are looked at one by one
+      const bool partly = kb + (kWarps + 1) * kKv8Page > min(first, k_end) || have != 3u;
       if (partly) {
-        const int end = there ? k_end : 0;
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -416,24 +433,31 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_attn_kernel(
             const int pos = cnt == 1 ? last : min(a.tok_pos[tok0 + row], last);
             const unsigned mask = a.tree_mask ? a.tree_mask[tok0 + row] : 0u;
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-              const int key = kb + 2 * g + r, in = key - first;
-              const bool seen = key <= pos && key < end && (!a.tree_mask || in < 0 || (in < 32 && ((mask >> (in & 31)) & 1u)));
-              if (!seen) s[n][2 * r + j] = -INFINITY;
-            }
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+              for (int r = 0; r < 2; ++r) {
+                const int key = kb + h * kWarps * kKv8Page + 2 * g + r, in = key - first;
+                const bool seen = key <= pos && key < k_end && (have >> h & 1u) && (!a.tree_mask || in < 0 || (in < 32 && ((mask >> (in & 31)) & 1u)));
+                if (!seen) s[h][n][2 * r + j] = -INFINITY;
+              }
           }
       }
       bool grows = false;
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) grows |= fmaxf(__fadd_rn(s[n][j], e0), __fadd_rn(s[n][2 + j], e1)) > __fadd_rn(m[n][j], kUp + kGrow);
+        for (int j = 0; j < 2; ++j) {
+          const float top = fmaxf(fmaxf(__fadd_rn(s[0][n][j], e[0][0]), __fadd_rn(s[0][n][2 + j], e[0][1])),
+                                  fmaxf(__fadd_rn(s[1][n][j], e[1][0]), __fadd_rn(s[1][n][2 + j], e[1][1])));
+          grows |= top > __fadd_rn(m[n][j], kUp + kGrow);
+        }
       if (__any_sync(0xffffffffu, grows)) {
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            float mx = fmaxf(__fadd_rn(s[n][j], e0), __fadd_rn(s[n][2 + j], e1));
+            float mx = fmaxf(fmaxf(__fadd_rn(s[0][n][j], e[0][0]), __fadd_rn(s[0][n][2 + j], e[0][1])),
+                             fmaxf(__fadd_rn(s[1][n][j], e[1][0]), __fadd_rn(s[1][n][2 + j], e[1][1])));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
@@ -441,70 +465,90 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_attn_kernel(
               const float f = ex2(__fadd_rn(m[n][j], kUp - mx));
               m[n][j] = __fadd_rn(mx, -kUp);
               l[n][j] = __fmul_rn(l[n][j], f);
+              bias[n][j] = __fmul_rn(bias[n][j], f);
+              bias[n][2 + j] = bias[n][j];
 #pragma unroll
               for (int k = 0; k < MT; ++k) { o[n][k][j] = __fmul_rn(o[n][k][j], f); o[n][k][2 + j] = __fmul_rn(o[n][k][2 + j], f); }
             }
           }
         __syncwarp();
       }
-      const float v0 = __fmul_rn(scale.y, kDown), v1 = __fmul_rn(scale.w, kDown);
-      uint32_t pb[NT][2];
+      uint32_t pb[2][NT][2];
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        float w[4];
+      for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float p = ex2(__fadd_rn(s[n][j], -m[n][j & 1]));
-          l[n][j & 1] = __fadd_rn(l[n][j & 1], p);
-          w[j] = __fmul_rn(p, j < 2 ? v0 : v1);
-          if (partly && s[n][j] == -INFINITY) w[j] = 0.f;       // a row that is not seen may have the scale NaN
+        for (int n = 0; n < NT; ++n) {
+          float w[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float p = ex2(__fadd_rn(s[h][n][j], -m[n][j & 1]));
+            l[n][j & 1] = __fadd_rn(l[n][j & 1], p);
+            w[j] = __fmul_rn(p, vs[h][j >> 1]);
+          }
+          if (partly)                               // a row that is not seen may have the scale NaN
+#pragma unroll
+            for (int j = 0; j < 4; ++j) if (s[h][n][j] == -INFINITY) w[j] = 0.f;
+          pb[h][n][0] = transpose8x8(pack_half(w[0], w[1]));
+          pb[h][n][1] = transpose8x8(pack_half(w[2], w[3]));
         }
-        pb[n][0] = transpose8x8(pack_half(w[0], w[1]));
-        pb[n][1] = transpose8x8(pack_half(w[2], w[3]));
-      }
-      uint32_t vw[4][VW];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        ring.v(stage, r, vw[r]);
-        // bytes past the end may be e4m3's NaN, which a weight of zero does not silence
-        if (FMT == KV8_FP8 && partly && kb + 4 * t + r >= (there ? k_end : 0))
+      for (int h = 0; h < 2; ++h) {
+        uint32_t vw[4][VW];
 #pragma unroll
-          for (int w = 0; w < VW; ++w) vw[r][w] = 0u;
-      }
-      __syncwarp();                                 // the block has been read
-      rd = rd == (kStages - 1) * BLK ? 0 : rd + BLK;
-      --pending;
-      top_up();
+        for (int r = 0; r < 4; ++r) {
+          ring.v(stage + h * BLK, r, vw[r]);
+          // bytes past the end may be e4m3's NaN, which a weight of zero does not silence
+          if (FMT == KV8_FP8 && partly && (kb + h * kWarps * kKv8Page + 4 * t + r >= k_end || !(have >> h & 1u)))
 #pragma unroll
-      for (int w = 0; w < VW; ++w) {
-        uint32_t f[4];
-        cross_pairs<FMT, 0>(vw[0][w], vw[2][w], f[0], f[1]);
-        cross_pairs<FMT, 0>(vw[1][w], vw[3][w], f[2], f[3]);
+            for (int w = 0; w < VW; ++w) vw[r][w] = 0u;
+        }
+        if (h == 1) {
+          __syncwarp();                             // the pair has been read
+          rd ^= PAIR;
+          --pending;
+          if (i + 2 < n_my) top_up();               // the last pair's place holds the results first
+        }
+        if constexpr (FMT == KV8_INT8) {
+          const uint32_t f[4] = {0x64806480u, 0x64806480u, 0x64806480u, 0x64806480u};         // 1152
 #pragma unroll
-        for (int n = 0; n < NT; ++n) mma_f16_16816(o[n][2 * w], f, pb[n][0], pb[n][1]);
-        cross_pairs<FMT, 1>(vw[0][w], vw[2][w], f[0], f[1]);
-        cross_pairs<FMT, 1>(vw[1][w], vw[3][w], f[2], f[3]);
+          for (int n = 0; n < NT; ++n) mma_f16_16816(bias[n], f, pb[h][n][0], pb[h][n][1]);
+        }
 #pragma unroll
-        for (int n = 0; n < NT; ++n) mma_f16_16816(o[n][2 * w + 1], f, pb[n][0], pb[n][1]);
+        for (int w = 0; w < VW; ++w) {
+          uint32_t f[4];
+          cross_pairs<FMT, 0>(vw[0][w], vw[2][w], f[0], f[1]);
+          cross_pairs<FMT, 0>(vw[1][w], vw[3][w], f[2], f[3]);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) mma_f16_16816(o[n][2 * w], f, pb[h][n][0], pb[h][n][1]);
+          cross_pairs<FMT, 1>(vw[0][w], vw[2][w], f[0], f[1]);
+          cross_pairs<FMT, 1>(vw[1][w], vw[3][w], f[2], f[3]);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) mma_f16_16816(o[n][2 * w + 1], f, pb[h][n][0], pb[h][n][1]);
+        }
       }
     }
 
-    if (joined) __syncthreads();                    // the item before has been read
-    joined = true;
+    const int at = warp * kStages * PAIR + (rd ^ PAIR);
+    if (lane == 0) sh_at[warp] = n_my > 0 ? at : -1;
+    if (n_my > 0) {
+      float (*tile)[LDO] = reinterpret_cast<float (*)[LDO]>(smem + at);
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        float x = l[n][j];
-        x = __fadd_rn(x, __shfl_xor_sync(0xffffffffu, x, 4));
-        x = __fadd_rn(x, __shfl_xor_sync(0xffffffffu, x, 8));
-        x = __fadd_rn(x, __shfl_xor_sync(0xffffffffu, x, 16));
-        const int c = n * 8 + 2 * t + j;
-        if (g == 0) { sh_m[warp][c] = m[n][j]; sh_l[warp][c] = __fmul_rn(x, kDown); }
+        for (int j = 0; j < 2; ++j) {
+          float x = l[n][j];
+          x = __fadd_rn(x, __shfl_xor_sync(0xffffffffu, x, 4));
+          x = __fadd_rn(x, __shfl_xor_sync(0xffffffffu, x, 8));
+          x = __fadd_rn(x, __shfl_xor_sync(0xffffffffu, x, 16));
+          const int c = n * 8 + 2 * t + j;
+          if (g == 0) { sh_m[warp][c] = m[n][j]; sh_l[warp][c] = __fmul_rn(x, kDown); }
+          const float b = FMT == KV8_INT8 ? -bias[n][j] : 0.f;
 #pragma unroll
-        for (int k = 0; k < MT; k += 2)
-          *reinterpret_cast<float4*>(&sh_o[warp][c][g * (HD / 8) + 2 * k]) = make_float4(o[n][k][j], o[n][k][2 + j], o[n][k + 1][j], o[n][k + 1][2 + j]);
-      }
+          for (int k = 0; k < MT; k += 2)
+            *reinterpret_cast<float4*>(&tile[c][g * (HD / 8) + 2 * k]) = make_float4(__fadd_rn(o[n][k][j], b), __fadd_rn(o[n][k][2 + j], b),
+                                                                                     __fadd_rn(o[n][k + 1][j], b), __fadd_rn(o[n][k + 1][2 + j], b));
+        }
+    }
     __syncthreads();
     for (int i = threadIdx.x; i < COLS * (HD / 4); i += kWarps * 32) {
       const int c = i / (HD / 4), d = i % (HD / 4) * 4, col = col0 + c;
@@ -512,15 +556,16 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_attn_kernel(
       const int tok = tok0 + col / gq, head = kvh * gq + col % gq;
       const int ns = splits_of(cnt == 1 ? last : min(a.tok_pos[tok], last), a.split_keys);
       if (split >= ns) continue;
-      float M = sh_m[0][c];
+      float M = kNoRef;
 #pragma unroll
-      for (int w = 1; w < kWarps; ++w) M = fmaxf(M, sh_m[w][c]);
+      for (int w = 0; w < kWarps; ++w) if (sh_at[w] >= 0) M = fmaxf(M, sh_m[w][c]);
       float L = 0.f;
       float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
+        if (sh_at[w] < 0) continue;
         const float f = ex2(__fadd_rn(sh_m[w][c], -M));
-        const float4 y = *reinterpret_cast<const float4*>(&sh_o[w][c][d]);
+        const float4 y = *reinterpret_cast<const float4*>(smem + sh_at[w] + (c * LDO + d) * 4);
         L = __fmaf_rn(sh_l[w][c], f, L);
         x.x = __fmaf_rn(y.x, f, x.x); x.y = __fmaf_rn(y.y, f, x.y); x.z = __fmaf_rn(y.z, f, x.z); x.w = __fmaf_rn(y.w, f, x.w);
       }
@@ -536,6 +581,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_attn_kernel(
         if (d == 0) *reinterpret_cast<float2*>(a.part_ml + slot * 2) = make_float2(M, L);
       }
     }
+    __syncthreads();                                // results have been read: their places take pages again
   }
 }
 
@@ -628,8 +674,8 @@ int run(const Kv8AttnArgs& a, cudaStream_t st) {
   const long items = (long)a.n_groups * a.hkv * a.max_splits * ((rows * gq + (wide ? 15 : 7)) / (wide ? 16 : 8));
   const unsigned grid = (unsigned)std::min<long>(items, 148 * (wide ? 2 : 3));
   auto kernel = wide ? kv8_attn_kernel<HD, FMT, 2> : kv8_attn_kernel<HD, FMT, 1>;
-  const size_t smem = wide ? attn_smem<HD, 2>() : attn_smem<HD, 1>();
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);     // of the current device
+  constexpr int smem = attn_smem<HD>();
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);     // of the current device
   if (e == cudaSuccess) e = launch(kernel, grid, kWarps * 32, smem, st, a);
   if (e == cudaSuccess && a.max_splits > 1) {
     // few rows with many splits: sixteen warps a CTA keep enough loads under way

@@ -13,16 +13,19 @@
 // finished there, the others leave (o, m, l) per split to kv8_join_kernel.  What a row adds up and in which order depends on its
 // own position alone, so a row has the same bits in a decode step, a verify block or any batch.
 //
-// Products.  The group's rows times the q heads of a KV head are the columns ("N" of the MMA, eight to a tile), keys are the rows
-// of K q^T and head channels the rows of V^T p^T, so a single decode row with eight q heads fills its tiles.  The order of
-// channels inside a product and of keys inside a page is free, and chosen so that every lane loads sixteen bytes of a row at a
-// time straight from global memory into its fragments; shared memory is not used on the way.  Only the weights need a
-// transposition between the products (movmatrix).
+// Products.  The group's rows times the q heads of a KV head are the columns, eight to a tile, so that a single decode row with
+// eight q heads wastes nothing.  S = q K^T takes q as A (its rows are the columns; for int8 the two bytes of eight columns) and K's
+// bytes as B just as they lie in shared memory; its result is, lane for lane, the B operand of O^T = V^T P^T, whose A are V's bytes
+// as fp16.  The order of channels inside a product and of keys inside a page is free, and chosen so that every lane reads sixteen
+// bytes of a row at a time and nothing has to be moved between lanes or registers.
 //
-// Range.  The weights reach the second product as fp16 numbers p_j vs_j.  m follows the largest s_j + log2 of vs_j's power of two,
-// so what is rounded is each key's contribution relative to the largest one, whatever the size of V; a key that has weight but no
-// V (a row of zeros has the least scale) cannot push the others out of fp16's range.  m is raised only when a column's largest
-// value has grown by 2^8 (fp16 has room for that), which leaves the accumulators alone for nearly all pages.
+// Loads.  Every warp copies its own pages, two at a time, into a ring of kStages pairs in shared memory (cp.async, no barrier but the
+// warp's) and runs ahead into the CTA's next item, whose page numbers were fetched an item earlier.
+//
+// Range.  The weights reach the second product as fp16 numbers p_j vs_j.  m is kept so that these stay below 2^kGrow: what is
+// rounded is each key's contribution relative to the largest one, whatever the size of V; a key that has weight but no V (a row
+// of zeros has the least scale) cannot push the others out of fp16's range.  m is raised only when a weight has passed 2^kGrow,
+// which leaves the accumulators alone for nearly all pages.
 #include <algorithm>
 #include <type_traits>
 
@@ -51,16 +54,9 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kStages = 2;                  // pairs of pages that a warp has in shared memory or under way
 constexpr float kNoRef = -3.4028234e38f;    // m before the first key
-constexpr float kGrow = 8.f;                // log2 of what a column may grow before m follows
-// l sums 2^(s - m) * 2^30 and the weights carry vs * 2^-30: with V of any size between 2^-64 and 2^121 neither leaves fp32
-constexpr float kUp = 30.f, kDown = 9.313225746154785e-10f;
+constexpr float kGrow = 256.f;              // what a weight may reach before m follows
 
 __device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
-__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
-  uint32_t y;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
-  return y;
-}
 __device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
   const __half2 v = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
@@ -69,15 +65,11 @@ __device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
 __device__ __forceinline__ void e4m3_pairs(uint32_t w, uint32_t& x, uint32_t& y) {
   asm("{ .reg .b16 lo, hi; mov.b32 {lo, hi}, %2; cvt.rn.f16x2.e4m3x2 %0, lo; cvt.rn.f16x2.e4m3x2 %1, hi; }" : "=r"(x), "=r"(y) : "r"(w));
 }
-// D(16x8, s32) += A(16x32, u8, row) * B(32x8, s8 or u8, col)
-template <bool SIGNED>
-__device__ __forceinline__ void mma_u8(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  if constexpr (SIGNED)
-    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  else
-    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.u8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+// D(16x8, s32) = A(16x32, s8, row) * B(32x8, u8, col) + C
+__device__ __forceinline__ void mma_s8u8(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, int c0, int c1, int c2, int c3) {
+  asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+               : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(c0), "r"(c1), "r"(c2), "r"(c3));
 }
 // Of two rows' words: pairs (row a, row b) of bytes 2 * HI and 2 * HI + 1
 template <int FMT, int HI>
@@ -126,33 +118,34 @@ __device__ __forceinline__ int splits_of(int last_key, int split_keys) { return 
 
 // Copies of blocks into the ring and where a lane finds its bytes there.  A block is looked at as 128-byte lines (one row of 128
 // channels, two of 64); the 16-byte pieces of a line are permuted so that the eight lanes of a load's phase hit different banks:
-// for K these are two rows times four neighbouring pieces, for V four rows times two.
+// for K these are two neighbouring rows times four pieces, for V every fourth row times two.
 template <int HD>
 struct Ring {
   static constexpr int kSlab = kKv8Page * HD;
-  uint32_t src, dst_k, dst_v[kSlab / 512];           // a lane's copies: 512 bytes a turn
+  uint32_t dst_k, dst_v[kSlab / 512];                // a lane's copies: 512 bytes a turn
   uint32_t rd_k, rd_v;
   __device__ __forceinline__ Ring(int lane) {
     const int g = lane >> 2, t = lane & 3, l4 = lane >> 3, c = lane & 7;
-    src = lane * 16;
-    // lines 4k + l4: K by the line's parity in units of two rows, V by fours of rows
-    dst_k = l4 * 128 + ((c ^ ((HD == 128 ? l4 >> 1 : l4) & 1) * 4) << 4);
+    // lines 4k + l4.  K: by the row's parity (rows of 64 channels lie right as they are); V: by the row / 4
+    dst_k = l4 * 128 + ((c ^ (HD == 128 ? (l4 & 1) * 4 : 0)) << 4);
 #pragma unroll
     for (int k = 0; k < kSlab / 512; ++k) dst_v[k] = kSlab + (4 * k + l4) * 128 + ((c ^ ((HD == 128 ? k : 2 * k + (l4 >> 1)) * 2)) << 4);
-    rd_k = HD == 128 ? 2 * g * 128 + ((t ^ (g & 1) * 4) << 4) : g * 128 + ((t ^ (g & 1) * 4) << 4);
+    rd_k = HD == 128 ? (4 * (g >> 1) + (g & 1)) * 128 + ((t ^ (g & 1) * 4) << 4) : 2 * (g >> 1) * 128 + ((g & 1) * 4 + t << 4);
     rd_v = kSlab + (HD == 128 ? 4 * t * 128 + ((g ^ t * 2) << 4) : 2 * t * 128 + (((g >> 1) ^ t * 2) << 4) + (g & 1) * 8);
   }
+  // `blk` is the block's address plus 16 * lane
   __device__ __forceinline__ void copy(uint32_t stage, const uint8_t* blk, int lane) const {
 #pragma unroll
     for (int k = 0; k < kSlab / 512; ++k) {
-      cp_async16(stage + dst_k + k * 512, blk + src + k * 512);
-      cp_async16(stage + dst_v[k], blk + kSlab + src + k * 512);
+      cp_async16(stage + dst_k + k * 512, blk + k * 512);
+      cp_async16(stage + dst_v[k], blk + kSlab + k * 512);
     }
-    if (lane < 8) cp_async16(stage + 2 * kSlab + src, blk + 2 * kSlab + src);
+    if (lane < 8) cp_async16(stage + 2 * kSlab + 16 * lane, blk + 2 * kSlab);
   }
-  __device__ __forceinline__ uint4 k(uint32_t stage, int r, int c) const {      // row 2g + r, piece t + 4c
-    if (HD == 128) return lds128(stage + ((rd_k + r * 128) ^ (c * 64)));
-    return lds128(stage + (rd_k ^ (r * 64)));
+  // row 4 (g / 2) + g % 2 + 2 r, piece t + 4c
+  __device__ __forceinline__ uint4 k(uint32_t stage, int r, int c) const {
+    if (HD == 128) return lds128(stage + r * 256 + (rd_k ^ (c * 64)));
+    return lds128(stage + r * 128 + rd_k);
   }
   __device__ __forceinline__ void v(uint32_t stage, int r, uint32_t (&w)[HD / 32]) const {     // row 4t + r, channels g * HD / 8 and on
     if constexpr (HD == 128) {
@@ -167,7 +160,7 @@ struct Ring {
 
 // One CTA's share of a group: keys of one split for eight or sixteen columns.
 struct Item {
-  int tok0, cnt, first, last, col0, kvh, split;
+  int tok0, cnt, first, last, seq, ns, col0, kvh, split;
   int n_my, page;                        // pages of this warp; lane i holds the number of page i
 };
 
@@ -177,13 +170,13 @@ constexpr int attn_smem() { return kWarps * kStages * 2 * kv8_block_bytes(HD); }
 template <int HD, int FMT, int NT>
 __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_attn_kernel(const Kv8AttnArgs a) {
   constexpr int KC = HD / 64;            // 16-byte pieces of a K row per lane
-  constexpr int KW = HD / 16;            // words of a K row per lane
   constexpr int VW = HD / 32;            // words of a V row per lane
-  constexpr int MT = HD / 16;            // channel tiles of V^T p^T
+  constexpr int MT = HD / 16;            // channel tiles of V^T P^T
+  constexpr int QM = FMT == KV8_INT8 ? NT : 1;            // A tiles of q: two bytes of eight columns, or sixteen columns in fp16
+  constexpr int QK = FMT == KV8_INT8 ? HD / 32 : HD / 16; // k-steps of q K^T
   constexpr int COLS = NT * 8;
   constexpr int LDO = HD + 4;
-  constexpr int BLK = kv8_block_bytes(HD);
-  constexpr int PAIR = 2 * BLK;
+  constexpr int BLK = kv8_block_bytes(HD), PAIR = 2 * BLK;
   // a warp's results of an item go over the pair of pages that it used last, which is not refilled before they have been read
   static_assert(COLS * LDO * 4 <= PAIR, "a tile of results fits a pair of pages");
   extern __shared__ __align__(128) uint8_t smem[];
@@ -220,77 +213,83 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_attn_kernel(
   const int item_end = item + share + (id < rest ? 1 : 0);
   if (item >= item_end) return;
   if (run != 0) load_run(0);
-  auto fetch = [&](int at, Item& it) {
-    while (at - base >= total) { base += total; load_run(run + 1); }
-    at -= base;
-    const int src = __ffs(__ballot_sync(0xffffffffu, incl > at)) - 1;
-    at -= __shfl_sync(0xffffffffu, incl, src) - __shfl_sync(0xffffffffu, mine, src);
-    it.tok0 = __shfl_sync(0xffffffffu, grp.tok0, src); it.cnt = __shfl_sync(0xffffffffu, grp.cnt, src);
-    it.first = __shfl_sync(0xffffffffu, grp.first, src); it.last = __shfl_sync(0xffffffffu, grp.last, src);
-    const int seq = __shfl_sync(0xffffffffu, grp.seq, src), ns = splits_of(it.last, a.split_keys);
-    const int ctiles = (it.cnt * gq + COLS - 1) / COLS;
-    it.split = at % ns; at /= ns;
-    it.col0 = at % ctiles * COLS; it.kvh = at / ctiles;
+  auto fetch = [&](int at, Item& it, bool next) {
+    if (next && it.split + 1 < it.ns) {
+      ++it.split;
+    } else {
+      while (at - base >= total) { base += total; load_run(run + 1); }
+      at -= base;
+      const int src = __ffs(__ballot_sync(0xffffffffu, incl > at)) - 1;
+      at -= __shfl_sync(0xffffffffu, incl, src) - __shfl_sync(0xffffffffu, mine, src);
+      it.tok0 = __shfl_sync(0xffffffffu, grp.tok0, src); it.cnt = __shfl_sync(0xffffffffu, grp.cnt, src);
+      it.first = __shfl_sync(0xffffffffu, grp.first, src); it.last = __shfl_sync(0xffffffffu, grp.last, src);
+      it.seq = __shfl_sync(0xffffffffu, grp.seq, src);
+      it.ns = splits_of(it.last, a.split_keys);
+      const int ctiles = (it.cnt * gq + COLS - 1) / COLS;
+      it.split = at % it.ns; at /= it.ns;
+      it.col0 = at % ctiles * COLS; it.kvh = at / ctiles;
+    }
     const int k_begin = it.split * a.split_keys, k_end = min(it.last + 1, k_begin + a.split_keys);
     const int n_pg = (k_end - k_begin + kKv8Page - 1) / kKv8Page;           // 0 for a group without keys
     it.n_my = (n_pg - warp + kWarps - 1) / kWarps;                          // at most 32: split_keys is at most 2048
     it.page = -1;
-    if (lane < it.n_my) it.page = a.block_table[(size_t)seq * a.bt_ld + k_begin / kKv8Page + warp + kWarps * lane];
+    if (lane < it.n_my) it.page = a.block_table[(size_t)it.seq * a.bt_ld + k_begin / kKv8Page + warp + kWarps * lane];
     __syncwarp();
   };
   Item cur, nxt;
-  fetch(item, nxt);
+  fetch(item, nxt, false);
   cur = nxt;
   cur.tok0 = -1;                         // no q yet
   int wr = 0, rd = 0, pending = 0;       // stages to fill and to read next; pairs sent for and not yet used
   // where this warp fetches (nxt once it is ahead of cur): pages left to send for and which come next
-  int f_i = 0, f_n = 0, f_page = 0, f_kvh = 0;
+  const int stride = a.hkv * BLK;
+  const uint8_t* f_base = nullptr;
+  int f_i = 0, f_n = 0, f_page = 0;
   bool ahead = false, more = true;
+  auto send = [&]() {                    // the next pair of pages, or a single last one
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      if (h == 1 && f_i + 1 >= f_n) break;
+      // a page that is not there: its keys are masked below, and something that is there is copied in their place
+      const int p = (int)min((unsigned)__shfl_sync(0xffffffffu, f_page, f_i + h), (unsigned)a.n_pages - 1u);
+      ring.copy(mem + wr + h * BLK, f_base + (long)p * stride, lane);
+    }
+    cp_async_commit();
+    wr ^= PAIR;
+    ++pending;
+    f_i += 2;
+  };
 
   // q, every column scaled by a power of two; qs undoes it on the scores and brings the softmax scale.
-  // int8: sixteen bits of fixed point, the largest value in [2^14, 2^15), as a signed and an unsigned byte (hi * 256 + lo): K's bytes
-  // then feed the product as they are, and the sums are exact.  What is lost is at most 2^-15 of the column's largest value, as much as
-  // a weight in fp16 loses.  The 128 in K's bytes comes off again with the accumulators' start, -128 * sum(q).
+  // int8: sixteen bits of fixed point, the largest value in [2^14, 2^15), as two signed bytes (hi * 256 + lo): K's bytes then feed the
+  // product as they are, and the sums are exact.  What is lost is at most 2^-15 of the column's largest value.  The 128 in K's
+  // bytes comes off again with the accumulators' start, -128 * sum(q).
   // e4m3: fp16 with the largest value in [2^10, 2^11), where a bf16 number stays exact down to 2^-24 of that.
-  uint32_t qb[NT][KW][2];
-  float qs[NT][2];
-  int q0[NT][2];
+  uint32_t qa[QM][QK][4];
+  float qs[NT];
+  int q0[NT];
 
   for (; item < item_end; ++item) {
     const bool same_q = nxt.tok0 == cur.tok0 && nxt.cnt == cur.cnt && nxt.col0 == cur.col0 && nxt.kvh == cur.kvh;
     cur = nxt;
-    if (!ahead) { f_i = 0; f_n = cur.n_my; f_page = cur.page; f_kvh = cur.kvh; }
+    if (!ahead) { f_i = 0; f_n = cur.n_my; f_page = cur.page; f_base = a.pool + cur.kvh * BLK + 16 * lane; }
     ahead = false;
     more = item + 1 < item_end;
-    if (more) fetch(item + 1, nxt);
+    if (more) fetch(item + 1, nxt, true);
     const int tok0 = cur.tok0, cnt = cur.cnt, first = cur.first, last = cur.last, col0 = cur.col0, kvh = cur.kvh, split = cur.split, n_my = cur.n_my;
     const int k_begin = split * a.split_keys, k_end = min(last + 1, k_begin + a.split_keys);
-    const unsigned valid = __ballot_sync(0xffffffffu, lane < n_my && (unsigned)cur.page < (unsigned)a.n_pages);
-    auto top_up = [&]() {
-      while (pending < kStages) {
-        if (f_i >= f_n) {
-          if (ahead || !more) return;
-          ahead = true;
-          f_i = 0; f_n = nxt.n_my; f_page = nxt.page; f_kvh = nxt.kvh;
-          continue;
-        }
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          if (h == 1 && f_i + 1 >= f_n) break;
-          int p = __shfl_sync(0xffffffffu, f_page, f_i + h);
-          if ((unsigned)p >= (unsigned)a.n_pages) {       // its keys are masked below; something there is copied in their place
-            if (lane == 0) atomicExch(a.status, (int)B2_ERR_BOUNDS);
-            p = 0;
-          }
-          ring.copy(mem + wr + h * BLK, a.pool + ((size_t)p * a.hkv + f_kvh) * BLK, lane);
-        }
-        cp_async_commit();
-        wr ^= PAIR;
-        ++pending;
-        f_i += 2;
+    const bool there = (unsigned)cur.page < (unsigned)a.n_pages;
+    if (lane < n_my && !there) atomicExch(a.status, (int)B2_ERR_BOUNDS);
+    const unsigned valid = __ballot_sync(0xffffffffu, lane < n_my && there);
+    while (pending < kStages) {
+      if (f_i >= f_n) {
+        if (ahead || !more) break;
+        ahead = true;
+        f_i = 0; f_n = nxt.n_my; f_page = nxt.page; f_base = a.pool + nxt.kvh * BLK + 16 * lane;
+        continue;
       }
-    };
-    top_up();
+      send();
+    }
 
     if (!same_q) {
 #pragma unroll
@@ -313,8 +312,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_attn_kernel(
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
         const uint32_t e = min((FMT == KV8_INT8 ? 268u : 264u) - (top >> 23), 253u);
         const float up = __uint_as_float(e << 23);
-        float down = __uint_as_float((254u - e) << 23) * a.scale_log2;
-        if (top >= 0x7f800000u) down = __uint_as_float(0x7fffffffu);           // an infinity or a NaN in q: a column of NaN
+        qs[n] = __fmul_rn(__uint_as_float((254u - e) << 23), a.scale_log2);
+        if (top >= 0x7f800000u) qs[n] = __uint_as_float(0x7fffffffu);           // an infinity or a NaN in q: a column of NaN
         int sum = 0;
 #pragma unroll
         for (int c = 0; c < KC; ++c)
@@ -323,36 +322,36 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_attn_kernel(
             const uint32_t a0 = (&raw[c][w >> 1].x)[2 * (w & 1)], a1 = (&raw[c][w >> 1].x)[2 * (w & 1) + 1];
             const float f0 = __uint_as_float(a0 << 16) * up, f1 = __uint_as_float(a0 & 0xffff0000u) * up;
             const float f2 = __uint_as_float(a1 << 16) * up, f3 = __uint_as_float(a1 & 0xffff0000u) * up;
-            if constexpr (FMT == KV8_INT8) {
-              const int i0 = __float2int_rn(f0), i1 = __float2int_rn(f1), i2 = __float2int_rn(f2), i3 = __float2int_rn(f3);
+            if constexpr (FMT == KV8_INT8) {           // rows g and g + 8 of the tile: hi and lo
+              // 32640 would need hi = 128: it becomes 32639
+              const int i0 = min(__float2int_rn(f0), 32639), i1 = min(__float2int_rn(f1), 32639);
+              const int i2 = min(__float2int_rn(f2), 32639), i3 = min(__float2int_rn(f3), 32639);
               sum += i0 + i1 + i2 + i3;
-              const uint32_t p01 = __byte_perm(i0, i1, 0x5140), p23 = __byte_perm(i2, i3, 0x5140);      // lo, lo, hi, hi
-              qb[n][c * 4 + w][0] = __byte_perm(p01, p23, 0x7632);
-              qb[n][c * 4 + w][1] = __byte_perm(p01, p23, 0x5410);
-            } else {
-              qb[n][c * 4 + w][0] = pack_half(f0, f1);
-              qb[n][c * 4 + w][1] = pack_half(f2, f3);
+              const int w2 = c * 2 + (w >> 1), half = 2 * (w & 1);
+              qa[n][w2][half] = __byte_perm(__byte_perm(i0 + 128, i1 + 128, 0x0051), __byte_perm(i2 + 128, i3 + 128, 0x0051), 0x5410);
+              qa[n][w2][half + 1] = __byte_perm(__byte_perm(i0, i1, 0x0040), __byte_perm(i2, i3, 0x0040), 0x5410);
+            } else {                                   // rows g and g + 8 of the tile: columns g and g + 8
+              qa[0][c * 4 + w][n] = pack_half(f0, f1);
+              qa[0][c * 4 + w][2 + n] = pack_half(f2, f3);
+              if (NT == 1) qa[0][c * 4 + w][1] = qa[0][c * 4 + w][3] = 0u;
             }
           }
-        qs[n][0] = __shfl_sync(0xffffffffu, down, 8 * t);
-        qs[n][1] = __shfl_sync(0xffffffffu, down, 8 * t + 4);
         if constexpr (FMT == KV8_INT8) {
           sum += __shfl_xor_sync(0xffffffffu, sum, 1);
           sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-          q0[n][0] = -128 * __shfl_sync(0xffffffffu, sum, 8 * t);
-          q0[n][1] = -128 * __shfl_sync(0xffffffffu, sum, 8 * t + 4);
+          q0[n] = -128 * sum;
         }
       }
     }
 
-    // m is the reference less kUp, so that 2^(s - m) carries the 2^30
-    float o[NT][MT][4], m[NT][2], l[NT][2];
+    // o: channels g * HD / 8 + 2k (0, 1) and + 1 (2, 3) of columns 2t (0, 2) and 2t + 1 (1, 3); m and l: of column g
+    float o[NT][MT][4], m[NT], l[NT];
     // int8: V's fp16 numbers are 1152 above the codes; the same sums of 1152 alone are taken off at the end.  Both lose alike to
     // the accumulators' truncation, 2^-23 of 1152 a step, so that what is left of it is a random part below 2^-10 of a code.
     float bias[NT][4];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      m[n][0] = m[n][1] = kNoRef; l[n][0] = l[n][1] = 0.f;
+      m[n] = kNoRef; l[n] = 0.f;
       bias[n][0] = bias[n][1] = bias[n][2] = bias[n][3] = 0.f;
 #pragma unroll
       for (int i = 0; i < MT; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
@@ -363,136 +362,141 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_attn_kernel(
       if (pending >= 2) cp_async_wait<1>(); else cp_async_wait<0>();
       __syncwarp();
       const uint32_t stage = mem + rd;
-      // s[h]: page i + h, keys 2g (0, 1) and 2g + 1 (2, 3), columns 2t (0, 2) and 2t + 1 (1, 3)
+      // s[h][n]: page i + h, column n * 8 + g, keys 4t .. 4t + 3
       float s[2][NT][4];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         if constexpr (FMT == KV8_INT8) {
-          int hi[NT][4], lo[NT][4];
+          int x[NT][2][4];                         // (hi, hi, lo, lo) of keys 4t + 2r, 4t + 2r + 1
 #pragma unroll
-          for (int n = 0; n < NT; ++n)
+          for (int r = 0; r < 2; ++r)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) { hi[n][j] = 0; lo[n][j] = q0[n][j & 1]; }
-#pragma unroll
-          for (int c = 0; c < KC; ++c) {
-            const uint4 k0 = ring.k(stage + h * BLK, 0, c), k1 = ring.k(stage + h * BLK, 1, c);
-#pragma unroll
-            for (int w = 0; w < 4; w += 2) {
-              const uint32_t f[4] = {(&k0.x)[w], (&k1.x)[w], (&k0.x)[w + 1], (&k1.x)[w + 1]};
+            for (int c = 0; c < KC; ++c) {
+              const uint4 k = ring.k(stage + h * BLK, r, c);
 #pragma unroll
               for (int n = 0; n < NT; ++n) {
-                mma_u8<true>(hi[n], f, qb[n][c * 4 + w][0], qb[n][c * 4 + w + 1][0]);
-                mma_u8<false>(lo[n], f, qb[n][c * 4 + w][1], qb[n][c * 4 + w + 1][1]);
+                int (&y)[4] = x[n][r];
+                if (c == 0) mma_s8u8(y, qa[n][0], k.x, k.y, 0, 0, q0[n], q0[n]);
+                else mma_s8u8(y, qa[n][2 * c], k.x, k.y, y[0], y[1], y[2], y[3]);
+                mma_s8u8(y, qa[n][2 * c + 1], k.z, k.w, y[0], y[1], y[2], y[3]);
               }
             }
-          }
 #pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) s[h][n][j] = __int2float_rn(hi[n][j] * 256 + lo[n][j]);
+            for (int j = 0; j < 4; ++j) s[h][n][j] = __int2float_rn(x[n][j >> 1][j & 1] * 256 + x[n][j >> 1][2 + (j & 1)]);
         } else {
 #pragma unroll
-          for (int n = 0; n < NT; ++n) s[h][n][0] = s[h][n][1] = s[h][n][2] = s[h][n][3] = 0.f;
+          for (int r = 0; r < 2; ++r) {
+            float x[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int c = 0; c < KC; ++c) {
-            const uint4 k0 = ring.k(stage + h * BLK, 0, c), k1 = ring.k(stage + h * BLK, 1, c);
+            for (int c = 0; c < KC; ++c) {
+              const uint4 k = ring.k(stage + h * BLK, r, c);
 #pragma unroll
-            for (int w = 0; w < 4; ++w) {
-              uint32_t f[4];
-              e4m3_pairs((&k0.x)[w], f[0], f[2]);
-              e4m3_pairs((&k1.x)[w], f[1], f[3]);
-#pragma unroll
-              for (int n = 0; n < NT; ++n) mma_f16_16816(s[h][n], f, qb[n][c * 4 + w][0], qb[n][c * 4 + w][1]);
+              for (int w = 0; w < 4; ++w) {
+                uint32_t b0, b1;
+                e4m3_pairs((&k.x)[w], b0, b1);
+                mma_f16_16816(x, qa[0][c * 4 + w], b0, b1);
+              }
             }
+#pragma unroll
+            for (int n = 0; n < NT; ++n) { s[h][n][2 * r] = x[2 * n]; s[h][n][2 * r + 1] = x[2 * n + 1]; }
           }
         }
       }
-      float e[2][2], vs[2][2];                      // of keys 2g, 2g + 1: log2 of V scale's power of two; V scale 2^-30
+      float vs[2][4];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint4 su = lds128(stage + h * BLK + 2 * kKv8Page * HD + g * 16);        // (K, V) scales of keys 2g, 2g + 1
-        e[h][0] = __uint_as_float(0x4b000000u | (su.y >> 23)) - 8388735.f;
-        e[h][1] = __uint_as_float(0x4b000000u | (su.w >> 23)) - 8388735.f;
-        vs[h][0] = __fmul_rn(__uint_as_float(su.y), kDown);
-        vs[h][1] = __fmul_rn(__uint_as_float(su.w), kDown);
+      for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+        for (int r = 0; r < 2; ++r) {
+          const uint4 su = lds128(stage + h * BLK + 2 * kKv8Page * HD + t * 32 + r * 16);       // (K, V) scales of two keys
+          vs[h][2 * r] = __uint_as_float(su.y); vs[h][2 * r + 1] = __uint_as_float(su.w);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) s[h][n][j] = __fmul_rn(__fmul_rn(s[h][n][j], __uint_as_float(j < 2 ? su.x : su.z)), qs[n][j & 1]);
-      }
+          for (int n = 0; n < NT; ++n) {
+            s[h][n][2 * r] = __fmul_rn(s[h][n][2 * r], __uint_as_float(su.x));
+            s[h][n][2 * r + 1] = __fmul_rn(s[h][n][2 * r + 1], __uint_as_float(su.z));
+          }
+        }
       const int kb = k_begin + (warp + kWarps * i) * kKv8Page;              // the pair's second page begins 64 keys later
       const unsigned have = valid >> i & 3u;
       // from the group's first slot on, at the split's end and where a page is missing, keys are looked at one by one
       const bool partly = kb + (kWarps + 1) * kKv8Page > min(first, k_end) || have != 3u;
       if (partly) {
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+        for (int n = 0; n < NT; ++n) {
+          const int row = min((col0 + n * 8 + g) / gq, cnt - 1);
+          const int pos = cnt == 1 ? last : min(a.tok_pos[tok0 + row], last);
+          const unsigned mask = a.tree_mask ? a.tree_mask[tok0 + row] : 0u;
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const int col = col0 + n * 8 + 2 * t + j, row = min(col / gq, cnt - 1);
-            const int pos = cnt == 1 ? last : min(a.tok_pos[tok0 + row], last);
-            const unsigned mask = a.tree_mask ? a.tree_mask[tok0 + row] : 0u;
+          for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-              for (int r = 0; r < 2; ++r) {
-                const int key = kb + h * kWarps * kKv8Page + 2 * g + r, in = key - first;
-                const bool seen = key <= pos && key < k_end && (have >> h & 1u) && (!a.tree_mask || in < 0 || (in < 32 && ((mask >> (in & 31)) & 1u)));
-                if (!seen) s[h][n][2 * r + j] = -INFINITY;
-              }
-          }
-      }
-      bool grows = false;
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const float top = fmaxf(fmaxf(__fadd_rn(s[0][n][j], e[0][0]), __fadd_rn(s[0][n][2 + j], e[0][1])),
-                                  fmaxf(__fadd_rn(s[1][n][j], e[1][0]), __fadd_rn(s[1][n][2 + j], e[1][1])));
-          grows |= top > __fadd_rn(m[n][j], kUp + kGrow);
-        }
-      if (__any_sync(0xffffffffu, grows)) {
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            float mx = fmaxf(fmaxf(__fadd_rn(s[0][n][j], e[0][0]), __fadd_rn(s[0][n][2 + j], e[0][1])),
-                             fmaxf(__fadd_rn(s[1][n][j], e[1][0]), __fadd_rn(s[1][n][2 + j], e[1][1])));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-            if (mx > __fadd_rn(m[n][j], kUp + kGrow)) {
-              const float f = ex2(__fadd_rn(m[n][j], kUp - mx));
-              m[n][j] = __fadd_rn(mx, -kUp);
-              l[n][j] = __fmul_rn(l[n][j], f);
-              bias[n][j] = __fmul_rn(bias[n][j], f);
-              bias[n][2 + j] = bias[n][j];
-#pragma unroll
-              for (int k = 0; k < MT; ++k) { o[n][k][j] = __fmul_rn(o[n][k][j], f); o[n][k][2 + j] = __fmul_rn(o[n][k][2 + j], f); }
+            for (int j = 0; j < 4; ++j) {
+              const int key = kb + h * kWarps * kKv8Page + 4 * t + j, in = key - first;
+              const bool seen = key <= pos && key < k_end && (have >> h & 1u) && (!a.tree_mask || in < 0 || (in < 32 && ((mask >> (in & 31)) & 1u)));
+              if (!seen) s[h][n][j] = -INFINITY;
             }
-          }
+        }
         __syncwarp();
       }
-      uint32_t pb[2][NT][2];
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
+      float w[2][NT][4];
+      float sum[NT];
+      auto weigh = [&]() {
+        float top = 0.f;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          float w[4];
+          sum[n] = 0.f;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float p = ex2(__fadd_rn(s[h][n][j], -m[n][j & 1]));
-            l[n][j & 1] = __fadd_rn(l[n][j & 1], p);
-            w[j] = __fmul_rn(p, vs[h][j >> 1]);
-          }
-          if (partly)                               // a row that is not seen may have the scale NaN
+          for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) if (s[h][n][j] == -INFINITY) w[j] = 0.f;
-          pb[h][n][0] = transpose8x8(pack_half(w[0], w[1]));
-          pb[h][n][1] = transpose8x8(pack_half(w[2], w[3]));
+            for (int j = 0; j < 4; ++j) {
+              const float p = ex2(__fmaf_rn(s[h][n][j], qs[n], -m[n]));
+              sum[n] = __fadd_rn(sum[n], p);
+              w[h][n][j] = __fmul_rn(p, vs[h][j]);
+            }
+          if (partly)             // a key that is not seen may have the scale NaN
+#pragma unroll
+            for (int j = 0; j < 8; ++j) if (s[j >> 2][n][j & 3] == -INFINITY) w[j >> 2][n][j & 3] = 0.f;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) top = fmaxf(top, w[j >> 2][n][j & 3]);
         }
+        return top;
+      };
+      if (__any_sync(0xffffffffu, weigh() > kGrow)) {
+        // columns that passed it: m becomes their largest s + log2 of vs's power of two, so that weights begin below 2 again
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          float top = 0.f, mx = kNoRef;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            top = fmaxf(top, w[j >> 2][n][j & 3]);
+            const float e = __uint_as_float(0x4b000000u | (__float_as_uint(vs[j >> 2][j & 3]) >> 23)) - 8388735.f;
+            mx = fmaxf(mx, __fadd_rn(__fmul_rn(s[j >> 2][n][j & 3], qs[n]), e));
+          }
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+          float f = 1.f;
+          if (top > kGrow) { f = ex2(__fadd_rn(m[n], -mx)); m[n] = mx; }
+          l[n] = __fmul_rn(l[n], f);
+          const float f0 = __shfl_sync(0xffffffffu, f, 8 * t), f1 = __shfl_sync(0xffffffffu, f, 8 * t + 4);
+#pragma unroll
+          for (int k = 0; k < MT; ++k) {
+            o[n][k][0] = __fmul_rn(o[n][k][0], f0); o[n][k][1] = __fmul_rn(o[n][k][1], f1);
+            o[n][k][2] = __fmul_rn(o[n][k][2], f0); o[n][k][3] = __fmul_rn(o[n][k][3], f1);
+          }
+          bias[n][0] = __fmul_rn(bias[n][0], f0); bias[n][1] = __fmul_rn(bias[n][1], f1);
+          bias[n][2] = bias[n][0]; bias[n][3] = bias[n][1];
+        }
+        weigh();
+      }
+#pragma unroll
+      for (int n = 0; n < NT; ++n) l[n] = __fadd_rn(l[n], sum[n]);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
+        uint32_t pb[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) { pb[n][0] = pack_half(w[h][n][0], w[h][n][1]); pb[n][1] = pack_half(w[h][n][2], w[h][n][3]); }
         uint32_t vw[4][VW];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
@@ -500,62 +504,72 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_attn_kernel(
           // bytes past the end may be e4m3's NaN, which a weight of zero does not silence
           if (FMT == KV8_FP8 && partly && (kb + h * kWarps * kKv8Page + 4 * t + r >= k_end || !(have >> h & 1u)))
 #pragma unroll
-            for (int w = 0; w < VW; ++w) vw[r][w] = 0u;
+            for (int x = 0; x < VW; ++x) vw[r][x] = 0u;
         }
         if (h == 1) {
           __syncwarp();                             // the pair has been read
           rd ^= PAIR;
           --pending;
-          if (i + 2 < n_my) top_up();               // the last pair's place holds the results first
+          if (i + 2 < n_my) {                       // the last pair's place holds the results first
+            if (f_i >= f_n && !ahead && more) {
+              ahead = true;
+              f_i = 0; f_n = nxt.n_my; f_page = nxt.page; f_base = a.pool + nxt.kvh * BLK + 16 * lane;
+            }
+            if (f_i < f_n) send();
+          }
         }
         if constexpr (FMT == KV8_INT8) {
           const uint32_t f[4] = {0x64806480u, 0x64806480u, 0x64806480u, 0x64806480u};         // 1152
 #pragma unroll
-          for (int n = 0; n < NT; ++n) mma_f16_16816(bias[n], f, pb[h][n][0], pb[h][n][1]);
+          for (int n = 0; n < NT; ++n) mma_f16_16816(bias[n], f, pb[n][0], pb[n][1]);
         }
 #pragma unroll
-        for (int w = 0; w < VW; ++w) {
+        for (int x = 0; x < VW; ++x) {
           uint32_t f[4];
-          cross_pairs<FMT, 0>(vw[0][w], vw[2][w], f[0], f[1]);
-          cross_pairs<FMT, 0>(vw[1][w], vw[3][w], f[2], f[3]);
+          cross_pairs<FMT, 0>(vw[0][x], vw[1][x], f[0], f[1]);
+          cross_pairs<FMT, 0>(vw[2][x], vw[3][x], f[2], f[3]);
 #pragma unroll
-          for (int n = 0; n < NT; ++n) mma_f16_16816(o[n][2 * w], f, pb[h][n][0], pb[h][n][1]);
-          cross_pairs<FMT, 1>(vw[0][w], vw[2][w], f[0], f[1]);
-          cross_pairs<FMT, 1>(vw[1][w], vw[3][w], f[2], f[3]);
+          for (int n = 0; n < NT; ++n) mma_f16_16816(o[n][2 * x], f, pb[n][0], pb[n][1]);
+          cross_pairs<FMT, 1>(vw[0][x], vw[1][x], f[0], f[1]);
+          cross_pairs<FMT, 1>(vw[2][x], vw[3][x], f[2], f[3]);
 #pragma unroll
-          for (int n = 0; n < NT; ++n) mma_f16_16816(o[n][2 * w + 1], f, pb[h][n][0], pb[h][n][1]);
+          for (int n = 0; n < NT; ++n) mma_f16_16816(o[n][2 * x + 1], f, pb[n][0], pb[n][1]);
         }
       }
     }
 
-    const int at = warp * kStages * PAIR + (rd ^ PAIR);
-    if (lane == 0) sh_at[warp] = n_my > 0 ? at : -1;
+    const int place = warp * kStages * PAIR + (rd ^ PAIR);
+    if (lane == 0) sh_at[warp] = n_my > 0 ? place : -1;
     if (n_my > 0) {
-      float (*tile)[LDO] = reinterpret_cast<float (*)[LDO]>(smem + at);
+      float (*tile)[LDO] = reinterpret_cast<float (*)[LDO]>(smem + place);
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+      for (int n = 0; n < NT; ++n) {
+        float x = l[n];
+        x = __fadd_rn(x, __shfl_xor_sync(0xffffffffu, x, 1));
+        x = __fadd_rn(x, __shfl_xor_sync(0xffffffffu, x, 2));
+        if (t == 0) { sh_m[warp][n * 8 + g] = m[n]; sh_l[warp][n * 8 + g] = x; }
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          float x = l[n][j];
-          x = __fadd_rn(x, __shfl_xor_sync(0xffffffffu, x, 4));
-          x = __fadd_rn(x, __shfl_xor_sync(0xffffffffu, x, 8));
-          x = __fadd_rn(x, __shfl_xor_sync(0xffffffffu, x, 16));
-          const int c = n * 8 + 2 * t + j;
-          if (g == 0) { sh_m[warp][c] = m[n][j]; sh_l[warp][c] = __fmul_rn(x, kDown); }
           const float b = FMT == KV8_INT8 ? -bias[n][j] : 0.f;
 #pragma unroll
           for (int k = 0; k < MT; k += 2)
-            *reinterpret_cast<float4*>(&tile[c][g * (HD / 8) + 2 * k]) = make_float4(__fadd_rn(o[n][k][j], b), __fadd_rn(o[n][k][2 + j], b),
-                                                                                     __fadd_rn(o[n][k + 1][j], b), __fadd_rn(o[n][k + 1][2 + j], b));
+            *reinterpret_cast<float4*>(&tile[n * 8 + 2 * t + j][g * (HD / 8) + 2 * k]) =
+                make_float4(__fadd_rn(o[n][k][j], b), __fadd_rn(o[n][k][2 + j], b), __fadd_rn(o[n][k + 1][j], b), __fadd_rn(o[n][k + 1][2 + j], b));
         }
+      }
     }
     __syncthreads();
+#pragma unroll
     for (int i = threadIdx.x; i < COLS * (HD / 4); i += kWarps * 32) {
       const int c = i / (HD / 4), d = i % (HD / 4) * 4, col = col0 + c;
       if (col >= cnt * gq) continue;
-      const int tok = tok0 + col / gq, head = kvh * gq + col % gq;
-      const int ns = splits_of(cnt == 1 ? last : min(a.tok_pos[tok], last), a.split_keys);
-      if (split >= ns) continue;
+      int tok = tok0, head = kvh * gq + col, ns = cur.ns;
+      if (cnt > 1) {
+        const int row = col / gq;
+        tok += row; head -= row * gq;
+        ns = splits_of(min(a.tok_pos[tok], last), a.split_keys);
+        if (split >= ns) continue;
+      }
       float M = kNoRef;
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) if (sh_at[w] >= 0) M = fmaxf(M, sh_m[w][c]);

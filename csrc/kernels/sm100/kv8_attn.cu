@@ -19,7 +19,7 @@
 // as fp16.  The order of channels inside a product and of keys inside a page is free, and chosen so that every lane reads sixteen
 // bytes of a row at a time and nothing has to be moved between lanes or registers.
 //
-// Loads.  Every warp copies its own pages, two at a time, into a ring of kStages pairs in shared memory (cp.async, no barrier but the
+// Loads.  Every warp copies its own pages, two at a time, into one of two places in shared memory (cp.async, no barrier but the
 // warp's) and runs ahead into the CTA's next item, whose page numbers were fetched an item earlier.
 //
 // Range.  The weights reach the second product as fp16 numbers p_j vs_j.  m is kept so that these stay below 2^kGrow: what is
@@ -52,7 +52,6 @@ struct Kv8AttnArgs {
 namespace {
 
 constexpr int kWarps = 4;
-constexpr int kStages = 2;                  // pairs of pages that a warp has in shared memory or under way
 constexpr float kNoRef = -3.4028234e38f;    // m before the first key
 constexpr float kGrow = 256.f;              // what a weight may reach before m follows
 
@@ -161,11 +160,11 @@ struct Ring {
 // One CTA's share of a group: keys of one split for eight or sixteen columns.
 struct Item {
   int tok0, cnt, first, last, seq, ns, col0, kvh, split;
-  int n_my, page;                        // pages of this warp; lane i holds the number of page i
+  int pairs, page;                       // pairs of pages of this warp, at least one; lane i holds the number of page i, -1 if none
 };
 
 template <int HD>
-constexpr int attn_smem() { return kWarps * kStages * 2 * kv8_block_bytes(HD); }
+constexpr int attn_smem() { return kWarps * 2 * 2 * kv8_block_bytes(HD); }
 
 template <int HD, int FMT, int NT>
 __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_attn_kernel(const Kv8AttnArgs a) {
@@ -187,7 +186,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_attn_kernel(
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int gq = a.hq / a.hkv;
   const Ring<HD> ring(lane);
-  const uint32_t mem = smem_u32(smem) + warp * kStages * PAIR;
+  const uint32_t mem = smem_u32(smem) + warp * 2 * PAIR, flip = mem ^ (mem + PAIR);
 
   // Items are numbered group after group and cut evenly over the CTAs; neighbours differ in the split first, so a CTA keeps its
   // q for most of them.  Every lane holds one group of a run of 32 and the number of items up to it.
@@ -231,33 +230,29 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_attn_kernel(
     }
     const int k_begin = it.split * a.split_keys, k_end = min(it.last + 1, k_begin + a.split_keys);
     const int n_pg = (k_end - k_begin + kKv8Page - 1) / kKv8Page;           // 0 for a group without keys
-    it.n_my = (n_pg - warp + kWarps - 1) / kWarps;                          // at most 32: split_keys is at most 2048
+    const int n_my = (n_pg - warp + kWarps - 1) / kWarps;                   // at most 32: split_keys is at most 2048
+    it.pairs = max((n_my + 1) >> 1, 1);
     it.page = -1;
-    if (lane < it.n_my) it.page = a.block_table[(size_t)it.seq * a.bt_ld + k_begin / kKv8Page + warp + kWarps * lane];
+    if (lane < n_my) it.page = a.block_table[(size_t)it.seq * a.bt_ld + k_begin / kKv8Page + warp + kWarps * lane];
     __syncwarp();
   };
   Item cur, nxt;
   fetch(item, nxt, false);
   cur = nxt;
-  cur.tok0 = -1;                         // no q yet
-  int wr = 0, rd = 0, pending = 0;       // stages to fill and to read next; pairs sent for and not yet used
-  // where this warp fetches (nxt once it is ahead of cur): pages left to send for and which come next
+  uint32_t rd = mem;                     // the pair in use; the other one is under way
   const int stride = a.hkv * BLK;
-  const uint8_t* f_base = nullptr;
-  int f_i = 0, f_n = 0, f_page = 0;
-  bool ahead = false, more = true;
-  auto send = [&]() {                    // the next pair of pages, or a single last one
+  // Sends for pair x of cur, or the first of nxt once cur has no more; every call is one group of copies, so that all but the last
+  // group have arrived when at most one is under way.  A page that is not there is not copied: its keys are masked below.
+  auto send = [&](uint32_t stage, int x) {
+    const bool mine = x < cur.pairs;
+    const uint8_t* base = a.pool + (mine ? cur.kvh : nxt.kvh) * BLK + 16 * lane;
+    const int page = mine ? cur.page : nxt.page, at = mine ? 2 * x : 0;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      if (h == 1 && f_i + 1 >= f_n) break;
-      // a page that is not there: its keys are masked below, and something that is there is copied in their place
-      const int p = (int)min((unsigned)__shfl_sync(0xffffffffu, f_page, f_i + h), (unsigned)a.n_pages - 1u);
-      ring.copy(mem + wr + h * BLK, f_base + (long)p * stride, lane);
+      const int p = __shfl_sync(0xffffffffu, page, at + h);
+      if ((unsigned)p < (unsigned)a.n_pages) ring.copy(stage + h * BLK, base + (long)p * stride, lane);
     }
     cp_async_commit();
-    wr ^= PAIR;
-    ++pending;
-    f_i += 2;
   };
 
   // q, every column scaled by a power of two; qs undoes it on the scores and brings the softmax scale.
@@ -269,27 +264,15 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_attn_kernel(
   float qs[NT];
   int q0[NT];
 
-  for (; item < item_end; ++item) {
-    const bool same_q = nxt.tok0 == cur.tok0 && nxt.cnt == cur.cnt && nxt.col0 == cur.col0 && nxt.kvh == cur.kvh;
+  send(rd, 0);
+  for (bool same_q = false; item < item_end; ++item) {
+    if (same_q) same_q = nxt.tok0 == cur.tok0 && nxt.cnt == cur.cnt && nxt.col0 == cur.col0 && nxt.kvh == cur.kvh;
     cur = nxt;
-    if (!ahead) { f_i = 0; f_n = cur.n_my; f_page = cur.page; f_base = a.pool + cur.kvh * BLK + 16 * lane; }
-    ahead = false;
-    more = item + 1 < item_end;
-    if (more) fetch(item + 1, nxt, true);
-    const int tok0 = cur.tok0, cnt = cur.cnt, first = cur.first, last = cur.last, col0 = cur.col0, kvh = cur.kvh, split = cur.split, n_my = cur.n_my;
+    if (item + 1 < item_end) fetch(item + 1, nxt, true); else nxt.page = -1;
+    const int tok0 = cur.tok0, cnt = cur.cnt, first = cur.first, last = cur.last, col0 = cur.col0, kvh = cur.kvh, split = cur.split, pairs = cur.pairs;
     const int k_begin = split * a.split_keys, k_end = min(last + 1, k_begin + a.split_keys);
-    const bool there = (unsigned)cur.page < (unsigned)a.n_pages;
-    if (lane < n_my && !there) atomicExch(a.status, (int)B2_ERR_BOUNDS);
-    const unsigned valid = __ballot_sync(0xffffffffu, lane < n_my && there);
-    while (pending < kStages) {
-      if (f_i >= f_n) {
-        if (ahead || !more) break;
-        ahead = true;
-        f_i = 0; f_n = nxt.n_my; f_page = nxt.page; f_base = a.pool + nxt.kvh * BLK + 16 * lane;
-        continue;
-      }
-      send();
-    }
+    const unsigned valid = __ballot_sync(0xffffffffu, (unsigned)cur.page < (unsigned)a.n_pages);
+    send(rd ^ flip, 1);
 
     if (!same_q) {
 #pragma unroll
@@ -343,6 +326,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_attn_kernel(
         }
       }
     }
+    same_q = true;
 
     // o: channels g * HD / 8 + 2k (0, 1) and + 1 (2, 3) of columns 2t (0, 2) and 2t + 1 (1, 3); m and l: of column g
     float o[NT][MT][4], m[NT], l[NT];
@@ -357,12 +341,11 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_attn_kernel(
       for (int i = 0; i < MT; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
     }
 
-    for (int i = 0; i < n_my; i += 2) {
-      // this pair has arrived once no more copies are under way than were sent for after it
-      if (pending >= 2) cp_async_wait<1>(); else cp_async_wait<0>();
+    for (int i = 0; i < pairs; ++i) {
+      cp_async_wait<1>();
       __syncwarp();
-      const uint32_t stage = mem + rd;
-      // s[h][n]: page i + h, column n * 8 + g, keys 4t .. 4t + 3
+      const uint32_t stage = rd;
+      // s[h][n]: page 2i + h of this warp, column n * 8 + g, keys 4t .. 4t + 3
       float s[2][NT][4];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -417,8 +400,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_attn_kernel(
             s[h][n][2 * r + 1] = __fmul_rn(s[h][n][2 * r + 1], __uint_as_float(su.z));
           }
         }
-      const int kb = k_begin + (warp + kWarps * i) * kKv8Page;              // the pair's second page begins 64 keys later
-      const unsigned have = valid >> i & 3u;
+      const int kb = k_begin + (warp + 2 * kWarps * i) * kKv8Page;          // the pair's second page begins 64 keys later
+      const unsigned have = valid >> 2 * i & 3u;
       // from the group's first slot on, at the split's end and where a page is missing, keys are looked at one by one
       const bool partly = kb + (kWarps + 1) * kKv8Page > min(first, k_end) || have != 3u;
       if (partly) {
@@ -508,14 +491,9 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_attn_kernel(
         }
         if (h == 1) {
           __syncwarp();                             // the pair has been read
-          rd ^= PAIR;
-          --pending;
-          if (i + 2 < n_my) {                       // the last pair's place holds the results first
-            if (f_i >= f_n && !ahead && more) {
-              ahead = true;
-              f_i = 0; f_n = nxt.n_my; f_page = nxt.page; f_base = a.pool + nxt.kvh * BLK + 16 * lane;
-            }
-            if (f_i < f_n) send();
+          if (i + 1 < pairs) {                      // the last pair's place holds the results first
+            send(rd, i + 2);
+            rd ^= flip;
           }
         }
         if constexpr (FMT == KV8_INT8) {
@@ -538,24 +516,22 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_attn_kernel(
       }
     }
 
-    const int place = warp * kStages * PAIR + (rd ^ PAIR);
-    if (lane == 0) sh_at[warp] = n_my > 0 ? place : -1;
-    if (n_my > 0) {
-      float (*tile)[LDO] = reinterpret_cast<float (*)[LDO]>(smem + place);
+    float (*tile)[LDO] = reinterpret_cast<float (*)[LDO]>(smem + (rd - smem_u32(smem)));
+    if (lane == 0) sh_at[warp] = rd - smem_u32(smem);
+    rd ^= flip;
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        float x = l[n];
-        x = __fadd_rn(x, __shfl_xor_sync(0xffffffffu, x, 1));
-        x = __fadd_rn(x, __shfl_xor_sync(0xffffffffu, x, 2));
-        if (t == 0) { sh_m[warp][n * 8 + g] = m[n]; sh_l[warp][n * 8 + g] = x; }
+    for (int n = 0; n < NT; ++n) {
+      float x = l[n];
+      x = __fadd_rn(x, __shfl_xor_sync(0xffffffffu, x, 1));
+      x = __fadd_rn(x, __shfl_xor_sync(0xffffffffu, x, 2));
+      if (t == 0) { sh_m[warp][n * 8 + g] = m[n]; sh_l[warp][n * 8 + g] = x; }
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const float b = FMT == KV8_INT8 ? -bias[n][j] : 0.f;
+      for (int j = 0; j < 2; ++j) {
+        const float b = FMT == KV8_INT8 ? -bias[n][j] : 0.f;
 #pragma unroll
-          for (int k = 0; k < MT; k += 2)
-            *reinterpret_cast<float4*>(&tile[n * 8 + 2 * t + j][g * (HD / 8) + 2 * k]) =
-                make_float4(__fadd_rn(o[n][k][j], b), __fadd_rn(o[n][k][2 + j], b), __fadd_rn(o[n][k + 1][j], b), __fadd_rn(o[n][k + 1][2 + j], b));
-        }
+        for (int k = 0; k < MT; k += 2)
+          *reinterpret_cast<float4*>(&tile[n * 8 + 2 * t + j][g * (HD / 8) + 2 * k]) =
+              make_float4(__fadd_rn(o[n][k][j], b), __fadd_rn(o[n][k][2 + j], b), __fadd_rn(o[n][k + 1][j], b), __fadd_rn(o[n][k + 1][2 + j], b));
       }
     }
     __syncthreads();
@@ -570,14 +546,13 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_attn_kernel(
         ns = splits_of(min(a.tok_pos[tok], last), a.split_keys);
         if (split >= ns) continue;
       }
-      float M = kNoRef;
+      float M = sh_m[0][c];
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) if (sh_at[w] >= 0) M = fmaxf(M, sh_m[w][c]);
+      for (int w = 1; w < kWarps; ++w) M = fmaxf(M, sh_m[w][c]);
       float L = 0.f;
       float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
-        if (sh_at[w] < 0) continue;
         const float f = ex2(__fadd_rn(sh_m[w][c], -M));
         const float4 y = *reinterpret_cast<const float4*>(smem + sh_at[w] + (c * LDO + d) * 4);
         L = __fmaf_rn(sh_l[w][c], f, L);
@@ -596,6 +571,9 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_attn_kernel(
       }
     }
     __syncthreads();                                // results have been read: their places take pages again
+    // pages that are named and not there: reported once an item, -1 past the split's end is none
+    const int n_pg = (k_end - k_begin + kKv8Page - 1) / kKv8Page;
+    if (warp + kWarps * lane < n_pg && !(valid >> lane & 1u)) atomicExch(a.status, (int)B2_ERR_BOUNDS);
   }
 }
 

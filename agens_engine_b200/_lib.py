@@ -161,7 +161,7 @@ class Kv8AttnArgs(C.Structure):
         ("out", C.c_void_p), ("ldo", C.c_long),
         ("status", C.c_void_p),
         ("split_keys", C.c_int), ("max_splits", C.c_int),
-        ("part_o", C.c_void_p), ("part_ml", C.c_void_p), ("counters", C.c_void_p),
+        ("part_o", C.c_void_p), ("part_ml", C.c_void_p),
     ]
 
 

@@ -23,7 +23,6 @@ PAGE = 16
 FORMATS = {"int8": 0, "fp8": 1}
 GROUP_ROWS = 32                    # most rows of one attention group (bits of a tree mask)
 MAX_SPLIT = 2048                   # most keys of one split
-JOIN = 16                          # neighbouring splits that are joined at once
 
 
 def block_bytes(hd: int) -> int:
@@ -47,44 +46,11 @@ def split_keys_for(max_ctx: int) -> int:
     return s
 
 
-class Kv8Workspace:
-    """What splits leave for one another: partial results, and counters that are zero between calls.  One workspace serves calls that run
-    one after the other, of any sizes; calls that may run at the same time (on two streams, in two graphs) need one each."""
-
-    def __init__(self, device, n_tok: int = 0, hq: int = 1, hd: int = 128, max_ctx: int = 1, split_keys: Optional[int] = None):
-        self.part = torch.empty(0, dtype=torch.float32, device=device)
-        self.counters = torch.zeros(0, dtype=torch.int32, device=device)
-        self._outgrown = []
-        if n_tok:
-            self.ensure(n_tok * hq, hd, -(-max_ctx // (split_keys or split_keys_for(max_ctx))))
-
-    def ensure(self, rows: int, hd: int, splits: int):
-        """Room for ``rows`` pairs of a token and a q head.  What it replaces is kept: graphs captured before go on using it."""
-        if splits < 2:
-            return
-        have, need = self.part.numel(), rows * splits * (hd + 2)
-        if need > have:
-            self._outgrown.append(self.part)
-            self.part = torch.empty(max(need, have + have // 2), dtype=torch.float32, device=self.part.device)
-        have, need = self.counters.numel(), rows * (-(-splits // JOIN) + 1)
-        if need > have:
-            self._outgrown.append(self.counters)
-            self.counters = torch.zeros(max(need, have + have // 2), dtype=torch.int32, device=self.counters.device)
-
-
-_default_ws: dict = {}
-
-
-def _workspace(device, dev: int) -> Kv8Workspace:
-    """The workspace of a call that brings none.  Eager calls of a stream run one after the other and share one; a captured call has its
-    own, since its graph may run at any time."""
-    if torch.cuda.is_current_stream_capturing():
-        return Kv8Workspace(device)
-    key = (dev, torch._C._cuda_getCurrentRawStream(dev))
-    ws = _default_ws.get(key)
-    if ws is None:
-        ws = _default_ws[key] = Kv8Workspace(device)
-    return ws
+def part_floats(n_tok: int, hq: int, hd: int, max_ctx: int, split_keys: Optional[int] = None) -> int:
+    """fp32 entries of the workspace that :func:`attn_decode8` needs for ``n_tok`` rows (0: none).  One workspace serves any number
+    of calls one after the other; calls that may run at the same time need one each, captured ones too."""
+    splits = -(-max_ctx // (split_keys or split_keys_for(max_ctx)))
+    return n_tok * hq * splits * (hd + 2) if splits > 1 else 0
 
 
 # Launches of a step follow one another every few microseconds, so the checks are written to cost little when they pass: one
@@ -210,19 +176,18 @@ def rope_kvstore8(qkv: torch.Tensor, hq: int, hkv: int, hd: int, inv_freq: torch
 
 def attn_decode8(q: torch.Tensor, pool: torch.Tensor, fmt: str, block_table: torch.Tensor, grp_tok0: torch.Tensor, grp_cnt: torch.Tensor,
                  tok_pos: torch.Tensor, tok_seq: torch.Tensor, hq: int, hkv: int, hd: int, split_keys: Optional[int] = None,
-                 max_ctx: Optional[int] = None, ws: Optional[Kv8Workspace] = None, tree_mask: Optional[torch.Tensor] = None,
+                 max_ctx: Optional[int] = None, part: Optional[torch.Tensor] = None, tree_mask: Optional[torch.Tensor] = None,
                  status: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Attention of new rows over 8-bit pages: ``attention.attn_decode`` for a pool of this module.  ``q``: bf16
     ``[n_tok, hq * hd]`` (RoPE applied).  Group ``g`` is the ``grp_cnt[g]`` (at most 32) rows from ``grp_tok0[g]`` on, all of one
     sequence in ascending order of ``tok_pos``, whose K and V are in the pool already; row i sees the slots up to ``tok_pos[i]``, of
     the slots from the group's first on those whose bit its ``tree_mask`` (int32 ``[n_tok]``) has.  A row that sees nothing
-    (``tok_pos`` -1 in a group of its own, an empty mask) gives zeros; rows of no group are left as they were in ``out``, a row of two
-    groups is not defined.
+    (``tok_pos`` -1 in a group of its own, an empty mask) gives zeros; rows of no group are left as they were in ``out``.
 
     ``split_keys`` (a multiple of 16, at most 2048; default :func:`split_keys_for` the table's length) cuts every sequence into
     splits that are joined at the end; a row's bits depend on its own position and on ``split_keys`` only.  ``max_ctx`` (default:
-    the table's length) bounds the positions.  ``ws``: where splits meet (default: one that the stream's eager calls share, a captured
-    call's own).  Returns bf16 ``[n_tok, hq * hd]``."""
+    the table's length) bounds the positions, ``part`` is a workspace of :func:`part_floats` entries (default: allocated for the
+    call).  Returns bf16 ``[n_tok, hq * hd]``."""
     f, dev = _format(fmt), q.get_device()
     n = q.shape[0]
     if hkv < 1 or hq < 1 or hq % hkv:
@@ -247,23 +212,19 @@ def attn_decode8(q: torch.Tensor, pool: torch.Tensor, fmt: str, block_table: tor
     elif not PAGE <= split_keys <= MAX_SPLIT or split_keys % PAGE:
         _fail(f"split_keys: a multiple of {PAGE} up to {MAX_SPLIT}")
     splits = -(-max_ctx // split_keys)
+    slots = n * hq * splits if splits > 1 else 0
+    if part is not None and not (part.dtype is _F32 and part.is_contiguous() and part.numel() >= slots * (hd + 2) and part.get_device() == dev
+                                 and part.data_ptr() % 16 == 0):
+        _fail(f"part: contiguous fp32 with at least {slots * (hd + 2)} entries on the device of the rows")
     if status is None:
         status = torch.zeros(1, dtype=_I32, device=q.device)
     at_status = _check_index(status, 1, dev, "status")
     if n and n_groups:
-        at_o = at_ml = at_cnt8 = 0
-        if splits > 1:
-            if dev < 0:
-                _fail("tensors on a CUDA device")
-            if ws is None:
-                ws = _workspace(q.device, dev)
-            ws.ensure(n * hq, hd, splits)
-            if ws.part.get_device() != dev:
-                _fail("the workspace is on the device of the rows")
-            at_o = ws.part.data_ptr()
-            at_ml, at_cnt8 = at_o + 4 * n * hq * splits * hd, ws.counters.data_ptr()
+        if part is None and slots:
+            part = torch.empty(slots * (hd + 2), dtype=_F32, device=q.device)
+        at_o = part.data_ptr() if slots else 0
         a = Kv8AttnArgs(q.data_ptr(), ldq, pool.data_ptr(), pool.shape[0], block_table.data_ptr(), bt_ld, cols, seqs, at_tok0, at_cnt, n_groups, at_pos, at_seq, n,
-                        at_mask, hq, hkv, _LOG2E / math.sqrt(hd), out.data_ptr(), ldo, at_status, split_keys, splits, at_o, at_ml, at_cnt8)
+                        at_mask, hq, hkv, _LOG2E / math.sqrt(hd), out.data_ptr(), ldo, at_status, split_keys, splits, at_o, at_o + 4 * slots * hd)
         _launch("b2_kv8_attn", dev, a, hd, f)
     return out
 

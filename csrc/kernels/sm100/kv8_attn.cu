@@ -10,10 +10,8 @@
 //
 // Split.  A sequence's keys are cut every split_keys keys, a constant of the engine; one CTA of four warps takes the keys of one
 // (group, KV head, columns, split), page i of them on warp i % 4, and joins its warps in shared memory.  Rows with one split are
-// finished there.  The others leave (o, m, l) of every split in the workspace; of sixteen neighbouring splits the CTA that comes last
-// (a counter that wraps to zero by itself) joins them in order, and where a row has more than sixteen, the CTA whose sixteen come last
-// joins those.  What a row adds up and in which order depends on its own position alone, so a row has the same bits in a
-// decode step, a verify block or any batch.  A kernel of its own for the join cost 3 us at one row of 700 keys, 7 us at 24 rows of 4001.
+// finished there, the others leave (o, m, l) per split to kv8_join_kernel.  What a row adds up and in which order depends on its
+// own position alone, so a row has the same bits in a decode step, a verify block or any batch.
 //
 // Products.  The group's rows times the q heads of a KV head are the columns, eight to a tile, so that a single decode row with
 // eight q heads wastes nothing.  S = q K^T takes q as A (its rows are the columns; for int8 the two bytes of eight columns) and K's
@@ -47,16 +45,13 @@ struct Kv8AttnArgs {
   bf16* out; long ldo;
   int* status;
   int split_keys, max_splits;
-  // unused when max_splits is 1
-  float* part_o;                            // [n_tok][hq][max_splits][hd]
+  float* part_o;                            // [n_tok][hq][max_splits][hd]; unused when max_splits is 1
   float* part_ml;                           // [n_tok][hq][max_splits][2]
-  unsigned* counters;                       // [n_tok * hq][ceil(max_splits / 16) + 1], zero before and after every launch
 };
 
 namespace {
 
 constexpr int kWarps = 4;
-constexpr int kJoin = 16;                   // splits of a block that are joined at once
 constexpr float kNoRef = -3.4028234e38f;    // m before the first key
 constexpr float kGrow = 256.f;              // what a weight may reach before m follows
 
@@ -101,14 +96,6 @@ __device__ __forceinline__ uint2 lds64(uint32_t addr) {
   uint2 v;
   asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr) : "memory");
   return v;
-}
-
-// One more arrival at a counter that wraps to zero after `of`: whether it was the last.  Releases what the CTA has written (after
-// its barrier) and acquires what the others have.
-__device__ __forceinline__ bool arrive(unsigned* counter, unsigned of) {
-  unsigned old;
-  asm volatile("atom.acq_rel.gpu.global.inc.u32 %0, [%1], %2;" : "=r"(old) : "l"(counter), "r"(of - 1) : "memory");
-  return old == of - 1;
 }
 
 struct Group { int tok0, cnt, first, last, seq; bool ok; };
@@ -176,63 +163,6 @@ struct Item {
   int pairs, page;                       // pairs of pages of this warp, at least one; lane i holds the number of page i, -1 if none
 };
 
-// Columns of a task whose parts are to be joined: parts first, first + step, ... (n of them) of every row that has so many.
-// blk >= 0: a block of sixteen splits, which is the row's result if the row has no other; else the blocks of the row.
-template <int HD, int COLS>
-__device__ __forceinline__ void join_parts(const Kv8AttnArgs& a, int tok0, int cnt, int last, int col0, int kvh, int blk) {
-  constexpr int PER = HD / 32;
-  using Vec = std::conditional_t<PER == 4, float4, float2>;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gq = a.hq / a.hkv;
-  for (int c = warp; c < COLS; c += kWarps) {
-    const int col = col0 + c;
-    if (col >= cnt * gq) break;
-    const int row = col / gq, tok = tok0 + row, head = kvh * gq + col - row * gq;
-    const int ns = splits_of(cnt == 1 ? last : min(a.tok_pos[tok], last), a.split_keys), blocks = (ns + kJoin - 1) / kJoin;
-    const int n = blk >= 0 ? min(ns - blk * kJoin, kJoin) : blocks, step = blk >= 0 ? 1 : kJoin;
-    if (n < 1 || ns == 1 || (blk < 0 && blocks == 1)) continue;
-    const size_t slot = ((size_t)tok * a.hq + head) * a.max_splits + (blk > 0 ? blk * kJoin : 0);
-    float2* ml = reinterpret_cast<float2*>(a.part_ml) + slot;
-    Vec* po = reinterpret_cast<Vec*>(a.part_o + slot * HD) + lane;
-    float M = kNoRef;
-    for (int i = lane; i < n; i += 32) M = fmaxf(M, __ldcg(&ml[i * step]).x);
-    M = warp_max(M);
-    float L = 0.f, x[PER];
-#pragma unroll
-    for (int d = 0; d < PER; ++d) x[d] = 0.f;
-    for (int i0 = 0; i0 < n; i0 += kJoin) {
-      Vec y[kJoin];
-      float f[kJoin], l[kJoin];
-#pragma unroll
-      for (int j = 0; j < kJoin; ++j) {                // past the end: the last part again, with the weight zero
-        const int i = min(i0 + j, n - 1) * step;
-        const float2 w = __ldcg(&ml[i]);
-        y[j] = __ldcg(&po[(size_t)i * 32]);
-        f[j] = w.x; l[j] = w.y;
-      }
-#pragma unroll
-      for (int j = 0; j < kJoin; ++j) {
-        const float w = i0 + j < n ? ex2(__fadd_rn(f[j], -M)) : 0.f;
-        L = __fmaf_rn(l[j], w, L);
-#pragma unroll
-        for (int d = 0; d < PER; ++d) x[d] = __fmaf_rn((&y[j].x)[d], w, x[d]);
-      }
-    }
-    if (blk < 0 || blocks == 1) {
-      const float inv = L == 0.f ? 0.f : __fdiv_rn(1.f, L);
-      bf16* out = a.out + (size_t)tok * a.ldo + (size_t)head * HD + lane * PER;
-#pragma unroll
-      for (int d = 0; d < PER; d += 2) *reinterpret_cast<__nv_bfloat162*>(out + d) = __floats2bfloat162_rn(__fmul_rn(x[d], inv), __fmul_rn(x[d + 1], inv));
-    } else {
-      Vec y;
-#pragma unroll
-      for (int d = 0; d < PER; ++d) (&y.x)[d] = x[d];
-      *po = y;
-      __syncwarp();                                  // every lane has read the block's weights
-      if (lane == 0) *ml = make_float2(M, L);
-    }
-  }
-}
-
 template <int HD>
 constexpr int attn_smem() { return kWarps * 2 * 2 * kv8_block_bytes(HD); }
 
@@ -250,7 +180,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_attn_kernel(
   static_assert(COLS * LDO * 4 <= PAIR, "a tile of results fits a pair of pages");
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float sh_m[kWarps][COLS], sh_l[kWarps][COLS];
-  __shared__ int sh_at[kWarps], sh_join, sh_last[8];
+  __shared__ int sh_at[kWarps];
   pdl_wait();
   pdl_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -333,23 +263,6 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_attn_kernel(
   uint32_t qa[QM][QK][4];
   float qs[NT];
   int q0[NT];
-
-  // The CTA's last arrival at a counter: thread 0 alone has the answer until the next barrier, an item later.
-  bool arrived = false, was_last = false;
-  auto tell = [&]() {                    // thread 0, before a barrier
-    if (threadIdx.x == 0) sh_join = arrived && was_last;
-  };
-  auto join = [&]() {                    // all, after it
-    if (!sh_join) return;
-    const int tok0 = sh_last[0], cnt = sh_last[1], last = sh_last[2], col0 = sh_last[3], kvh = sh_last[4], blk = sh_last[5], ns = sh_last[6];
-    const int blocks = (ns + kJoin - 1) / kJoin;
-    join_parts<HD, COLS>(a, tok0, cnt, last, col0, kvh, blk);
-    if (blocks == 1) return;
-    __syncthreads();
-    if (threadIdx.x == 0) sh_join = arrive(a.counters + ((size_t)tok0 * a.hq + (kvh * gq * cnt + col0)) * (((size_t)a.max_splits + kJoin - 1) / kJoin + 1), blocks);
-    __syncthreads();
-    if (sh_join) join_parts<HD, COLS>(a, tok0, cnt, last, col0, kvh, -1);
-  };
 
   send(rd, 0);
   for (bool same_q = false; item < item_end; ++item) {
@@ -605,7 +518,6 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_attn_kernel(
 
     float (*tile)[LDO] = reinterpret_cast<float (*)[LDO]>(smem + (rd - smem_u32(smem)));
     if (lane == 0) sh_at[warp] = rd - smem_u32(smem);
-    tell();
     rd ^= flip;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -658,24 +570,79 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_attn_kernel(
         if (d == 0) *reinterpret_cast<float2*>(a.part_ml + slot * 2) = make_float2(M, L);
       }
     }
-    join();                                         // what the item before was the last of
     __syncthreads();                                // results have been read: their places take pages again
-    if (threadIdx.x == 0) {
-      arrived = cur.ns > 1;
-      if (arrived) {
-        const int blk = split / kJoin;
-        was_last = arrive(a.counters + ((size_t)tok0 * a.hq + (kvh * gq * cnt + col0)) * (((size_t)a.max_splits + kJoin - 1) / kJoin + 1) + 1 + blk,
-                          min(cur.ns - blk * kJoin, kJoin));
-        sh_last[0] = tok0; sh_last[1] = cnt; sh_last[2] = last; sh_last[3] = col0; sh_last[4] = kvh; sh_last[5] = blk; sh_last[6] = cur.ns;
-      }
-    }
     // pages that are named and not there: reported once an item, -1 past the split's end is none
     const int n_pg = (k_end - k_begin + kKv8Page - 1) / kKv8Page;
     if (warp + kWarps * lane < n_pg && !(valid >> lane & 1u)) atomicExch(a.status, (int)B2_ERR_BOUNDS);
   }
-  tell();
-  __syncthreads();
-  join();
+}
+
+// Joins the splits of rows that have more than one: a CTA per (group, row, q head).  Sixteen sums, sum j of the splits j, j + 16, ...
+// in order, are added in order of j.  WARPS warps take 16 / WARPS sums each, side by side; both variants give the same bits.
+template <int HD, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32) kv8_join_kernel(const Kv8AttnArgs a, int rows_at_once) {
+  constexpr int PER = HD / 32, SETS = 16, MY = SETS / WARPS, AHEAD = 8 / MY;
+  using Vec = std::conditional_t<PER == 4, float4, float2>;
+  __shared__ float sh[SETS][HD + 1];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  pdl_wait();
+  pdl_launch_dependents();
+  const int head = blockIdx.x % a.hq, r0 = blockIdx.x / a.hq % rows_at_once;
+  const Group grp = group_at(a, blockIdx.x / a.hq / rows_at_once);
+  if (!grp.ok) return;
+  for (int r = r0; r < grp.cnt; r += rows_at_once) {
+    const int tok = grp.tok0 + r;
+    const int ns = splits_of(grp.cnt == 1 ? grp.last : min(a.tok_pos[tok], grp.last), a.split_keys);
+    if (ns == 1) continue;
+    const size_t slot = ((size_t)tok * a.hq + head) * a.max_splits;
+    const Vec* po = reinterpret_cast<const Vec*>(a.part_o + slot * HD) + lane;
+    const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + slot;
+    float M = kNoRef;
+    for (int s = lane; s < ns; s += 32) M = fmaxf(M, ml[s].x);
+    M = warp_max(M);
+    float L[MY], x[MY][PER];
+#pragma unroll
+    for (int k = 0; k < MY; ++k) {
+      L[k] = 0.f;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) x[k][i] = 0.f;
+    }
+    for (int s0 = warp * MY; s0 < ns; s0 += AHEAD * SETS) {
+      float2 w[AHEAD][MY];
+      Vec y[AHEAD][MY];
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j)
+#pragma unroll
+        for (int k = 0; k < MY; ++k) {                 // past the end: the last split again, with the weight zero
+          const int s = min(s0 + j * SETS + k, ns - 1);
+          w[j][k] = ml[s];
+          y[j][k] = po[(size_t)s * 32];
+        }
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j)
+#pragma unroll
+        for (int k = 0; k < MY; ++k) {
+          const float f = s0 + j * SETS + k < ns ? ex2(__fadd_rn(w[j][k].x, -M)) : 0.f;
+          L[k] = __fmaf_rn(w[j][k].y, f, L[k]);
+#pragma unroll
+          for (int i = 0; i < PER; ++i) x[k][i] = __fmaf_rn((&y[j][k].x)[i], f, x[k][i]);
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < MY; ++k) {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) sh[warp * MY + k][lane * PER + i] = x[k][i];
+      if (lane == 0) sh[warp * MY + k][HD] = L[k];
+    }
+    __syncthreads();
+    for (int d = threadIdx.x; d < HD; d += WARPS * 32) {
+      float sum = sh[0][d], Ls = sh[0][HD];
+#pragma unroll
+      for (int w = 1; w < SETS; ++w) { sum = __fadd_rn(sum, sh[w][d]); Ls = __fadd_rn(Ls, sh[w][HD]); }
+      a.out[(size_t)tok * a.ldo + (size_t)head * HD + d] = __float2bfloat16_rn(Ls == 0.f ? 0.f : __fmul_rn(sum, __fdiv_rn(1.f, Ls)));
+    }
+    __syncthreads();
+  }
 }
 
 template <class K, class... A>
@@ -702,6 +669,12 @@ int run(const Kv8AttnArgs& a, cudaStream_t st) {
   constexpr int smem = attn_smem<HD>();
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);     // of the current device
   if (e == cudaSuccess) e = launch(kernel, grid, kWarps * 32, smem, st, a);
+  if (e == cudaSuccess && a.max_splits > 1) {
+    // few rows with many splits: sixteen warps a CTA keep enough loads under way
+    const unsigned blocks = (unsigned)(a.n_groups * rows * a.hq);
+    e = a.max_splits > 16 && blocks <= 148 * 4 ? launch(kv8_join_kernel<HD, 16>, blocks, 512, 0, st, a, (int)rows)
+                                               : launch(kv8_join_kernel<HD, 4>, blocks, 128, 0, st, a, (int)rows);
+  }
   return e == cudaSuccess ? B2_OK : B2_ERR_LAUNCH;
 }
 
@@ -715,7 +688,7 @@ B2_API int b2_kv8_attn(const Kv8AttnArgs* args, int hd, int fmt, cudaStream_t st
   if (a.n_groups < 1 || a.n_tok < 1 || a.hkv < 1 || a.hq < 1 || a.hq % a.hkv || a.n_seq < 1 || a.bt_cols < 1 || a.n_pages < 1) return B2_ERR_ARG;
   if ((hd != 64 && hd != 128) || (fmt != KV8_INT8 && fmt != KV8_FP8) || a.ldq % 8 || a.ldo % 8) return B2_ERR_ARG;
   if (a.split_keys < kKv8Page || a.split_keys > 2048 || a.split_keys % kKv8Page || a.max_splits < 1) return B2_ERR_ARG;
-  if (a.max_splits > 1 && (!a.part_o || !a.part_ml || !a.counters)) return B2_ERR_ARG;
+  if (a.max_splits > 1 && (!a.part_o || !a.part_ml)) return B2_ERR_ARG;
   // item and block numbers are 32-bit
   if (a.bt_cols > (1 << 26) || (long)a.n_groups * a.hq * 32 * a.max_splits > 0x7fff0000l || ((long)a.n_tok + a.n_groups) * a.hq > 0x7fffffffl) return B2_ERR_ARG;
   if (hd == 128) return fmt == KV8_INT8 ? run<128, KV8_INT8>(a, st) : run<128, KV8_FP8>(a, st);

@@ -51,7 +51,8 @@ BAD_ATTN = [
     (dict(tok_pos=torch.zeros(2, dtype=torch.int32)), "tok_pos"), (dict(tree_mask=torch.zeros(3, dtype=torch.int64)), "tree_mask"),
     (dict(tree_mask=torch.zeros(2, dtype=torch.int32)), "tree_mask"), (dict(block_table=torch.zeros(1, 4)), "block_table"),
     (dict(split_keys=40), "split_keys"), (dict(split_keys=4096), "split_keys"), (dict(split_keys=0), "split_keys"), (dict(max_ctx=65), "max_ctx"), (dict(max_ctx=0), "max_ctx"),
-    (dict(split_keys=16), "CUDA device"), (dict(), "CUDA device"),
+    (dict(split_keys=16, part=torch.zeros(3 * HQ * 4 * (HD + 2) - 1)), "part"), (dict(part=torch.zeros(9999, dtype=torch.float64)), "part"),
+    (dict(split_keys=16, part=torch.zeros(3 * HQ * 4 * (HD + 2))), "CUDA device"), (dict(), "CUDA device"),
 ]
 
 
@@ -98,16 +99,7 @@ def test_the_library_refuses_what_the_launchers_would_not_pass_on():
 
 def test_splits_for_a_context():
     assert [K.split_keys_for(n) for n in (1, 256, 16384, 16385, 32769, 131072, 1 << 20)] == [256, 256, 256, 512, 1024, 2048, 2048]
-    ws = K.Kv8Workspace("cpu")
-    ws.ensure(24, 128, 1)
-    assert ws.part.numel() == ws.counters.numel() == 0
-    ws.ensure(24, 128, 17)
-    assert ws.part.numel() == 24 * 17 * 130 and ws.counters.numel() == 24 * 3 and not bool(ws.counters.any())
-    before = ws.part
-    ws.ensure(24, 64, 20)                                     # fits
-    ws.ensure(25, 128, 17)
-    assert ws.part.numel() == 24 * 17 * 130 * 3 // 2 and any(t is before for t in ws._outgrown)
-    assert K.Kv8Workspace("cpu", 2, 4, 64, 100, 16).part.numel() == 2 * 4 * 7 * 66
+    assert K.part_floats(3, 8, 128, 256) == 0 and K.part_floats(3, 8, 128, 257) == 3 * 8 * 2 * 130 and K.part_floats(1, 2, 64, 100, 16) == 2 * 7 * 66
 
 
 @pytest.mark.parametrize("fmt", FMTS)

@@ -52,6 +52,7 @@ struct Kv8AttnArgs {
 namespace {
 
 constexpr int kWarps = 4;
+constexpr int kJoin = 16;                   // splits that are joined at once
 constexpr float kNoRef = -3.4028234e38f;    // m before the first key
 constexpr float kGrow = 256.f;              // what a weight may reach before m follows
 
@@ -577,71 +578,80 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_attn_kernel(
   }
 }
 
-// Joins the splits of rows that have more than one: a CTA per (group, row, q head).  Sixteen sums, sum j of the splits j, j + 16, ...
-// in order, are added in order of j.  WARPS warps take 16 / WARPS sums each, side by side; both variants give the same bits.
-template <int HD, int WARPS>
-__global__ void __launch_bounds__(WARPS * 32) kv8_join_kernel(const Kv8AttnArgs a, int rows_at_once) {
-  constexpr int PER = HD / 32, SETS = 16, MY = SETS / WARPS, AHEAD = 8 / MY;
+// Joins the splits of rows that have more than one.  A block of kJoin neighbouring splits is one warp's: all its parts are under way
+// at once and added in order.  `warps` of them share a (row, q head); block b is warp b % 16's, the warps' sums are added in order.
+// With warps == 1 (rows of at most sixteen splits) a CTA has four (row, q head)s.  Neither choice changes a row's bits.
+template <int HD>
+__global__ void __launch_bounds__(512) kv8_join_kernel(const Kv8AttnArgs a, int rows_at_once, int warps) {
+  constexpr int PER = HD / 32;
   using Vec = std::conditional_t<PER == 4, float4, float2>;
-  __shared__ float sh[SETS][HD + 1];
+  __shared__ float sh_x[16][HD], sh_m[16], sh_l[16];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int task = warps == 1 ? blockIdx.x * 4 + warp : blockIdx.x, w = warps == 1 ? 0 : warp;
+  const int head = task % a.hq, r0 = task / a.hq % rows_at_once;
+  // (groups and positions are from before the kernel that this one follows, which has waited for them)
+  const Group grp = group_at(a, task / a.hq / rows_at_once);
   pdl_wait();
   pdl_launch_dependents();
-  const int head = blockIdx.x % a.hq, r0 = blockIdx.x / a.hq % rows_at_once;
-  const Group grp = group_at(a, blockIdx.x / a.hq / rows_at_once);
   if (!grp.ok) return;
   for (int r = r0; r < grp.cnt; r += rows_at_once) {
     const int tok = grp.tok0 + r;
     const int ns = splits_of(grp.cnt == 1 ? grp.last : min(a.tok_pos[tok], grp.last), a.split_keys);
     if (ns == 1) continue;
     const size_t slot = ((size_t)tok * a.hq + head) * a.max_splits;
-    const Vec* po = reinterpret_cast<const Vec*>(a.part_o + slot * HD) + lane;
-    const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + slot;
-    float M = kNoRef;
-    for (int s = lane; s < ns; s += 32) M = fmaxf(M, ml[s].x);
-    M = warp_max(M);
-    float L[MY], x[MY][PER];
+    float M = kNoRef, L = 0.f, x[PER];
 #pragma unroll
-    for (int k = 0; k < MY; ++k) {
-      L[k] = 0.f;
+    for (int d = 0; d < PER; ++d) x[d] = 0.f;
+    for (int s0 = w * kJoin; s0 < ns; s0 += warps * kJoin) {
+      const int n = min(ns - s0, kJoin);
+      const float2 part = lane < n ? reinterpret_cast<const float2*>(a.part_ml)[slot + s0 + lane] : make_float2(kNoRef, 0.f);
+      const Vec* po = reinterpret_cast<const Vec*>(a.part_o + (slot + s0) * HD) + lane;
+      Vec y[kJoin];
 #pragma unroll
-      for (int i = 0; i < PER; ++i) x[k][i] = 0.f;
+      for (int j = 0; j < kJoin; ++j) y[j] = po[min(j, n - 1) * 32];        // past the end: the last part again, with the weight zero
+      const float m = warp_max(part.x), M2 = fmaxf(M, m), f = lane < n ? ex2(__fadd_rn(part.x, -m)) : 0.f;
+      float z[PER], l = warp_sum(__fmul_rn(part.y, f));
+#pragma unroll
+      for (int d = 0; d < PER; ++d) z[d] = 0.f;
+#pragma unroll
+      for (int j = 0; j < kJoin; ++j) {
+        const float fj = __shfl_sync(0xffffffffu, f, j);
+#pragma unroll
+        for (int d = 0; d < PER; ++d) z[d] = __fmaf_rn((&y[j].x)[d], fj, z[d]);
+      }
+      const float old = ex2(__fadd_rn(M, -M2)), add = ex2(__fadd_rn(m, -M2));
+      M = M2;
+      L = __fmaf_rn(l, add, __fmul_rn(L, old));
+#pragma unroll
+      for (int d = 0; d < PER; ++d) x[d] = __fmaf_rn(z[d], add, __fmul_rn(x[d], old));
     }
-    for (int s0 = warp * MY; s0 < ns; s0 += AHEAD * SETS) {
-      float2 w[AHEAD][MY];
-      Vec y[AHEAD][MY];
+    if (warps > 1 && ns > kJoin) {
 #pragma unroll
-      for (int j = 0; j < AHEAD; ++j)
+      for (int d = 0; d < PER; ++d) sh_x[warp][lane * PER + d] = x[d];
+      if (lane == 0) { sh_m[warp] = M; sh_l[warp] = L; }
+      __syncthreads();
+      if (warp == 0)
+        for (int v = 1; v < warps; ++v) M = fmaxf(M, sh_m[v]);
+      const float own = ex2(__fadd_rn(sh_m[0], -M));
+      if (warp == 0) {
+        L = __fmul_rn(L, own);
 #pragma unroll
-        for (int k = 0; k < MY; ++k) {                 // past the end: the last split again, with the weight zero
-          const int s = min(s0 + j * SETS + k, ns - 1);
-          w[j][k] = ml[s];
-          y[j][k] = po[(size_t)s * 32];
+        for (int d = 0; d < PER; ++d) x[d] = __fmul_rn(x[d], own);
+        for (int v = 1; v < warps; ++v) {
+          const float f = ex2(__fadd_rn(sh_m[v], -M));
+          L = __fmaf_rn(sh_l[v], f, L);
+#pragma unroll
+          for (int d = 0; d < PER; ++d) x[d] = __fmaf_rn(sh_x[v][lane * PER + d], f, x[d]);
         }
-#pragma unroll
-      for (int j = 0; j < AHEAD; ++j)
-#pragma unroll
-        for (int k = 0; k < MY; ++k) {
-          const float f = s0 + j * SETS + k < ns ? ex2(__fadd_rn(w[j][k].x, -M)) : 0.f;
-          L[k] = __fmaf_rn(w[j][k].y, f, L[k]);
-#pragma unroll
-          for (int i = 0; i < PER; ++i) x[k][i] = __fmaf_rn((&y[j][k].x)[i], f, x[k][i]);
-        }
+      }
+      __syncthreads();
     }
+    if (w == 0) {
+      const float inv = L == 0.f ? 0.f : __fdiv_rn(1.f, L);
+      bf16* out = a.out + (size_t)tok * a.ldo + (size_t)head * HD + lane * PER;
 #pragma unroll
-    for (int k = 0; k < MY; ++k) {
-#pragma unroll
-      for (int i = 0; i < PER; ++i) sh[warp * MY + k][lane * PER + i] = x[k][i];
-      if (lane == 0) sh[warp * MY + k][HD] = L[k];
+      for (int d = 0; d < PER; d += 2) *reinterpret_cast<__nv_bfloat162*>(out + d) = __floats2bfloat162_rn(__fmul_rn(x[d], inv), __fmul_rn(x[d + 1], inv));
     }
-    __syncthreads();
-    for (int d = threadIdx.x; d < HD; d += WARPS * 32) {
-      float sum = sh[0][d], Ls = sh[0][HD];
-#pragma unroll
-      for (int w = 1; w < SETS; ++w) { sum = __fadd_rn(sum, sh[w][d]); Ls = __fadd_rn(Ls, sh[w][HD]); }
-      a.out[(size_t)tok * a.ldo + (size_t)head * HD + d] = __float2bfloat16_rn(Ls == 0.f ? 0.f : __fmul_rn(sum, __fdiv_rn(1.f, Ls)));
-    }
-    __syncthreads();
   }
 }
 
@@ -670,10 +680,9 @@ int run(const Kv8AttnArgs& a, cudaStream_t st) {
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);     // of the current device
   if (e == cudaSuccess) e = launch(kernel, grid, kWarps * 32, smem, st, a);
   if (e == cudaSuccess && a.max_splits > 1) {
-    // few rows with many splits: sixteen warps a CTA keep enough loads under way
-    const unsigned blocks = (unsigned)(a.n_groups * rows * a.hq);
-    e = a.max_splits > 16 && blocks <= 148 * 4 ? launch(kv8_join_kernel<HD, 16>, blocks, 512, 0, st, a, (int)rows)
-                                               : launch(kv8_join_kernel<HD, 4>, blocks, 128, 0, st, a, (int)rows);
+    const int warps = std::min((a.max_splits + kJoin - 1) / kJoin, 16);
+    const long tasks = (long)a.n_groups * rows * a.hq;
+    e = launch(kv8_join_kernel<HD>, (unsigned)(warps == 1 ? (tasks + 3) / 4 : tasks), warps == 1 ? 128 : 32 * warps, 0, st, a, (int)rows, warps);
   }
   return e == cudaSuccess ? B2_OK : B2_ERR_LAUNCH;
 }

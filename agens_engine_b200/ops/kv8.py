@@ -37,19 +37,22 @@ def make_pool(n_pages: int, hkv: int, hd: int, device) -> torch.Tensor:
     return torch.zeros(n_pages, hkv, block_bytes(hd), dtype=torch.uint8, device=device)
 
 
-def split_keys_for(max_ctx: int) -> int:
-    """Keys of one attention split for contexts of up to ``max_ctx`` tokens: 256, doubled while more than 64 splits were needed.  A
-    constant of the engine, since a row's bits depend on it."""
-    s = 256
-    while s < MAX_SPLIT and s * 64 < max_ctx:
+def split_keys_for(max_ctx: int, heads: int = 8) -> int:
+    """Keys of one attention split for ``heads`` pairs of a sequence and a KV head with contexts of up to ``max_ctx`` tokens: 128, doubled
+    up to 512 while that makes more splits than CTAs run at once, and beyond while a context had more than 256.  A constant of the
+    engine, since a row's bits depend on it."""
+    s = 128
+    while s < 512 and heads * -(-max_ctx // s) > 444:
+        s *= 2
+    while s < MAX_SPLIT and s * 256 < max_ctx:
         s *= 2
     return s
 
 
-def part_floats(n_tok: int, hq: int, hd: int, max_ctx: int, split_keys: Optional[int] = None) -> int:
+def part_floats(n_tok: int, hq: int, hd: int, max_ctx: int, split_keys: int) -> int:
     """fp32 entries of the workspace that :func:`attn_decode8` needs for ``n_tok`` rows (0: none).  One workspace serves any number
     of calls one after the other; calls that may run at the same time need one each, captured ones too."""
-    splits = -(-max_ctx // (split_keys or split_keys_for(max_ctx)))
+    splits = -(-max_ctx // split_keys)
     return n_tok * hq * splits * (hd + 2) if splits > 1 else 0
 
 
@@ -184,7 +187,7 @@ def attn_decode8(q: torch.Tensor, pool: torch.Tensor, fmt: str, block_table: tor
     the slots from the group's first on those whose bit its ``tree_mask`` (int32 ``[n_tok]``) has.  A row that sees nothing
     (``tok_pos`` -1 in a group of its own, an empty mask) gives zeros; rows of no group are left as they were in ``out``.
 
-    ``split_keys`` (a multiple of 16, at most 2048; default :func:`split_keys_for` the table's length) cuts every sequence into
+    ``split_keys`` (a multiple of 16, at most 2048; default :func:`split_keys_for` the table's size) cuts every sequence into
     splits that are joined at the end; a row's bits depend on its own position and on ``split_keys`` only.  ``max_ctx`` (default:
     the table's length) bounds the positions, ``part`` is a workspace of :func:`part_floats` entries (default: allocated for the
     call).  Returns bf16 ``[n_tok, hq * hd]``."""
@@ -208,7 +211,7 @@ def attn_decode8(q: torch.Tensor, pool: torch.Tensor, fmt: str, block_table: tor
     elif not 0 < max_ctx <= cols * PAGE:
         _fail(f"max_ctx: 1 .. {cols * PAGE}, what the block table holds")
     if split_keys is None:
-        split_keys = split_keys_for(max_ctx)
+        split_keys = split_keys_for(max_ctx, seqs * hkv)
     elif not PAGE <= split_keys <= MAX_SPLIT or split_keys % PAGE:
         _fail(f"split_keys: a multiple of {PAGE} up to {MAX_SPLIT}")
     splits = -(-max_ctx // split_keys)

@@ -38,47 +38,54 @@ __device__ __forceinline__ uint2 pack4(const float (&f)[4]) {
 }
 
 // Rotation (pairs i, i + hd/2) by pos * inv_freq, q rounded once to bf16, k and v quantised from fp32.
-// HD / 8 lanes hold a head, four rotary pairs each, so a warp takes 32 / (HD / 8) heads at a time.
+// HD / 8 lanes hold a head, four rotary pairs each, so a warp takes 32 / (HD / 8) heads at a time ("a turn") and has the next turn's
+// loads under way meanwhile.  `parts` CTAs share a token; each takes the token's sines and cosines once.
 template <int HD, int FMT>
-__global__ void __launch_bounds__(256) kv8_store_kernel(const Kv8StoreArgs a, int warps_per_tok) {
+__global__ void __launch_bounds__(256) kv8_store_kernel(const Kv8StoreArgs a, int parts) {
   constexpr int LPH = HD / 8, HPW = 32 / LPH, HALF = HD / 2;
+  __shared__ __align__(16) float sh_c[HALF], sh_s[HALF];
   pdl_wait();
   pdl_launch_dependents();
-  const int lane = threadIdx.x & 31, l = lane % LPH;
-  const long gw = (long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-  const int tok = (int)(gw / warps_per_tok), w = (int)(gw % warps_per_tok);
-  if (tok >= a.n) return;
+  const int lane = threadIdx.x & 31, l = lane % LPH, sub = lane / LPH;
+  const int tok = blockIdx.x / parts, part = blockIdx.x % parts;
+  const int heads = a.hq + 2 * a.hkv, turns = (heads + HPW - 1) / HPW;
+  int turn = part * 8 + (threadIdx.x >> 5);
+  const bf16* row = a.qkv + (size_t)tok * a.ld + l * 4;
+  uint2 lo2 = make_uint2(0u, 0u), hi2 = lo2;
+  auto load = [&](int t) {
+    const int head = t * HPW + sub;
+    if (t < turns && head < heads) {
+      lo2 = ld_nc_v2(row + (size_t)head * HD);
+      hi2 = ld_nc_v2(row + (size_t)head * HD + HALF);
+    }
+  };
+  load(turn);
   const int pos = a.tok_pos[tok], seq = a.tok_seq[tok];
-  int page = -1;
-  if (pos >= 0 && pos / kKv8Page < a.bt_cols && seq >= 0 && seq < a.n_seq) page = a.block_table[(size_t)seq * a.bt_ld + pos / kKv8Page];
-  const bool stored = page >= 0 && page < a.n_pages;
-  if (!stored && lane == 0) atomicExch(a.status, (int)B2_ERR_BOUNDS);
 
   // The angle in turns, in 64 bits: a 32-bit product of a position of 100000 and a frequency near one is off by several
   // thousandths of a radian.  Its fraction goes to sincospi, which needs no argument reduction of its own.
-  float c[4], s[4];
-  const int rpos = a.rope_pos ? a.rope_pos[tok] : pos;
-  const float4 f4 = *reinterpret_cast<const float4*>(a.inv_freq + l * 4);
-  const float fr[4] = {f4.x, f4.y, f4.z, f4.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int p = a.rope_pos3 ? a.rope_pos3[(size_t)min((int)a.pair_axis[l * 4 + i], 2) * a.n + tok] : rpos;
-    double t = (double)p * (double)fr[i] * 0.15915494309189535;
+  if (threadIdx.x < HALF) {
+    const int i = threadIdx.x;
+    int p = a.rope_pos ? a.rope_pos[tok] : pos;
+    if (a.rope_pos3) p = a.rope_pos3[(size_t)min((int)a.pair_axis[i], 2) * a.n + tok];
+    double t = (double)p * (double)a.inv_freq[i] * 0.15915494309189535;
     t -= rint(t);
-    sincospif((float)(2.0 * t), &s[i], &c[i]);
+    sincospif((float)(2.0 * t), &sh_s[i], &sh_c[i]);
   }
+  int page = -1;
+  if (pos >= 0 && pos / kKv8Page < a.bt_cols && seq >= 0 && seq < a.n_seq) page = a.block_table[(size_t)seq * a.bt_ld + pos / kKv8Page];
+  const bool stored = page >= 0 && page < a.n_pages;
+  if (!stored && part == 0 && threadIdx.x == 0) atomicExch(a.status, (int)B2_ERR_BOUNDS);
+  __syncthreads();
+  const float4 c4 = *reinterpret_cast<const float4*>(sh_c + l * 4), s4 = *reinterpret_cast<const float4*>(sh_s + l * 4);
+  const float c[4] = {c4.x, c4.y, c4.z, c4.w}, s[4] = {s4.x, s4.y, s4.z, s4.w};
 
-  const int heads = a.hq + 2 * a.hkv;
-  const int turns = (heads + HPW - 1) / HPW;
-  for (int turn = w; turn < turns; turn += warps_per_tok) {
-    const int head = turn * HPW + lane / LPH;
-    const bool live = head < heads;
-    float lo[4] = {0.f, 0.f, 0.f, 0.f}, hi[4] = {0.f, 0.f, 0.f, 0.f};
-    if (live) {
-      const bf16* src = a.qkv + (size_t)tok * a.ld + (size_t)head * HD + l * 4;
-      unpack4(*reinterpret_cast<const uint2*>(src), lo);
-      unpack4(*reinterpret_cast<const uint2*>(src + HALF), hi);
-    }
+  for (; turn < turns; turn += 8 * parts) {
+    const int head = turn * HPW + sub;
+    float lo[4], hi[4];
+    unpack4(lo2, lo);
+    unpack4(hi2, hi);
+    load(turn + 8 * parts);
     if (head < a.hq + a.hkv) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -87,18 +94,19 @@ __global__ void __launch_bounds__(256) kv8_store_kernel(const Kv8StoreArgs a, in
         hi[i] = y * c[i] + x * s[i];
       }
     }
-    if (live && head < a.hq) {
+    if (head < a.hq) {
       bf16* dst = a.q_out + (size_t)tok * a.ldq + (size_t)head * HD + l * 4;
       *reinterpret_cast<uint2*>(dst) = pack4(lo);
       *reinterpret_cast<uint2*>(dst + HALF) = pack4(hi);
     }
+    if (turn * HPW + HPW <= a.hq) continue;            // q heads only, for the whole warp
     // the largest magnitude, compared as bits: a NaN's are above an infinity's, so neither is lost
     uint32_t mx = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) mx = max(mx, max(__float_as_uint(lo[i]) & 0x7fffffffu, __float_as_uint(hi[i]) & 0x7fffffffu));
 #pragma unroll
     for (int o = LPH / 2; o > 0; o >>= 1) mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-    if (!live || head < a.hq || !stored) continue;
+    if (head >= heads || head < a.hq || !stored) continue;
     const bool is_v = head >= a.hq + a.hkv;
     const int kvh = head - a.hq - (is_v ? a.hkv : 0), slot = pos % kKv8Page;
     const float scale = fmaxf(__fdiv_rn(__uint_as_float(mx), FMT == KV8_INT8 ? 127.f : 448.f), kKv8MinScale);
@@ -111,48 +119,51 @@ __global__ void __launch_bounds__(256) kv8_store_kernel(const Kv8StoreArgs a, in
       chi |= kv8_code<FMT>(__fdiv_rn(hi[i], scale)) << (8 * i);
     }
     uint8_t* blk = a.pool + ((size_t)page * a.hkv + kvh) * kv8_block_bytes(HD);
-    uint8_t* row = blk + (is_v ? kKv8Page * HD : 0) + slot * HD + l * 4;
-    *reinterpret_cast<uint32_t*>(row) = clo;
-    *reinterpret_cast<uint32_t*>(row + HALF) = chi;
+    uint8_t* codes = blk + (is_v ? kKv8Page * HD : 0) + slot * HD + l * 4;
+    *reinterpret_cast<uint32_t*>(codes) = clo;
+    *reinterpret_cast<uint32_t*>(codes + HALF) = chi;
     if (l == 0) reinterpret_cast<float*>(blk + 2 * kKv8Page * HD)[slot * 2 + is_v] = finite ? scale : __uint_as_float(0x7fffffffu);
   }
 }
 
-// Pages [n_out] of the pool as bf16 pages [n_out][2][hkv][16][hd]; slots from n_tokens on are zeros.  One thread, sixteen codes.
+// Pages [n_out] of the pool as bf16 pages [n_out][2][hkv][16][hd]; slots from n_tokens on are zeros.  A thread expands eight codes of
+// K and eight of V, so that a warp's stores are whole lines.
 template <int HD, int FMT>
 __global__ void __launch_bounds__(256) kv8_read_kernel(const uint8_t* __restrict__ pool, int n_pages, int hkv, const int* __restrict__ pages,
                                                        int n_out, long n_tokens, bf16* __restrict__ out, int* __restrict__ status) {
-  constexpr int CPR = HD / 16, CPB = 2 * kKv8Page * CPR;      // 16-code chunks of a row and of a block
+  constexpr int CPR = HD / 8, CPB = kKv8Page * CPR;      // 8-code chunks of a row and of a block's K (or V)
   pdl_wait();
   pdl_launch_dependents();
   const long id = (long)blockIdx.x * blockDim.x + threadIdx.x;
   const long b = id / CPB;
-  const int c = (int)(id % CPB);
+  const int c = (int)(id % CPB), row = c / CPR;
   if (b >= (long)n_out * hkv) return;
   const int pi = (int)(b / hkv), h = (int)(b % hkv);
-  const int kv = c / (CPB / 2), row = (c / CPR) % kKv8Page, cc = c % CPR;
-  const int page = pages[pi];
-  float v[16];
-#pragma unroll
-  for (int i = 0; i < 16; ++i) v[i] = 0.f;
-  if ((long)pi * kKv8Page + row < n_tokens) {
-    if (page < 0 || page >= n_pages) {
-      if (c == 0) atomicExch(status, (int)B2_ERR_BOUNDS);
-    } else {
-      const uint8_t* blk = pool + ((size_t)page * hkv + h) * kv8_block_bytes(HD);
-      const uint4 w = *reinterpret_cast<const uint4*>(blk + (size_t)c * 16);
-      const float s = reinterpret_cast<const float*>(blk + 2 * kKv8Page * HD)[row * 2 + kv];
-      const uint32_t wd[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-      for (int i = 0; i < 16; ++i) v[i] = kv8_value<FMT>((wd[i >> 2] >> (8 * (i & 3))) & 0xffu) * s;
-    }
+  const bool live = (long)pi * kKv8Page + row < n_tokens;
+  const int page = live ? pages[pi] : -1;
+  const bool there = page >= 0 && page < n_pages;
+  if (live && !there && row == 0) atomicExch(status, (int)B2_ERR_BOUNDS);
+  uint2 w[2] = {make_uint2(0u, 0u), make_uint2(0u, 0u)};
+  uint2 sc = make_uint2(0u, 0u);
+  if (there) {
+    const uint8_t* blk = pool + ((size_t)page * hkv + h) * kv8_block_bytes(HD);
+    w[0] = ld_nc_v2(blk + (size_t)c * 8);
+    w[1] = ld_nc_v2(blk + kKv8Page * HD + (size_t)c * 8);
+    sc = ld_nc_v2(blk + 2 * kKv8Page * HD + row * 8);
   }
-  __align__(16) __nv_bfloat162 o[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) o[i] = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
-  uint4* dst = reinterpret_cast<uint4*>(out + (((size_t)pi * 2 + kv) * hkv + h) * kKv8Page * HD + (size_t)row * HD + cc * 16);
-  dst[0] = reinterpret_cast<const uint4*>(o)[0];
-  dst[1] = reinterpret_cast<const uint4*>(o)[1];
+  for (int kv = 0; kv < 2; ++kv) {
+    const float s = __uint_as_float(kv ? sc.y : sc.x);
+    uint4 o;
+    uint32_t* ow = &o.x;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t word = (i < 2 ? w[kv].x : w[kv].y) >> (16 * (i & 1));
+      const __nv_bfloat162 v = __floats2bfloat162_rn(kv8_value<FMT>(word & 0xffu) * s, kv8_value<FMT>((word >> 8) & 0xffu) * s);
+      ow[i] = there ? *reinterpret_cast<const uint32_t*>(&v) : 0u;
+    }
+    *reinterpret_cast<uint4*>(out + (((size_t)pi * 2 + kv) * hkv + h) * kKv8Page * HD + (size_t)c * 8) = o;
+  }
 }
 
 template <class K, class... A>
@@ -176,19 +187,20 @@ B2_API int b2_kv8_store(const Kv8StoreArgs* args, int hd, int fmt, cudaStream_t 
   if (a.n < 1 || a.hq < 1 || a.hkv < 1 || a.n_seq < 1 || a.bt_cols < 1 || a.n_pages < 1) return B2_ERR_ARG;
   if ((hd != 64 && hd != 128) || (fmt != KV8_INT8 && fmt != KV8_FP8) || a.ld % 4 || a.ldq % 4) return B2_ERR_ARG;
   const int hpw = 32 / (hd / 8), turns = (a.hq + 2 * a.hkv + hpw - 1) / hpw;
-  const int wpt = std::min(turns, 8);
-  const long blocks = ((long)a.n * wpt + 7) / 8;
+  // few tokens: a CTA for eight turns, so that no warp has two; many: a CTA for a token, whose sines and cosines are taken once
+  const int most = (turns + 7) / 8, parts = (long)a.n * most <= 148 * 4 ? most : 1;
+  const long blocks = (long)a.n * parts;
   if (blocks > 0x7fffffffl) return B2_ERR_ARG;
   auto k = hd == 128 ? (fmt == KV8_INT8 ? kv8_store_kernel<128, KV8_INT8> : kv8_store_kernel<128, KV8_FP8>)
                      : (fmt == KV8_INT8 ? kv8_store_kernel<64, KV8_INT8> : kv8_store_kernel<64, KV8_FP8>);
-  return launch(k, blocks, 256, st, a, wpt);
+  return launch(k, blocks, 256, st, a, parts);
 }
 
 B2_API int b2_kv8_read(const uint8_t* pool, int n_pages, int hkv, int hd, int fmt, const int* pages, int n_out, long n_tokens,
                        bf16* out, int* status, cudaStream_t st) {
   if (n_out < 1 || hkv < 1 || n_pages < 1 || n_tokens < 0) return B2_ERR_ARG;
   if ((hd != 64 && hd != 128) || (fmt != KV8_INT8 && fmt != KV8_FP8)) return B2_ERR_ARG;
-  const long blocks = ((long)n_out * hkv * 2 * hd + 255) / 256;
+  const long blocks = ((long)n_out * hkv * 2 * hd + 255) / 256;        // 2 * hd chunks of eight codes in a block's K
   if (blocks > 0x7fffffffl) return B2_ERR_ARG;
   auto k = hd == 128 ? (fmt == KV8_INT8 ? kv8_read_kernel<128, KV8_INT8> : kv8_read_kernel<128, KV8_FP8>)
                      : (fmt == KV8_INT8 ? kv8_read_kernel<64, KV8_INT8> : kv8_read_kernel<64, KV8_FP8>);

@@ -98,8 +98,9 @@ def test_the_library_refuses_what_the_launchers_would_not_pass_on():
 
 
 def test_splits_for_a_context():
-    assert [K.split_keys_for(n) for n in (1, 256, 16384, 16385, 32769, 131072, 1 << 20)] == [256, 256, 256, 512, 1024, 2048, 2048]
-    assert K.part_floats(3, 8, 128, 256) == 0 and K.part_floats(3, 8, 128, 257) == 3 * 8 * 2 * 130 and K.part_floats(1, 2, 64, 100, 16) == 2 * 7 * 66
+    assert [K.split_keys_for(n) for n in (1, 700, 7040, 7041, 8000, 16000, 131072, 131073, 1 << 19, 1 << 20)] == [128, 128, 128, 256, 256, 512, 512, 1024, 2048, 2048]
+    assert [K.split_keys_for(4000, h) for h in (2, 8, 16, 1000)] == [128, 128, 256, 512]
+    assert K.part_floats(3, 8, 128, 256, 256) == 0 and K.part_floats(3, 8, 128, 257, 256) == 3 * 8 * 2 * 130 and K.part_floats(1, 2, 64, 100, 16) == 2 * 7 * 66
 
 
 @pytest.mark.parametrize("fmt", FMTS)

@@ -152,8 +152,8 @@ def rope_kvstore8(qkv: torch.Tensor, hq: int, hkv: int, hd: int, inv_freq: torch
     if hq < 1 or hkv < 1:
         _fail("hq and hkv are positive")
     _check_heads(pool, dev, hkv, hd)
-    ld = _check_rows(qkv, n, (hq + 2 * hkv) * hd, dev, "qkv", 4)
-    ldq = _check_rows(q_out, n, hq * hd, dev, "q_out", 4)
+    ld = _check_rows(qkv, n, (hq + 2 * hkv) * hd, dev, "qkv", 8)
+    ldq = _check_rows(q_out, n, hq * hd, dev, "q_out", 8)
     seqs, cols, bt_ld = _check_table(block_table, dev)
     at_pos, at_seq = _check_index(tok_pos, n, dev, "tok_pos"), _check_index(tok_seq, n, dev, "tok_seq")
     at_rope = 0 if rope_pos is None else _check_index(rope_pos, n, dev, "rope_pos")

@@ -26,23 +26,25 @@ struct Kv8StoreArgs {
 
 namespace {
 
-__device__ __forceinline__ void unpack4(uint2 v, float (&f)[4]) {
-  const __nv_bfloat162 a = *reinterpret_cast<const __nv_bfloat162*>(&v.x), b = *reinterpret_cast<const __nv_bfloat162*>(&v.y);
-  f[0] = __low2float(a); f[1] = __high2float(a); f[2] = __low2float(b); f[3] = __high2float(b);
+__device__ __forceinline__ void unpack8(uint4 v, float (&f)[8]) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) { f[2 * i] = __uint_as_float(w[i] << 16); f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
 }
-__device__ __forceinline__ uint2 pack4(const float (&f)[4]) {
-  uint2 v;
-  *reinterpret_cast<__nv_bfloat162*>(&v.x) = __floats2bfloat162_rn(f[0], f[1]);
-  *reinterpret_cast<__nv_bfloat162*>(&v.y) = __floats2bfloat162_rn(f[2], f[3]);
+__device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
+  uint4 v;
+  uint32_t* w = &v.x;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) { const __nv_bfloat162 b = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]); w[i] = *reinterpret_cast<const uint32_t*>(&b); }
   return v;
 }
 
 // Rotation (pairs i, i + hd/2) by pos * inv_freq, q rounded once to bf16, k and v quantised from fp32.
-// HD / 8 lanes hold a head, four rotary pairs each, so a warp takes 32 / (HD / 8) heads at a time ("a turn") and has the next turn's
+// HD / 16 lanes hold a head, eight rotary pairs each, so a warp takes 32 / (HD / 16) heads at a time ("a turn") and has the next turn's
 // loads under way meanwhile.  `parts` CTAs share a token; each takes the token's sines and cosines once.
 template <int HD, int FMT>
 __global__ void __launch_bounds__(256) kv8_store_kernel(const Kv8StoreArgs a, int parts) {
-  constexpr int LPH = HD / 8, HPW = 32 / LPH, HALF = HD / 2;
+  constexpr int LPH = HD / 16, HPW = 32 / LPH, HALF = HD / 2;
   __shared__ __align__(16) float sh_c[HALF], sh_s[HALF];
   pdl_wait();
   pdl_launch_dependents();
@@ -50,13 +52,13 @@ __global__ void __launch_bounds__(256) kv8_store_kernel(const Kv8StoreArgs a, in
   const int tok = blockIdx.x / parts, part = blockIdx.x % parts;
   const int heads = a.hq + 2 * a.hkv, turns = (heads + HPW - 1) / HPW;
   int turn = part * 8 + (threadIdx.x >> 5);
-  const bf16* row = a.qkv + (size_t)tok * a.ld + l * 4;
-  uint2 lo2 = make_uint2(0u, 0u), hi2 = lo2;
+  const bf16* row = a.qkv + (size_t)tok * a.ld + l * 8;
+  uint4 lo8 = make_uint4(0u, 0u, 0u, 0u), hi8 = lo8;
   auto load = [&](int t) {
     const int head = t * HPW + sub;
     if (t < turns && head < heads) {
-      lo2 = ld_nc_v2(row + (size_t)head * HD);
-      hi2 = ld_nc_v2(row + (size_t)head * HD + HALF);
+      lo8 = ld_nc_v4(row + (size_t)head * HD);
+      hi8 = ld_nc_v4(row + (size_t)head * HD + HALF);
     }
   };
   load(turn);
@@ -77,33 +79,34 @@ __global__ void __launch_bounds__(256) kv8_store_kernel(const Kv8StoreArgs a, in
   const bool stored = page >= 0 && page < a.n_pages;
   if (!stored && part == 0 && threadIdx.x == 0) atomicExch(a.status, (int)B2_ERR_BOUNDS);
   __syncthreads();
-  const float4 c4 = *reinterpret_cast<const float4*>(sh_c + l * 4), s4 = *reinterpret_cast<const float4*>(sh_s + l * 4);
-  const float c[4] = {c4.x, c4.y, c4.z, c4.w}, s[4] = {s4.x, s4.y, s4.z, s4.w};
+  float c[8], s[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) { c[i] = sh_c[l * 8 + i]; s[i] = sh_s[l * 8 + i]; }
 
   for (; turn < turns; turn += 8 * parts) {
     const int head = turn * HPW + sub;
-    float lo[4], hi[4];
-    unpack4(lo2, lo);
-    unpack4(hi2, hi);
+    float lo[8], hi[8];
+    unpack8(lo8, lo);
+    unpack8(hi8, hi);
     load(turn + 8 * parts);
     if (head < a.hq + a.hkv) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < 8; ++i) {
         const float x = lo[i], y = hi[i];
         lo[i] = x * c[i] - y * s[i];
         hi[i] = y * c[i] + x * s[i];
       }
     }
     if (head < a.hq) {
-      bf16* dst = a.q_out + (size_t)tok * a.ldq + (size_t)head * HD + l * 4;
-      *reinterpret_cast<uint2*>(dst) = pack4(lo);
-      *reinterpret_cast<uint2*>(dst + HALF) = pack4(hi);
+      bf16* dst = a.q_out + (size_t)tok * a.ldq + (size_t)head * HD + l * 8;
+      *reinterpret_cast<uint4*>(dst) = pack8(lo);
+      *reinterpret_cast<uint4*>(dst + HALF) = pack8(hi);
     }
     if (turn * HPW + HPW <= a.hq) continue;            // q heads only, for the whole warp
     // the largest magnitude, compared as bits: a NaN's are above an infinity's, so neither is lost
     uint32_t mx = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) mx = max(mx, max(__float_as_uint(lo[i]) & 0x7fffffffu, __float_as_uint(hi[i]) & 0x7fffffffu));
+    for (int i = 0; i < 8; ++i) mx = max(mx, max(__float_as_uint(lo[i]) & 0x7fffffffu, __float_as_uint(hi[i]) & 0x7fffffffu));
 #pragma unroll
     for (int o = LPH / 2; o > 0; o >>= 1) mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
     if (head >= heads || head < a.hq || !stored) continue;
@@ -111,17 +114,17 @@ __global__ void __launch_bounds__(256) kv8_store_kernel(const Kv8StoreArgs a, in
     const int kvh = head - a.hq - (is_v ? a.hkv : 0), slot = pos % kKv8Page;
     const float scale = fmaxf(__fdiv_rn(__uint_as_float(mx), FMT == KV8_INT8 ? 127.f : 448.f), kKv8MinScale);
     const bool finite = mx < 0x7f800000u;
-    uint32_t clo = 0, chi = 0;
+    uint32_t clo[2] = {0u, 0u}, chi[2] = {0u, 0u};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 8; ++i) {
       if (!finite) lo[i] = hi[i] = 0.f;            // codes stay numbers: what tells of the row is its scale
-      clo |= kv8_code<FMT>(__fdiv_rn(lo[i], scale)) << (8 * i);
-      chi |= kv8_code<FMT>(__fdiv_rn(hi[i], scale)) << (8 * i);
+      clo[i >> 2] |= kv8_code<FMT>(__fdiv_rn(lo[i], scale)) << (8 * (i & 3));
+      chi[i >> 2] |= kv8_code<FMT>(__fdiv_rn(hi[i], scale)) << (8 * (i & 3));
     }
     uint8_t* blk = a.pool + ((size_t)page * a.hkv + kvh) * kv8_block_bytes(HD);
-    uint8_t* codes = blk + (is_v ? kKv8Page * HD : 0) + slot * HD + l * 4;
-    *reinterpret_cast<uint32_t*>(codes) = clo;
-    *reinterpret_cast<uint32_t*>(codes + HALF) = chi;
+    uint8_t* codes = blk + (is_v ? kKv8Page * HD : 0) + slot * HD + l * 8;
+    *reinterpret_cast<uint2*>(codes) = make_uint2(clo[0], clo[1]);
+    *reinterpret_cast<uint2*>(codes + HALF) = make_uint2(chi[0], chi[1]);
     if (l == 0) reinterpret_cast<float*>(blk + 2 * kKv8Page * HD)[slot * 2 + is_v] = finite ? scale : __uint_as_float(0x7fffffffu);
   }
 }
@@ -185,8 +188,8 @@ using namespace b2;
 B2_API int b2_kv8_store(const Kv8StoreArgs* args, int hd, int fmt, cudaStream_t st) {
   const Kv8StoreArgs& a = *args;
   if (a.n < 1 || a.hq < 1 || a.hkv < 1 || a.n_seq < 1 || a.bt_cols < 1 || a.n_pages < 1) return B2_ERR_ARG;
-  if ((hd != 64 && hd != 128) || (fmt != KV8_INT8 && fmt != KV8_FP8) || a.ld % 4 || a.ldq % 4) return B2_ERR_ARG;
-  const int hpw = 32 / (hd / 8), turns = (a.hq + 2 * a.hkv + hpw - 1) / hpw;
+  if ((hd != 64 && hd != 128) || (fmt != KV8_INT8 && fmt != KV8_FP8) || a.ld % 8 || a.ldq % 8) return B2_ERR_ARG;
+  const int hpw = 32 / (hd / 16), turns = (a.hq + 2 * a.hkv + hpw - 1) / hpw;
   // few tokens: a CTA for eight turns, so that no warp has two; many: a CTA for a token, whose sines and cosines are taken once
   const int most = (turns + 7) / 8, parts = (long)a.n * most <= 148 * 4 ? most : 1;
   const long blocks = (long)a.n * parts;

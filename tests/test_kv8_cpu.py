@@ -26,7 +26,7 @@ BAD_STORE = [
     (dict(pool=torch.zeros(4, HKV, 100, dtype=torch.uint8)), "pages"), (dict(pool=torch.zeros(4, HKV, 2176, dtype=torch.int8)), "uint8"),
     (dict(pool=torch.zeros(4, 2 * HKV, 2176, dtype=torch.uint8)[:, ::2]), "contiguous"), (dict(pool=torch.zeros(0, HKV, 2176, dtype=torch.uint8)), "pages"),
     (dict(qkv=torch.zeros(3, 8 * HD)), "qkv"), (dict(qkv=torch.zeros(3, 16 * HD, dtype=torch.bfloat16)[:, ::2]), "unit stride"),
-    (dict(qkv=torch.zeros(3, 8 * HD + 2, dtype=torch.bfloat16)[:, :8 * HD]), "boundaries"), (dict(qkv=torch.zeros(3, 8 * HD + 8, dtype=torch.bfloat16)[:, 1:8 * HD + 1]), "boundaries"),
+    (dict(qkv=torch.zeros(3, 8 * HD + 4, dtype=torch.bfloat16)[:, :8 * HD]), "boundaries"), (dict(qkv=torch.zeros(3, 8 * HD + 8, dtype=torch.bfloat16)[:, 1:8 * HD + 1]), "boundaries"),
     (dict(q_out=torch.zeros(2, HQ * HD, dtype=torch.bfloat16)), "q_out"), (dict(tok_pos=torch.zeros(3, dtype=torch.int64)), "tok_pos"),
     (dict(tok_seq=torch.zeros(2, dtype=torch.int32)), "tok_seq"), (dict(tok_pos=torch.zeros(6, dtype=torch.int32)[::2]), "tok_pos"),
     (dict(block_table=torch.zeros(4, dtype=torch.int32)), "block_table"), (dict(block_table=torch.zeros(4, 2, dtype=torch.int32).t()), "block_table"),
@@ -80,7 +80,7 @@ def test_the_library_refuses_what_the_launchers_would_not_pass_on():
     from agens_engine_b200 import _lib
     lib = _lib.cuda_lib()
     s = _lib.Kv8StoreArgs(n=1, hq=1, hkv=1, n_seq=1, bt_cols=1, n_pages=1)
-    for hd, fmt, kw in ((96, 0, {}), (64, 2, {}), (64, 0, dict(n=0)), (64, 0, dict(ld=3)), (128, 1, dict(n_pages=0)), (64, 0, dict(n_seq=0))):
+    for hd, fmt, kw in ((96, 0, {}), (64, 2, {}), (64, 0, dict(n=0)), (64, 0, dict(ld=4)), (128, 1, dict(n_pages=0)), (64, 0, dict(n_seq=0))):
         b = _lib.Kv8StoreArgs(n=1, hq=1, hkv=1, n_seq=1, bt_cols=1, n_pages=1)
         for k, v in kw.items():
             setattr(b, k, v)

@@ -21,11 +21,23 @@ constexpr float kKv8MinScale = 5.421010862427522e-20f;   // 2^-64
 
 __host__ __device__ constexpr int kv8_block_bytes(int hd) { return 2 * kKv8Page * hd + kKv8Page * 8; }
 
-// fp32 value of a stored byte
+// four e4m3 numbers -> fp16 pairs (0, 1) and (2, 3)
+__device__ __forceinline__ void e4m3_pairs(uint32_t w, uint32_t& x, uint32_t& y) {
+  asm("{ .reg .b16 lo, hi; mov.b32 {lo, hi}, %2; cvt.rn.f16x2.e4m3x2 %0, lo; cvt.rn.f16x2.e4m3x2 %1, hi; }" : "=r"(x), "=r"(y) : "r"(w));
+}
+
+// fp32 values of four stored bytes
 template <int FMT>
-__device__ __forceinline__ float kv8_value(uint32_t byte) {
-  if (FMT == KV8_INT8) return (float)((int)byte - 128);
-  return __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)byte, __NV_E4M3)));
+__device__ __forceinline__ void kv8_values(uint32_t w, float* f) {
+  if (FMT == KV8_INT8) {                     // 0x4b0000xx is 2^23 + xx
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7440 + i)) - 8388736.f;
+  } else {
+    uint32_t lo, hi;
+    e4m3_pairs(w, lo, hi);
+    const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&lo)), b = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+    f[0] = a.x; f[1] = a.y; f[2] = b.x; f[3] = b.y;
+  }
 }
 
 // stored byte of y = x / scale

@@ -61,10 +61,6 @@ __device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
   const __half2 v = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
 }
-// four e4m3 numbers -> fp16 pairs (0, 1) and (2, 3)
-__device__ __forceinline__ void e4m3_pairs(uint32_t w, uint32_t& x, uint32_t& y) {
-  asm("{ .reg .b16 lo, hi; mov.b32 {lo, hi}, %2; cvt.rn.f16x2.e4m3x2 %0, lo; cvt.rn.f16x2.e4m3x2 %1, hi; }" : "=r"(x), "=r"(y) : "r"(w));
-}
 // D(16x8, s32) = A(16x32, s8, row) * B(32x8, u8, col) + C
 __device__ __forceinline__ void mma_s8u8(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, int c0, int c1, int c2, int c3) {
   asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"

@@ -129,50 +129,42 @@ __global__ void __launch_bounds__(256) kv8_store_kernel(const Kv8StoreArgs a, in
   }
 }
 
-// Pages [n_out] of the pool as bf16 pages [n_out][2][hkv][16][hd]; slots from n_tokens on are zeros.  A thread expands eight codes of
-// K and eight of V, so that a warp's stores are whole lines.
+// Pages [n_out] of the pool as bf16 pages [n_out][2][hkv][16][hd]; slots from n_tokens on are zeros.  A CTA expands a page of a KV
+// head, a thread eight codes of K and eight of V, so that a warp's stores are whole lines.
 template <int HD, int FMT>
-__global__ void __launch_bounds__(256) kv8_read_kernel(const uint8_t* __restrict__ pool, int n_pages, int hkv, const int* __restrict__ pages,
-                                                       int n_out, long n_tokens, bf16* __restrict__ out, int* __restrict__ status) {
-  constexpr int CPR = HD / 8, CPB = kKv8Page * CPR;      // 8-code chunks of a row and of a block's K (or V)
+__global__ void __launch_bounds__(2 * HD) kv8_read_kernel(const uint8_t* __restrict__ pool, int n_pages, int hkv, const int* __restrict__ pages,
+                                                          long n_tokens, bf16* __restrict__ out, int* __restrict__ status) {
   pdl_wait();
   pdl_launch_dependents();
-  const long id = (long)blockIdx.x * blockDim.x + threadIdx.x;
-  const long b = id / CPB;
-  const int c = (int)(id % CPB), row = c / CPR;
-  if (b >= (long)n_out * hkv) return;
-  const int pi = (int)(b / hkv), h = (int)(b % hkv);
+  const int pi = blockIdx.x, h = blockIdx.y, c = threadIdx.x, row = c / (HD / 8);
   const bool live = (long)pi * kKv8Page + row < n_tokens;
   const int page = live ? pages[pi] : -1;
   const bool there = page >= 0 && page < n_pages;
-  if (live && !there && row == 0) atomicExch(status, (int)B2_ERR_BOUNDS);
+  if (live && !there && c == 0) atomicExch(status, (int)B2_ERR_BOUNDS);
   uint2 w[2] = {make_uint2(0u, 0u), make_uint2(0u, 0u)};
   uint2 sc = make_uint2(0u, 0u);
   if (there) {
     const uint8_t* blk = pool + ((size_t)page * hkv + h) * kv8_block_bytes(HD);
-    w[0] = ld_nc_v2(blk + (size_t)c * 8);
-    w[1] = ld_nc_v2(blk + kKv8Page * HD + (size_t)c * 8);
+    w[0] = ld_nc_v2(blk + c * 8);
+    w[1] = ld_nc_v2(blk + kKv8Page * HD + c * 8);
     sc = ld_nc_v2(blk + 2 * kKv8Page * HD + row * 8);
   }
 #pragma unroll
   for (int kv = 0; kv < 2; ++kv) {
     const float s = __uint_as_float(kv ? sc.y : sc.x);
-    uint4 o;
-    uint32_t* ow = &o.x;
+    float f[8];
+    kv8_values<FMT>(w[kv].x, f);
+    kv8_values<FMT>(w[kv].y, f + 4);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t word = (i < 2 ? w[kv].x : w[kv].y) >> (16 * (i & 1));
-      const __nv_bfloat162 v = __floats2bfloat162_rn(kv8_value<FMT>(word & 0xffu) * s, kv8_value<FMT>((word >> 8) & 0xffu) * s);
-      ow[i] = there ? *reinterpret_cast<const uint32_t*>(&v) : 0u;
-    }
-    *reinterpret_cast<uint4*>(out + (((size_t)pi * 2 + kv) * hkv + h) * kKv8Page * HD + (size_t)c * 8) = o;
+    for (int i = 0; i < 8; ++i) f[i] = there ? __fmul_rn(f[i], s) : 0.f;
+    *reinterpret_cast<uint4*>(out + (((size_t)pi * 2 + kv) * hkv + h) * kKv8Page * HD + c * 8) = pack8(f);
   }
 }
 
 template <class K, class... A>
-int launch(K kernel, long blocks, int threads, cudaStream_t st, A... args) {
+int launch(K kernel, dim3 blocks, int threads, cudaStream_t st, A... args) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)blocks); cfg.blockDim = dim3(threads); cfg.stream = st;
+  cfg.gridDim = blocks; cfg.blockDim = dim3(threads); cfg.stream = st;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[0].val.programmaticStreamSerializationAllowed = 1;
@@ -196,16 +188,14 @@ B2_API int b2_kv8_store(const Kv8StoreArgs* args, int hd, int fmt, cudaStream_t 
   if (blocks > 0x7fffffffl) return B2_ERR_ARG;
   auto k = hd == 128 ? (fmt == KV8_INT8 ? kv8_store_kernel<128, KV8_INT8> : kv8_store_kernel<128, KV8_FP8>)
                      : (fmt == KV8_INT8 ? kv8_store_kernel<64, KV8_INT8> : kv8_store_kernel<64, KV8_FP8>);
-  return launch(k, blocks, 256, st, a, parts);
+  return launch(k, dim3((unsigned)blocks), 256, st, a, parts);
 }
 
 B2_API int b2_kv8_read(const uint8_t* pool, int n_pages, int hkv, int hd, int fmt, const int* pages, int n_out, long n_tokens,
                        bf16* out, int* status, cudaStream_t st) {
-  if (n_out < 1 || hkv < 1 || n_pages < 1 || n_tokens < 0) return B2_ERR_ARG;
+  if (n_out < 1 || hkv < 1 || hkv > 65535 || n_pages < 1 || n_tokens < 0) return B2_ERR_ARG;
   if ((hd != 64 && hd != 128) || (fmt != KV8_INT8 && fmt != KV8_FP8)) return B2_ERR_ARG;
-  const long blocks = ((long)n_out * hkv * 2 * hd + 255) / 256;        // 2 * hd chunks of eight codes in a block's K
-  if (blocks > 0x7fffffffl) return B2_ERR_ARG;
   auto k = hd == 128 ? (fmt == KV8_INT8 ? kv8_read_kernel<128, KV8_INT8> : kv8_read_kernel<128, KV8_FP8>)
                      : (fmt == KV8_INT8 ? kv8_read_kernel<64, KV8_INT8> : kv8_read_kernel<64, KV8_FP8>);
-  return launch(k, blocks, 256, st, pool, n_pages, hkv, pages, n_out, n_tokens, out, status);
+  return launch(k, dim3(n_out, hkv), 2 * hd, st, pool, n_pages, hkv, pages, n_tokens, out, status);
 }

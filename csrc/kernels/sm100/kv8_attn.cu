@@ -67,13 +67,19 @@ __device__ __forceinline__ void mma_s8u8(int (&d)[4], const uint32_t (&a)[4], ui
                : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(c0), "r"(c1), "r"(c2), "r"(c3));
 }
+// Taken off here and not from the finished sums (64 instructions a pair of pages less, 1 % of the time): the accumulators truncate,
+// and 1152 in every term cost a flat row of 131072 keys half of its last bf16 digit.
+__device__ __forceinline__ uint32_t minus_1152(uint32_t two) {
+  const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&two), __half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480)));
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
 // Of two rows' words: pairs (row a, row b) of bytes 2 * HI and 2 * HI + 1
 template <int FMT, int HI>
 __device__ __forceinline__ void cross_pairs(uint32_t wa, uint32_t wb, uint32_t& x, uint32_t& y) {
   if (FMT == KV8_INT8) {
     const uint32_t z = __byte_perm(wa, wb, HI ? 0x7632 : 0x5410);
-    x = lop3_and_or(z, 0x00ff00ffu, 0x64006400u);          // 0x64xx is 1024 + xx, 1152 above the code
-    y = __byte_perm(z, 0x64646464u, 0x4341);
+    x = minus_1152(lop3_and_or(z, 0x00ff00ffu, 0x64006400u));          // 0x64xx is 1024 + xx
+    y = minus_1152(__byte_perm(z, 0x64646464u, 0x4341));
   } else {
     e4m3_pairs(__byte_perm(wa, wb, HI ? 0x7362 : 0x5140), x, y);
   }
@@ -327,13 +333,9 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_attn_kernel(
 
     // o: channels g * HD / 8 + 2k (0, 1) and + 1 (2, 3) of columns 2t (0, 2) and 2t + 1 (1, 3); m and l: of column g
     float o[NT][MT][4], m[NT], l[NT];
-    // int8: V's fp16 numbers are 1152 above the codes; the same sums of 1152 alone are taken off at the end.  Both lose alike to
-    // the accumulators' truncation, 2^-23 of 1152 a step, so that what is left of it is a random part below 2^-10 of a code.
-    float bias[NT][4];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       m[n] = kNoRef; l[n] = 0.f;
-      bias[n][0] = bias[n][1] = bias[n][2] = bias[n][3] = 0.f;
 #pragma unroll
       for (int i = 0; i < MT; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
     }
@@ -465,8 +467,6 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_attn_kernel(
             o[n][k][0] = __fmul_rn(o[n][k][0], f0); o[n][k][1] = __fmul_rn(o[n][k][1], f1);
             o[n][k][2] = __fmul_rn(o[n][k][2], f0); o[n][k][3] = __fmul_rn(o[n][k][3], f1);
           }
-          bias[n][0] = __fmul_rn(bias[n][0], f0); bias[n][1] = __fmul_rn(bias[n][1], f1);
-          bias[n][2] = bias[n][0]; bias[n][3] = bias[n][1];
         }
         weigh();
       }
@@ -492,11 +492,6 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_attn_kernel(
             send(rd, i + 2);
             rd ^= flip;
           }
-        }
-        if constexpr (FMT == KV8_INT8) {
-          const uint32_t f[4] = {0x64806480u, 0x64806480u, 0x64806480u, 0x64806480u};         // 1152
-#pragma unroll
-          for (int n = 0; n < NT; ++n) mma_f16_16816(bias[n], f, pb[n][0], pb[n][1]);
         }
 #pragma unroll
         for (int x = 0; x < VW; ++x) {
@@ -524,11 +519,10 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_attn_kernel(
       if (t == 0) { sh_m[warp][n * 8 + g] = m[n]; sh_l[warp][n * 8 + g] = x; }
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        const float b = FMT == KV8_INT8 ? -bias[n][j] : 0.f;
 #pragma unroll
         for (int k = 0; k < MT; k += 2)
           *reinterpret_cast<float4*>(&tile[n * 8 + 2 * t + j][g * (HD / 8) + 2 * k]) =
-              make_float4(__fadd_rn(o[n][k][j], b), __fadd_rn(o[n][k][2 + j], b), __fadd_rn(o[n][k + 1][j], b), __fadd_rn(o[n][k + 1][2 + j], b));
+              make_float4(o[n][k][j], o[n][k][2 + j], o[n][k + 1][j], o[n][k + 1][2 + j]);
       }
     }
     __syncthreads();

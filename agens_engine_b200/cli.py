@@ -36,6 +36,7 @@ class EngineConfig:
     mode: str = "server"
     prefill_chunk: int = 256
     split_keys: int = 64
+    kv_cache: str = "bf16"                # bf16, or 8-bit pages: int8, fp8
     spec_copy: int = 0
     spec_drafter: Optional[str] = None
     mtp: Optional[str] = None
@@ -71,6 +72,8 @@ class EngineConfig:
             if e is not None:
                 cur = getattr(cfg, f.name)
                 setattr(cfg, f.name, type(cur)(e) if cur is not None else e)
+        if cfg.kv_cache not in ("bf16", "int8", "fp8"):
+            raise SystemExit(f"--kv-cache: bf16, int8 or fp8, got {cfg.kv_cache!r}")
         return cfg
 
 
@@ -90,10 +93,12 @@ def _named_config(name: str):
 def _model_config(cfg: EngineConfig):
     if cfg.model_dir:
         from .models.config import ModelConfig
-        return ModelConfig.from_json(os.path.join(cfg.model_dir, "config.json"))
-    if cfg.random:
-        return _named_config(cfg.random)
-    raise SystemExit("give --model-dir DIR or --random NAME")
+        mc = ModelConfig.from_json(os.path.join(cfg.model_dir, "config.json"))
+    elif cfg.random:
+        mc = _named_config(cfg.random)
+    else:
+        raise SystemExit("give --model-dir DIR or --random NAME")
+    return dataclasses.replace(mc, kv_cache=cfg.kv_cache)
 
 
 def build_model(cfg: EngineConfig, **kw):
@@ -109,6 +114,7 @@ def build_model(cfg: EngineConfig, **kw):
     kw.setdefault("max_ctx", cfg.wctx)
     kw.setdefault("prefill_chunk", cfg.prefill_chunk)
     kw.setdefault("split_keys", cfg.split_keys)
+    kw.setdefault("kv_cache", cfg.kv_cache)
     # long contexts: at most 1024 attention splits per (row, head), so that the split partials stay near 1 GB at 256K
     want = (kw["max_ctx"] + 1023) // 1024
     while kw["split_keys"] < want:
@@ -223,17 +229,14 @@ def cmd_devices(ns):
 def cmd_plan(ns):
     from .serve import host as H
     cfg = EngineConfig.resolve(ns)
-    mc = _named_config(cfg.random) if cfg.random else None
-    if cfg.model_dir:
-        from .models.config import ModelConfig
-        mc = ModelConfig.from_json(os.path.join(cfg.model_dir, "config.json"))
-    if mc is None:
-        raise SystemExit("give --model-dir DIR or --random NAME")
-    rep = H.plan(budget_gib=cfg.budget_gib, gpu_free_gib=ns.gpu_free_gib, weights_bytes=mc.weight_bytes(cfg.tp),
+    from .serve import budget as B
+    mc = _model_config(cfg)
+    kv = B.kv_cache_plan(mc, cfg.wctx, cfg.max_batch, cfg.tp, cfg.split_keys)
+    rep = H.plan(budget_gib=cfg.budget_gib, gpu_free_gib=ns.gpu_free_gib, weights_bytes=mc.weight_bytes(cfg.tp) + kv["extra_bytes"],
                  kv_bytes_per_token=mc.kv_bytes_per_token(cfg.tp), page_size=mc.page_size, max_batch=cfg.max_batch,
                  sessions=cfg.max_convs, prefill_chunk=ns.plan_prefill_chunk, d_model=mc.d_model, ffn=mc.ffn, q_dim=mc.q_dim,
                  kv_dim=mc.kv_dim, vocab=mc.vocab, n_heads=mc.n_heads, head_dim=mc.head_dim, tp=cfg.tp, wctx=cfg.wctx,
-                 host_avail_gib=ns.host_avail_gib)
+                 host_avail_gib=ns.host_avail_gib, allow_host_tier=kv["host_tier"], split_keys=kv["split_keys"])
     for line in rep.get("lines", []):
         print(line)
     print(json.dumps({k: v for k, v in rep.items() if k != "lines"}, indent=1))
@@ -637,6 +640,7 @@ def _engine_flags(p):
     p.add_argument("--mode", choices=["personal", "server"]); p.add_argument("--prefill-chunk", type=int)
     p.add_argument("--profile"); p.add_argument("--draft-depth", type=int); p.add_argument("--row-graphs", type=int)
     p.add_argument("--prompt-len", type=int, default=64); p.add_argument("--new-tokens", type=int, default=32)
+    p.add_argument("--kv-cache", choices=["bf16", "int8", "fp8"])
 
 
 def main(argv=None) -> int:

@@ -31,6 +31,7 @@ class ModelConfig:
     default_bits: int = 4
     vocab_valid: Optional[int] = None      # ids >= vocab_valid are never produced (reference: VOCAB_VALID)
     page_size: int = 16
+    kv_cache: str = "bf16"                 # "bf16", or 8-bit pages: "int8" / "fp8" (ops/kv8.py)
 
     def bits_of(self, layer: int, linear: str) -> int:
         return self.bits.get(f"{layer}.{linear}", self.default_bits)
@@ -44,8 +45,9 @@ class ModelConfig:
         return self.n_kv_heads * self.head_dim
 
     def kv_bytes_per_token(self, tp: int = 1) -> int:
-        """bf16 K and V of every layer for one token on one rank (reference: config.rs:236-243)."""
-        return self.n_layers * 2 * (self.n_kv_heads // tp) * self.head_dim * 2
+        """K and V of every layer for one token on one rank (reference: config.rs:236-243): bf16, or codes and two fp32 scales."""
+        row = 4 * self.head_dim if self.kv_cache == "bf16" else 2 * self.head_dim + 8
+        return self.n_layers * (self.n_kv_heads // tp) * row
 
     def n_params_linear(self) -> int:
         per = self.d_model * (self.q_dim + 2 * self.kv_dim) + self.q_dim * self.d_model + 3 * self.d_model * self.ffn

@@ -9,6 +9,7 @@ only per-step input is the token produced by the previous step, handled on the d
 """
 from __future__ import annotations
 
+import dataclasses
 import math
 import os
 from typing import Dict, List, Optional
@@ -19,6 +20,7 @@ from .. import _lib
 from .._lib import EPI_ARGMAX, EPI_F32, EPI_RESID, EPI_STORE, EPI_SWIGLU, PRO_NORM, PRO_PLAIN, check, current_stream, ptr
 from ..ops import attention as A
 from ..ops import basic
+from ..ops import kv8 as K8
 from ..ops import linear as L
 from .config import LINEARS, ModelConfig
 
@@ -31,8 +33,17 @@ M_ROWS = 128         # most token rows of one step (64 decode rows or 128 verify
 class DenseModel:
     def __init__(self, cfg: ModelConfig, device="cuda:0", max_seqs: int = 1, max_ctx: int = 4096,
                  n_pages: Optional[int] = None, split_keys: int = 64, prefill_chunk: int = 256,
-                 lm_rows: Optional[int] = None):
+                 lm_rows: Optional[int] = None, kv_cache: Optional[str] = None):
+        """``kv_cache``: "bf16" (default: what the config says), or "int8" / "fp8": 8-bit pages (``ops/kv8.py``), half the bytes.  A
+        model with 8-bit pages runs its steps on the per-op kernels and does not tier its KV to the host."""
+        if kv_cache is not None and kv_cache != cfg.kv_cache:
+            cfg = dataclasses.replace(cfg, kv_cache=kv_cache)
+        if cfg.kv_cache not in ("bf16", *K8.FORMATS):
+            raise ValueError(f"kv_cache: bf16, {' or '.join(K8.FORMATS)}, got {cfg.kv_cache!r}")
+        if cfg.kv_cache != "bf16" and (cfg.page_size != K8.PAGE or cfg.head_dim not in (64, 128)):
+            raise ValueError(f"an 8-bit KV cache has pages of {K8.PAGE} tokens and heads of 64 or 128")
         self.cfg, self.dev = cfg, torch.device(device)
+        self.kv8 = cfg.kv_cache if cfg.kv_cache != "bf16" else None
         self.lm_rows = lm_rows or cfg.vocab          # rows of the (possibly vocab-sharded, padded) lm_head
         self.max_seqs, self.max_ctx, self.split_keys = max_seqs, max_ctx, split_keys
         self.prefill_chunk = prefill_chunk
@@ -123,8 +134,15 @@ class DenseModel:
         bf = lambda *s: torch.zeros(*s, dtype=torch.bfloat16, device=dev)
         # rows of one step: eight per sequence slot (a verify group), at least M_GEMV, at most M_ROWS
         M = self.max_rows = min(M_ROWS, max(M_GEMV, 8 * self.max_seqs))
-        self.kv = [torch.zeros(self.n_pages, 2, cfg.n_kv_heads, cfg.page_size, cfg.head_dim, dtype=torch.bfloat16, device=dev)
-                   for _ in range(cfg.n_layers)]
+        if self.kv8:
+            self.kv = [K8.make_pool(self.n_pages, cfg.n_kv_heads, cfg.head_dim, dev) for _ in range(cfg.n_layers)]
+            self.split8 = K8.split_keys_for(self.max_ctx, self.max_seqs * cfg.n_kv_heads)
+            # bf16 copy of one sequence's pages of one layer: what the prefill attention of a long chunk reads
+            self._stage = torch.empty(self.pages_per_seq, 2, cfg.n_kv_heads, cfg.page_size, cfg.head_dim, dtype=torch.bfloat16, device=dev)
+            self._stage_table = torch.arange(self.pages_per_seq, dtype=torch.int32, device=dev).view(1, -1)
+        else:
+            self.kv = [torch.zeros(self.n_pages, 2, cfg.n_kv_heads, cfg.page_size, cfg.head_dim, dtype=torch.bfloat16, device=dev)
+                       for _ in range(cfg.n_layers)]
         self.block_table = torch.full((self.max_seqs, self.pages_per_seq), -1, dtype=torch.int32, device=dev)
         self.seq_len = i32(self.max_seqs)
         # the per-step row description lives in one buffer so that an eager step uploads it with a single copy
@@ -144,8 +162,12 @@ class DenseModel:
         self.q = bf(M, cfg.q_dim)
         self.attn = bf(M, cfg.q_dim)
         self.act = bf(M, cfg.ffn)
-        self.part_o = torch.empty(M, cfg.n_heads, self.max_splits, cfg.head_dim, dtype=torch.float32, device=dev)
-        self.part_ml = torch.empty(M, cfg.n_heads, self.max_splits, 2, dtype=torch.float32, device=dev)
+        if self.kv8:
+            self.part8 = torch.empty(K8.part_floats(M, cfg.n_heads, cfg.head_dim, self.pages_per_seq * cfg.page_size, self.split8),
+                                     dtype=torch.float32, device=dev)
+        else:
+            self.part_o = torch.empty(M, cfg.n_heads, self.max_splits, cfg.head_dim, dtype=torch.float32, device=dev)
+            self.part_ml = torch.empty(M, cfg.n_heads, self.max_splits, 2, dtype=torch.float32, device=dev)
         lm_panels = (self.lm_rows + 31) // 32
         self.amax_val = torch.empty(lm_panels, L.SS_LD, dtype=torch.float32, device=dev)
         self.amax_idx = torch.empty(lm_panels, L.SS_LD, dtype=torch.int32, device=dev)
@@ -186,8 +208,9 @@ class DenseModel:
         self.step = StepRunner(self, uniform=self.step_uniform)
 
     def _step_possible(self) -> bool:
-        # (the step kernel reads quantised weights only: a model with bf16 linears stays on the per-op kernels)
-        return self.dev.type == "cuda" and self.cfg.head_dim == 128 and self.cfg.page_size == 16 and bool(self.layers) \
+        # (the step kernel reads quantised weights and bf16 pages only: a model with bf16 linears, or with an 8-bit KV cache, stays on
+        # the per-op kernels)
+        return self.dev.type == "cuda" and not self.kv8 and self.cfg.head_dim == 128 and self.cfg.page_size == 16 and bool(self.layers) \
             and all(isinstance(d[lin], L.WqLinear) for d in self.layers for lin in LINEARS)
 
     def enable_step(self, on=True, uniform: Optional[bool] = None):
@@ -254,6 +277,8 @@ class DenseModel:
     def enable_host_tier(self, window_tokens: int, batch_pages: int = 256):
         """KV pages older than ``window_tokens`` (rounded up to batches of ``batch_pages`` pages) move to pinned host
         memory; attention streams them back on a side stream.  Eager steps only (graph replays need resident KV)."""
+        if self.kv8:
+            raise ValueError("the host tier moves bf16 pages: a model with an 8-bit KV cache keeps its pages on the GPU")
         from .kv_tier import HostKvTier
         self.tier = HostKvTier(self, window_tokens, batch_pages)
         return self.tier
@@ -335,7 +360,7 @@ class DenseModel:
         self._resident_or_raise(seq, used, "park")
         idx = torch.tensor(self.seq_pages[seq][:used], dtype=torch.long, device=self.dev)
         shape = (self.cfg.n_layers, used) + tuple(self.kv[0].shape[1:])
-        host_kv = torch.empty(shape, dtype=torch.bfloat16, pin_memory=True)
+        host_kv = torch.empty(shape, dtype=self.kv[0].dtype, pin_memory=True)
         for l, kv in enumerate(self.kv):
             host_kv[l].copy_(kv.index_select(0, idx), non_blocking=True)
         torch.cuda.current_stream(self.dev).synchronize()
@@ -369,8 +394,10 @@ class DenseModel:
         idx = torch.tensor(self.seq_pages[seq][:used], dtype=torch.long, device=self.dev)
         kv = torch.stack([layer.index_select(0, idx) for layer in self.kv]).cpu()
         meta = {"format": "b200e-session-1", "len": str(n), "n_layers": str(self.cfg.n_layers), "n_kv_heads": str(self.cfg.n_kv_heads),
-                "head_dim": str(self.cfg.head_dim), "page_size": str(self.cfg.page_size)}
+                "head_dim": str(self.cfg.head_dim), "page_size": str(self.cfg.page_size), "kv_cache": self.cfg.kv_cache}
         t = {"kv": kv, "len": torch.tensor([n], dtype=torch.int32)}
+        if self.kv8:                         # the two 8-bit formats have the same shape
+            t["kv_format"] = torch.tensor([K8.FORMATS[self.kv8]], dtype=torch.int32)
         if tokens is not None:
             t["tokens"] = torch.tensor(list(tokens), dtype=torch.int32)
         K.write_safetensors(path, t, metadata=meta)
@@ -382,10 +409,11 @@ class DenseModel:
         kv = f.tensor("kv").clone()
         toks = f.tensor("tokens").tolist() if "tokens" in f.keys() else []
         n = int(f.tensor("len")[0])
+        fmt = int(f.tensor("kv_format")[0]) if "kv_format" in f.keys() else None
         f.close()
-        want = (self.cfg.n_layers, (n + self.cfg.page_size - 1) // self.cfg.page_size, 2, self.cfg.n_kv_heads, self.cfg.page_size, self.cfg.head_dim)
-        if tuple(kv.shape) != want:
-            raise ValueError(f"session file does not match this model: {tuple(kv.shape)} vs {want}")
+        want = (self.cfg.n_layers, (n + self.cfg.page_size - 1) // self.cfg.page_size) + tuple(self.kv[0].shape[1:])
+        if tuple(kv.shape) != want or kv.dtype != self.kv[0].dtype or fmt != (K8.FORMATS[self.kv8] if self.kv8 else None):
+            raise ValueError(f"session file does not match this model: {tuple(kv.shape)} vs {want}, KV cache {self.cfg.kv_cache}")
         self.unpark(seq, {"len": n, "kv": kv.pin_memory()})
         return toks
 
@@ -417,16 +445,23 @@ class DenseModel:
         for li, d in enumerate(self.layers):
             L.gemv(d["qkv"], h_a, ws, pro=PRO_NORM, ss_in=self.ss_a, ss_parts=parts_a, norm_w=d["ln1"], eps=cfg.rms_eps,
                    out=self.qkv[:m])
-            basic.rope_kvstore(self.qkv[:m], cfg.n_heads, cfg.n_kv_heads, cfg.head_dim, self.inv_freq, self.tok_pos,
-                               self.tok_seq, self.block_table, self.kv[li], self.q[:m], status=self.status,
-                               rope_pos=self.rope_pos if self._use_rope_pos else None)
-            if self._tiered_groups:
-                self.tier.attend(li, self.q[:m], self.grp_tok0[:n_groups], self.grp_cnt[:n_groups], self.tok_pos, self.tok_seq,
-                                 self._tiered_groups, self.split_keys, self.max_splits, self.part_o, self.part_ml, self.attn[:m])
+            rope_pos = self.rope_pos if self._use_rope_pos else None
+            if self.kv8:
+                K8.rope_kvstore8(self.qkv[:m], cfg.n_heads, cfg.n_kv_heads, cfg.head_dim, self.inv_freq, self.tok_pos, self.tok_seq,
+                                 self.block_table, self.kv[li], self.kv8, self.q[:m], rope_pos=rope_pos, status=self.status)
+                K8.attn_decode8(self.q[:m], self.kv[li], self.kv8, self.block_table, self.grp_tok0[:n_groups], self.grp_cnt[:n_groups],
+                                self.tok_pos, self.tok_seq, cfg.n_heads, cfg.n_kv_heads, cfg.head_dim, split_keys=self.split8,
+                                part=self.part8, status=self.status, out=self.attn[:m])
             else:
-                A.attn_decode(self.q[:m], self.kv[li], self.block_table, self.grp_tok0[:n_groups], self.grp_cnt[:n_groups],
-                              self.tok_pos, self.tok_seq, cfg.n_heads, cfg.n_kv_heads, cfg.head_dim, self.split_keys,
-                              self.max_splits, part_o=self.part_o, part_ml=self.part_ml, status=self.status, out=self.attn[:m])
+                basic.rope_kvstore(self.qkv[:m], cfg.n_heads, cfg.n_kv_heads, cfg.head_dim, self.inv_freq, self.tok_pos,
+                                   self.tok_seq, self.block_table, self.kv[li], self.q[:m], status=self.status, rope_pos=rope_pos)
+                if self._tiered_groups:
+                    self.tier.attend(li, self.q[:m], self.grp_tok0[:n_groups], self.grp_cnt[:n_groups], self.tok_pos, self.tok_seq,
+                                     self._tiered_groups, self.split_keys, self.max_splits, self.part_o, self.part_ml, self.attn[:m])
+                else:
+                    A.attn_decode(self.q[:m], self.kv[li], self.block_table, self.grp_tok0[:n_groups], self.grp_cnt[:n_groups],
+                                  self.tok_pos, self.tok_seq, cfg.n_heads, cfg.n_kv_heads, cfg.head_dim, self.split_keys,
+                                  self.max_splits, part_o=self.part_o, part_ml=self.part_ml, status=self.status, out=self.attn[:m])
             parts_b = self._row_parallel(d["o"], self.attn[:m], h_a, h_b, self.ss_b, 2 * li)
             L.gemv(d["gate_up"], h_b, ws, pro=PRO_NORM, ss_in=self.ss_b, ss_parts=parts_b, norm_w=d["ln2"],
                    eps=cfg.rms_eps, epi=EPI_SWIGLU, out=self.act[:m])
@@ -642,7 +677,9 @@ class DenseModel:
             else:
                 x, h = basic.rmsnorm(delta, d["ln1"], cfg.rms_eps, resid=h)
             qkv = self._linear_big(d["qkv"], x)
-            if getattr(self, "_rope3", None) is not None:
+            if self.kv8:
+                a = self._prefill_attend8(li, qkv, q, seq, pos0, pos, seqv)
+            elif getattr(self, "_rope3", None) is not None:
                 r3 = self._rope3[0][:, self._sub_slice[0]:self._sub_slice[1]].contiguous()
                 basic.rope_kvstore_m(qkv, cfg.n_heads, cfg.n_kv_heads, cfg.head_dim, self.inv_freq, pos, r3, self._rope3[1], seqv,
                                      self.block_table, self.kv[li], q, status=self.status)
@@ -650,7 +687,9 @@ class DenseModel:
                 rp = pos + self.rope_delta[seq] if self.rope_delta.get(seq, 0) else None
                 basic.rope_kvstore(qkv, cfg.n_heads, cfg.n_kv_heads, cfg.head_dim, self.inv_freq, pos, seqv, self.block_table,
                                    self.kv[li], q, status=self.status, rope_pos=rp)
-            if tiered:
+            if self.kv8:
+                pass
+            elif tiered:
                 a = self.tier.attend(li, q, pg0, pgc, pos, seqv, {seq: (0, pg0.numel())}, self.prefill_split, p_splits, p_o, p_ml, p_out,
                                      shared_kv=True)
             else:
@@ -671,6 +710,27 @@ class DenseModel:
         basic.sumsq(self.h_a[:1], self.ss_a)
         self._head_small(1, 1, want_logits, standalone=True)
         return int(self.out_ids[0]), (self._full_logits(1)[0] if want_logits else None)
+
+    def _prefill_attend8(self, li: int, qkv: torch.Tensor, q: torch.Tensor, seq: int, pos0: int, pos: torch.Tensor,
+                         seqv: torch.Tensor) -> torch.Tensor:
+        """A prefill chunk of layer ``li`` over 8-bit pages: the chunk's K and V are stored, then a long chunk reads the sequence's pages
+        back in bf16 for the prefill attention, a short one attends to them as they are."""
+        cfg, T = self.cfg, q.shape[0]
+        r3 = getattr(self, "_rope3", None)
+        kw = dict(rope_pos=pos + self.rope_delta[seq]) if r3 is None and self.rope_delta.get(seq, 0) else {}
+        if r3 is not None:
+            kw = dict(rope_pos3=r3[0][:, self._sub_slice[0]:self._sub_slice[1]].contiguous(), pair_axis=r3[1])
+        K8.rope_kvstore8(qkv, cfg.n_heads, cfg.n_kv_heads, cfg.head_dim, self.inv_freq, pos, seqv, self.block_table, self.kv[li], self.kv8, q,
+                         status=self.status, **kw)
+        if T < A.PREFILL_TC_MIN_TOKENS:
+            g0, gc, _, _ = A.prefill_groups(T, pos0, seq, self.dev)
+            part = self.part8 if T <= self.max_rows else None
+            return K8.attn_decode8(q, self.kv[li], self.kv8, self.block_table, g0, gc, pos, seqv, cfg.n_heads, cfg.n_kv_heads, cfg.head_dim,
+                                   split_keys=self.split8, part=part, status=self.status)
+        used = (pos0 + T + cfg.page_size - 1) // cfg.page_size
+        K8.kv_read8(self.kv[li], self.kv8, self.block_table[seq, :used], n_tokens=pos0 + T, out=self._stage[:used], status=self.status)
+        return A.attn_prefill(q, self._stage, self._stage_table, 0, pos0, cfg.n_heads, cfg.n_kv_heads, cfg.head_dim, status=self.status,
+                              split_keys=self._prefill_split_for(pos0 + T))
 
     # ------------------------------------------------------------------------------------------------ decode
     def _decode_body(self, seqs: List[int]):
@@ -761,4 +821,5 @@ class DenseModel:
         7 per layer, lm_head, argmax."""
         if self._step_ok(batch):
             return 1
-        return 2 + 7 * self.cfg.n_layers + 2
+        per_layer = 6 if self.kv8 and self.part8.numel() == 0 else 7      # one split: nothing to join
+        return 2 + per_layer * self.cfg.n_layers + 2

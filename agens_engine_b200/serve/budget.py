@@ -86,22 +86,33 @@ class Deployment:
     plan: dict
 
 
+def kv_cache_plan(cfg, wctx: int, max_batch: int, tp: int = 1, split_keys: int = 64) -> dict:
+    """What the KV cache's format means for a plan: bytes beside the pool, keys per attention split, whether pages may be tiered.  With
+    8-bit pages (``cfg.kv_cache``) one sequence's pages of one layer are held in bf16 for prefill and pages stay on the GPU."""
+    if cfg.kv_cache == "bf16":
+        return {"extra_bytes": 0, "split_keys": split_keys, "host_tier": True}
+    from ..ops.kv8 import split_keys_for
+    return {"extra_bytes": wctx * (cfg.kv_dim // tp) * 4, "split_keys": split_keys_for(wctx, max_batch * (cfg.n_kv_heads // tp)), "host_tier": False}
+
+
 def plan_deployment(cfg, budget_gib: float, wctx: int, max_batch: int, sessions: int, prefill_chunk: int, tp: int = 1,
                     gpu_free_gib: Optional[float] = None, host_avail_gib: float = -1.0, allow_host_tier: bool = True,
                     weights_bytes: Optional[int] = None, dual_layout: bool = False, split_keys: int = 64) -> Deployment:
     """Runs the planner for one rank of a ``tp``-way deployment of the architecture ``cfg`` (the full model's config).
     ``weights_bytes``: measured bytes when the weights are already on the device, else the architecture's estimate
-    plus 0.6 GiB of CUDA context; ``dual_layout`` doubles the quantised linears (the step kernel's second layout)."""
+    plus 0.6 GiB of CUDA context; ``dual_layout`` doubles the quantised linears (the step kernel's second layout, which a model
+    with an 8-bit KV cache does not have)."""
     from . import host as H
+    kv = kv_cache_plan(cfg, wctx, max_batch, tp, split_keys)
     if weights_bytes is None:
         lin = cfg.weight_bytes(tp) - cfg.vocab * cfg.d_model * 2
-        weights_bytes = cfg.weight_bytes(tp) + (lin if dual_layout else 0) + int(0.6 * GiB)
+        weights_bytes = cfg.weight_bytes(tp) + (lin if dual_layout and cfg.kv_cache == "bf16" else 0) + int(0.6 * GiB)
     p = H.plan(budget_gib=float(budget_gib), gpu_free_gib=float(gpu_free_gib if gpu_free_gib is not None else 170.0),
-               weights_bytes=int(weights_bytes), kv_bytes_per_token=int(cfg.kv_bytes_per_token(tp)), page_size=cfg.page_size,
+               weights_bytes=int(weights_bytes) + kv["extra_bytes"], kv_bytes_per_token=int(cfg.kv_bytes_per_token(tp)), page_size=cfg.page_size,
                max_batch=int(max_batch), sessions=int(sessions), prefill_chunk=int(prefill_chunk), d_model=cfg.d_model, ffn=cfg.ffn,
                q_dim=cfg.q_dim, kv_dim=cfg.kv_dim, vocab=cfg.vocab, n_heads=cfg.n_heads, head_dim=cfg.head_dim, tp=int(tp),
-               wctx=int(wctx), host_avail_gib=float(host_avail_gib), allow_host_tier=bool(allow_host_tier),
-               split_keys=int(split_keys))
+               wctx=int(wctx), host_avail_gib=float(host_avail_gib), allow_host_tier=bool(allow_host_tier and kv["host_tier"]),
+               split_keys=int(kv["split_keys"]))
     if "error" in p:
         raise ValueError(p["error"])
     ps = cfg.page_size

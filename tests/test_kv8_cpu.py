@@ -113,3 +113,44 @@ def test_the_format_holds_rows_to_half_a_step(fmt):
     assert bool(((k - x).abs() <= step * (1 + 1e-6)).all()) and torch.equal(k, v)
     assert bool(torch.isnan(values(c.pool, HD, fmt)[0][c.bt[0, -1].long(), :, 2:]).all())      # 50 = 3 * 16 + 2: what lies behind is NaN
     assert fields(c.pool, HD)[0].shape == (7, 2, 16, HD)
+
+
+def test_the_budget_counts_8_bit_pages():
+    import dataclasses
+    from agens_engine_b200.models import config as Cf
+    from agens_engine_b200.serve import budget as B
+    cfg = Cf.dense_32b(seed=0)
+    k8 = dataclasses.replace(cfg, kv_cache="int8")
+    assert cfg.kv_bytes_per_token() == 64 * 2 * 8 * 128 * 2 and k8.kv_bytes_per_token() == 64 * 8 * (2 * 128 + 8) and k8.kv_bytes_per_token(4) == 64 * 2 * 264
+    a, b = (B.plan_deployment(c, 24, 262144, 1, 1, 2048, gpu_free_gib=170, host_avail_gib=64) for c in (cfg, k8))
+    assert a.host_tier and not b.host_tier and b.fits            # 8-bit pages are not tiered: the context is what the pool holds
+    assert b.max_ctx == b.n_pages * 16 > 1.9 * a.n_pages * 16
+    kv = B.kv_cache_plan(k8, 262144, 1)
+    assert kv == {"extra_bytes": 262144 * 1024 * 4, "split_keys": 1024, "host_tier": False}
+    assert B.kv_cache_plan(cfg, 262144, 1, split_keys=64) == {"extra_bytes": 0, "split_keys": 64, "host_tier": True}
+
+
+def test_the_command_line_takes_a_cache_format(monkeypatch, capsys):
+    from agens_engine_b200 import cli
+    out = {}
+    for fmt in ("bf16", "fp8"):
+        assert cli.main(["plan", "--random", "dense-32b", "--budget-gib", "64", "--wctx", "65536", "--kv-cache", fmt, "--host-avail-gib", "8"]) == 0
+        out[fmt] = [line for line in capsys.readouterr().out.splitlines() if "KV pool" in line][0]
+    pages = {k: int(v.split("KV pool ")[1].split()[0]) for k, v in out.items()}
+    assert pages["fp8"] > 1.8 * pages["bf16"]
+    monkeypatch.setenv("B200E_KV_CACHE", "int4")
+    with pytest.raises(SystemExit, match="kv-cache"):
+        cli.main(["plan", "--random", "dense-32b", "--budget-gib", "64"])
+
+
+def test_a_model_refuses_a_format_that_is_not_there():
+    import dataclasses
+    from agens_engine_b200.models import config as Cf
+    from agens_engine_b200.models.dense import DenseModel
+    cfg = Cf.oracle_tiny()
+    with pytest.raises(ValueError, match="kv_cache"):
+        DenseModel(cfg, "cpu", kv_cache="q8")
+    with pytest.raises(ValueError, match="16 tokens"):
+        DenseModel(dataclasses.replace(cfg, page_size=32), "cpu", kv_cache="int8")
+    with pytest.raises(ValueError, match="heads of 64 or 128"):
+        DenseModel(dataclasses.replace(cfg, head_dim=32), "cpu", kv_cache="fp8")

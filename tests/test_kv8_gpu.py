@@ -284,6 +284,72 @@ def test_attend_split_sizes_and_a_workspace_of_the_caller(split):
     assert torch.equal(many, out)
 
 
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("lens,new,split", [([1500, 1400, 1450, 901], [6] * 4, 128), ([40 + 83 * i % 600 for i in range(40)], [1] * 40, 64)])
+def test_attend_work_of_many_groups_heads_and_splits(lens, new, split, fmt):
+    """Several times as much as runs at once: what works on one head or group goes on with the next one."""
+    hq, hkv, hd = 64, 8, 128
+    c = Cache(lens, hkv, hd, fmt, seed=split, k_amp=2.0)
+    pos, seq, g0, gc = _groups(lens, new)
+    q = bf(torch.randn(len(pos), hq * hd))
+    out = _attend(c, q, hq, pos, seq, g0, gc, split_keys=split)
+    _check_attend(c, q, hq, out, pos, seq, g0, gc)
+    pool = c.pool.to(DEV)
+    for t in range(len(pos)):
+        assert torch.equal(_attend(c, q[t:t + 1], hq, pos[t:t + 1], seq[t:t + 1], [0], [1], pool=pool, split_keys=split)[0], out[t]), t
+
+
+def test_attend_more_groups_than_a_warp_has_lanes():
+    hq, hkv, hd = 4, 2, 64
+    lens = [1 + 37 * i % 190 for i in range(75)]
+    new = [1 + i % min(5, n) for i, n in enumerate(lens)]
+    c = Cache(lens, hkv, hd, "int8", seed=1)
+    pos, seq, g0, gc = _groups(lens, new)
+    gc[40] = 0                                                # rows of no group: not written
+    q = bf(torch.randn(len(pos), hq * hd))
+    out = torch.full((len(pos), hq * hd), 9.0, dtype=torch.bfloat16, device=DEV)
+    got = _attend(c, q, hq, pos, seq, g0, gc, split_keys=32, out=out)
+    _check_attend(c, q, hq, got, pos, seq, g0, gc)
+    assert bool((got[g0[40]:g0[41]] == 9).all())
+
+
+def test_attend_calls_that_run_at_the_same_time():
+    """Two streams and two graphs, captured on one stream and replayed on two, none with a workspace of the caller."""
+    hq, hkv, hd = 64, 8, 128
+    c = Cache([3000, 2500], hkv, hd, "int8", seed=5)
+    pool, bt = c.pool.to(DEV), c.bt.to(DEV)
+    q = [bf(torch.randn(2, hq * hd)).to(DEV) for _ in range(4)]
+    args = (bt, i32([0, 1]), i32([1, 1]), i32([2999, 2499]), i32([0, 1]), hq, hkv, hd)
+    st = torch.zeros(1, dtype=torch.int32, device=DEV)
+    run = lambda i, o: K.attn_decode8(q[i], pool, "int8", *args, split_keys=64, status=st, out=o)
+    want = [run(i, None).clone() for i in range(4)]
+    out = [torch.zeros_like(want[0]) for _ in range(4)]
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    graphs = []
+    torch.cuda.synchronize()
+    for i in (2, 3):
+        with torch.cuda.stream(streams[0]):
+            run(i, out[i])
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=streams[0]):
+            run(i, out[i])
+        graphs.append(g)
+    for _ in range(20):
+        for o in out:
+            o.zero_()
+        torch.cuda.synchronize()
+        for i in range(4):
+            with torch.cuda.stream(streams[i]):
+                if i < 2:
+                    run(i, out[i])
+                else:
+                    graphs[i - 2].replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want))
+    assert int(st.item()) == 0
+
+
 def test_attend_refuses_positions_past_max_ctx():
     hq, hkv, hd = 4, 2, 64
     c = Cache([600, 600], hkv, hd, "int8")

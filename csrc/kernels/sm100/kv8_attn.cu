@@ -22,10 +22,20 @@
 // Loads.  Every warp copies its own pages, two at a time, into one of two places in shared memory (cp.async, no barrier but the
 // warp's) and runs ahead into the CTA's next item, whose page numbers were fetched an item earlier.
 //
-// Range.  The weights reach the second product as fp16 numbers p_j vs_j.  m is kept so that these stay below 2^kGrow: what is
-// rounded is each key's contribution relative to the largest one, whatever the size of V; a key that has weight but no V (a row
-// of zeros has the least scale) cannot push the others out of fp16's range.  m is raised only when a weight has passed 2^kGrow,
-// which leaves the accumulators alone for nearly all pages.
+// Range.  The weights reach the second product as fp16 numbers p_j vs_j: what is rounded is each key's contribution relative to the
+// largest one, whatever the size of V, and a key that has weight but no V (a row of zeros has the least scale) cannot push the
+// others out of fp16's range.  m begins as the largest contribution of a warp's first pair of pages and is raised only when a weight
+// passes kGrow = 2^14, a quarter of fp16's range, which leaves the accumulators alone for nearly all pages.
+//
+// What bounds it, and what it measured (B200, 64 q and 8 KV heads of 128, join included).  Decode: the copies.  One sequence of 131072
+// keys 56 us (277 MB: 4.97 TB/s; the same loop with its copies alone 48 us), 24 sequences of 3300 to 6500 in fp8 36 us (155 MB, 4.3 TB/s;
+// 30 us), one of 700 7.2 us: launch, one page's latency, join.  Verify blocks (4 sequences of 9001, 6 rows each, int8): 54 us for
+// 63 MB, the chain of products, weights and conversions of two warps a scheduler (0.34 instructions a cycle, half of the stalls are
+// results of the instruction before); sixteen columns an item, since twenty-four took 59 and eight convert all of K and V twice as often.
+// Tried and slower: codes in registers instead of shared memory (24 sequences 53 us), pages converted once for 64 columns by all warps
+// together (verify 66 us, a barrier every pair of pages), bulk copies of four rows (41 and 63 us: they arrive later), tcgen05 products
+// with V converted into shared memory (54 and 56 us, 77 for 131072 keys: with eight columns the products are all issue and latency,
+// and rows of verify blocks must not differ from decode), joining in the last CTA of a row (45 us).
 #include <algorithm>
 #include <type_traits>
 
@@ -54,7 +64,7 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kJoin = 16;                   // splits that are joined at once
 constexpr float kNoRef = -3.4028234e38f;    // m before the first key
-constexpr float kGrow = 256.f;              // what a weight may reach before m follows
+constexpr float kGrow = 16384.f;              // what a weight may reach before m follows
 
 __device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 __device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
@@ -443,14 +453,14 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_attn_kernel(
         }
         return top;
       };
-      if (__any_sync(0xffffffffu, weigh() > kGrow)) {
+      if (i == 0 || __any_sync(0xffffffffu, weigh() > kGrow)) {
         // columns that passed it: m becomes their largest s + log2 of vs's power of two, so that weights begin below 2 again
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          float top = 0.f, mx = kNoRef;
+          float top = i == 0 ? INFINITY : 0.f, mx = kNoRef;
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
-            top = fmaxf(top, w[j >> 2][n][j & 3]);
+            if (i != 0) top = fmaxf(top, w[j >> 2][n][j & 3]);
             const float e = __uint_as_float(0x4b000000u | (__float_as_uint(vs[j >> 2][j & 3]) >> 23)) - 8388735.f;
             mx = fmaxf(mx, __fadd_rn(__fmul_rn(s[j >> 2][n][j & 3], qs[n]), e));
           }
@@ -460,6 +470,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_attn_kernel(
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
           float f = 1.f;
           if (top > kGrow) { f = ex2(__fadd_rn(m[n], -mx)); m[n] = mx; }
+          if (i == 0) continue;                     // nothing has been added up
           l[n] = __fmul_rn(l[n], f);
           const float f0 = __shfl_sync(0xffffffffu, f, 8 * t), f1 = __shfl_sync(0xffffffffu, f, 8 * t + 4);
 #pragma unroll

@@ -11,13 +11,14 @@ What a kernel finds out of range (a page, a position past the block table) sets 
 """
 from __future__ import annotations
 
+import functools
 import math
 from typing import Optional
 
 import torch
 
 from .. import _lib
-from .._lib import Kv8AttnArgs, Kv8StoreArgs, check
+from .._lib import Kv8AttnArgs, Kv8ReadArgs, Kv8StoreArgs, check, packer
 
 PAGE = 16
 FORMATS = {"int8": 0, "fp8": 1}
@@ -37,6 +38,7 @@ def make_pool(n_pages: int, hkv: int, hd: int, device) -> torch.Tensor:
     return torch.zeros(n_pages, hkv, block_bytes(hd), dtype=torch.uint8, device=device)
 
 
+@functools.lru_cache(maxsize=None)
 def split_keys_for(max_ctx: int, heads: int = 8) -> int:
     """Keys of one attention split for ``heads`` pairs of a sequence and a KV head with contexts of up to ``max_ctx`` tokens: 128, doubled
     up to 512 while that makes more splits than CTAs run at once, and beyond while a context had more than 256.  A constant of the
@@ -123,6 +125,7 @@ def _check_table(bt: torch.Tensor, dev: int):
 _BF16, _I32, _U8, _F32 = torch.bfloat16, torch.int32, torch.uint8, torch.float32
 _LOG2E = math.log2(math.e)
 _HD_OF = {block_bytes(hd): hd for hd in (64, 128)}
+_store_args, _attn_args, _read_args = packer(Kv8StoreArgs), packer(Kv8AttnArgs), packer(Kv8ReadArgs)
 
 
 def _launch(name: str, dev: int, *args):
@@ -171,7 +174,7 @@ def rope_kvstore8(qkv: torch.Tensor, hq: int, hkv: int, hd: int, inv_freq: torch
         status = torch.zeros(1, dtype=_I32, device=qkv.device)
     at_status = _check_index(status, 1, dev, "status")
     if n:
-        a = Kv8StoreArgs(qkv.data_ptr(), ld, n, hq, hkv, inv_freq.data_ptr(), at_pos, at_rope, at_rope3, at_axis, at_seq, seqs, block_table.data_ptr(), bt_ld,
+        a = _store_args(qkv.data_ptr(), ld, n, hq, hkv, inv_freq.data_ptr(), at_pos, at_rope, at_rope3, at_axis, at_seq, seqs, block_table.data_ptr(), bt_ld,
                          cols, pool.data_ptr(), pool.shape[0], q_out.data_ptr(), ldq, at_status)
         _launch("b2_kv8_store", dev, a, hd, f)
     return status
@@ -226,7 +229,7 @@ def attn_decode8(q: torch.Tensor, pool: torch.Tensor, fmt: str, block_table: tor
         if part is None and slots:
             part = torch.empty(slots * (hd + 2), dtype=_F32, device=q.device)
         at_o = part.data_ptr() if slots else 0
-        a = Kv8AttnArgs(q.data_ptr(), ldq, pool.data_ptr(), pool.shape[0], block_table.data_ptr(), bt_ld, cols, seqs, at_tok0, at_cnt, n_groups, at_pos, at_seq, n,
+        a = _attn_args(q.data_ptr(), ldq, pool.data_ptr(), pool.shape[0], block_table.data_ptr(), bt_ld, cols, seqs, at_tok0, at_cnt, n_groups, at_pos, at_seq, n,
                         at_mask, hq, hkv, _LOG2E / math.sqrt(hd), out.data_ptr(), ldo, at_status, split_keys, splits, at_o, at_o + 4 * slots * hd)
         _launch("b2_kv8_attn", dev, a, hd, f)
     return out
@@ -252,5 +255,5 @@ def kv_read8(pool: torch.Tensor, fmt: str, pages: torch.Tensor, n_tokens: Option
         status = torch.zeros(1, dtype=_I32, device=pool.device)
     at_status = _check_index(status, 1, dev, "status")
     if n:
-        _launch("b2_kv8_read", dev, pool.data_ptr(), pool.shape[0], hkv, hd, f, at_pages, n, n_tokens, out.data_ptr(), at_status)
+        _launch("b2_kv8_read", dev, _read_args(pool.data_ptr(), pool.shape[0], hkv, at_pages, n, n_tokens, out.data_ptr(), at_status), hd, f)
     return out

@@ -24,6 +24,13 @@ struct Kv8StoreArgs {
   int* status;
 };
 
+struct Kv8ReadArgs {
+  const uint8_t* pool; int n_pages, hkv;
+  const int* pages; int n_out; long n_tokens;
+  bf16* out;
+  int* status;
+};
+
 namespace {
 
 __device__ __forceinline__ void unpack8(uint4 v, float (&f)[8]) {
@@ -132,19 +139,18 @@ __global__ void __launch_bounds__(256) kv8_store_kernel(const Kv8StoreArgs a, in
 // Pages [n_out] of the pool as bf16 pages [n_out][2][hkv][16][hd]; slots from n_tokens on are zeros.  A CTA expands a page of a KV
 // head, a thread eight codes of K and eight of V, so that a warp's stores are whole lines.
 template <int HD, int FMT>
-__global__ void __launch_bounds__(2 * HD) kv8_read_kernel(const uint8_t* __restrict__ pool, int n_pages, int hkv, const int* __restrict__ pages,
-                                                          long n_tokens, bf16* __restrict__ out, int* __restrict__ status) {
+__global__ void __launch_bounds__(2 * HD) kv8_read_kernel(const Kv8ReadArgs a) {
   pdl_wait();
   pdl_launch_dependents();
   const int pi = blockIdx.x, h = blockIdx.y, c = threadIdx.x, row = c / (HD / 8);
-  const bool live = (long)pi * kKv8Page + row < n_tokens;
-  const int page = live ? pages[pi] : -1;
-  const bool there = page >= 0 && page < n_pages;
-  if (live && !there && c == 0) atomicExch(status, (int)B2_ERR_BOUNDS);
+  const bool live = (long)pi * kKv8Page + row < a.n_tokens;
+  const int page = live ? a.pages[pi] : -1;
+  const bool there = page >= 0 && page < a.n_pages;
+  if (live && !there && c == 0) atomicExch(a.status, (int)B2_ERR_BOUNDS);
   uint2 w[2] = {make_uint2(0u, 0u), make_uint2(0u, 0u)};
   uint2 sc = make_uint2(0u, 0u);
   if (there) {
-    const uint8_t* blk = pool + ((size_t)page * hkv + h) * kv8_block_bytes(HD);
+    const uint8_t* blk = a.pool + ((size_t)page * a.hkv + h) * kv8_block_bytes(HD);
     w[0] = ld_nc_v2(blk + c * 8);
     w[1] = ld_nc_v2(blk + kKv8Page * HD + c * 8);
     sc = ld_nc_v2(blk + 2 * kKv8Page * HD + row * 8);
@@ -157,7 +163,7 @@ __global__ void __launch_bounds__(2 * HD) kv8_read_kernel(const uint8_t* __restr
     kv8_values<FMT>(w[kv].y, f + 4);
 #pragma unroll
     for (int i = 0; i < 8; ++i) f[i] = there ? __fmul_rn(f[i], s) : 0.f;
-    *reinterpret_cast<uint4*>(out + (((size_t)pi * 2 + kv) * hkv + h) * kKv8Page * HD + c * 8) = pack8(f);
+    *reinterpret_cast<uint4*>(a.out + (((size_t)pi * 2 + kv) * a.hkv + h) * kKv8Page * HD + c * 8) = pack8(f);
   }
 }
 
@@ -191,11 +197,11 @@ B2_API int b2_kv8_store(const Kv8StoreArgs* args, int hd, int fmt, cudaStream_t 
   return launch(k, dim3((unsigned)blocks), 256, st, a, parts);
 }
 
-B2_API int b2_kv8_read(const uint8_t* pool, int n_pages, int hkv, int hd, int fmt, const int* pages, int n_out, long n_tokens,
-                       bf16* out, int* status, cudaStream_t st) {
-  if (n_out < 1 || hkv < 1 || hkv > 65535 || n_pages < 1 || n_tokens < 0) return B2_ERR_ARG;
+B2_API int b2_kv8_read(const Kv8ReadArgs* args, int hd, int fmt, cudaStream_t st) {
+  const Kv8ReadArgs& a = *args;
+  if (a.n_out < 1 || a.hkv < 1 || a.hkv > 65535 || a.n_pages < 1 || a.n_tokens < 0) return B2_ERR_ARG;
   if ((hd != 64 && hd != 128) || (fmt != KV8_INT8 && fmt != KV8_FP8)) return B2_ERR_ARG;
   auto k = hd == 128 ? (fmt == KV8_INT8 ? kv8_read_kernel<128, KV8_INT8> : kv8_read_kernel<128, KV8_FP8>)
                      : (fmt == KV8_INT8 ? kv8_read_kernel<64, KV8_INT8> : kv8_read_kernel<64, KV8_FP8>);
-  return launch(k, dim3(n_out, hkv), 2 * hd, st, pool, n_pages, hkv, pages, n_tokens, out, status);
+  return launch(k, dim3(a.n_out, a.hkv), 2 * hd, st, a);
 }

@@ -1,7 +1,10 @@
 """What the 8-bit key-value cache refuses, and its reference's own format, without a GPU."""
+import ctypes as C
+
 import pytest
 import torch
 
+from agens_engine_b200 import _lib
 from agens_engine_b200.ops import kv8 as K
 
 from tests.kv8_reference import FMTS, Cache, encode, fields, values
@@ -76,8 +79,6 @@ def test_read_refuses():
 
 def test_the_library_refuses_what_the_launchers_would_not_pass_on():
     """The C entries check their own arguments: nothing is launched (1 is a bad argument)."""
-    import ctypes as C
-    from agens_engine_b200 import _lib
     lib = _lib.cuda_lib()
     s = _lib.Kv8StoreArgs(n=1, hq=1, hkv=1, n_seq=1, bt_cols=1, n_pages=1)
     for hd, fmt, kw in ((96, 0, {}), (64, 2, {}), (64, 0, dict(n=0)), (64, 0, dict(ld=4)), (128, 1, dict(n_pages=0)), (64, 0, dict(n_seq=0))):
@@ -94,7 +95,14 @@ def test_the_library_refuses_what_the_launchers_would_not_pass_on():
         assert lib.b2_kv8_attn(C.byref(b), hd, fmt, None) == 1
     for bad in ((0, 1, 64, 0, 1, 0), (1, 0, 64, 0, 1, 0), (1, 1, 80, 0, 1, 0), (1, 1, 64, 5, 1, 0), (1, 1, 64, 0, 0, 0), (1, 1, 64, 0, 1, -1)):
         n_pages, hkv, hd, fmt, n_out, n_tok = bad
-        assert lib.b2_kv8_read(None, n_pages, hkv, hd, fmt, None, n_out, n_tok, None, None, None) == 1
+        assert lib.b2_kv8_read(_lib.packer(_lib.Kv8ReadArgs)(0, n_pages, hkv, 0, n_out, n_tok, 0, 0), hd, fmt, None) == 1
+
+
+@pytest.mark.parametrize("cls", [_lib.Kv8StoreArgs, _lib.Kv8AttnArgs, _lib.Kv8ReadArgs])
+def test_packed_arguments_are_the_structures_bytes(cls):
+    values = [1000 + 7 * i if t is not C.c_float else 0.375 for i, (_, t) in enumerate(cls._fields_)]
+    got = cls.from_buffer_copy(_lib.packer(cls)(*values))
+    assert [getattr(got, name) for name, _ in cls._fields_] == values
 
 
 def test_splits_for_a_context():

@@ -46,62 +46,72 @@ __device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
   return v;
 }
 
-// Rotation (pairs i, i + hd/2) by pos * inv_freq, q rounded once to bf16, k and v quantised from fp32.
+// Rotation (pairs i, i + hd/2) by pos * inv_freq, q rounded once to bf16, k and v quantised from fp32:
+//     (lo, hi) -> (lo cos - hi sin, hi cos + lo sin);    scale = max(max |x| / top, 2^-64), code = round(x / scale)
 // HD / 16 lanes hold a head, eight rotary pairs each, so a warp takes 32 / (HD / 16) heads at a time ("a turn") and has the next turn's
-// loads under way meanwhile.  `parts` CTAs share a token; each takes the token's sines and cosines once.
+// loads under way meanwhile.  `parts` CTAs share a token, or a CTA has `toks` (one or two); each takes a token's sines and cosines once.
+// Bound by the chain of launch, positions, sines and rows for few tokens (one token of 64 q and 8 KV heads of 128: 2.4 us, 48 tokens
+// 2.5 us), by memory for many: 2048 tokens 17.1 us, 80 MB at 4.7 TB/s (19.4 with a token a CTA; two turns under way were slower).
 template <int HD, int FMT>
-__global__ void __launch_bounds__(256) kv8_store_kernel(const Kv8StoreArgs a, int parts) {
+__global__ void __launch_bounds__(256) kv8_store_kernel(const Kv8StoreArgs a, int parts, int toks) {
   constexpr int LPH = HD / 16, HPW = 32 / LPH, HALF = HD / 2;
-  __shared__ __align__(16) float sh_c[HALF], sh_s[HALF];
+  __shared__ __align__(16) float sh_c[2][HALF], sh_s[2][HALF];
+  __shared__ int sh_page[2], sh_slot[2];
   pdl_wait();
   pdl_launch_dependents();
   const int lane = threadIdx.x & 31, l = lane % LPH, sub = lane / LPH;
-  const int tok = blockIdx.x / parts, part = blockIdx.x % parts;
-  const int heads = a.hq + 2 * a.hkv, turns = (heads + HPW - 1) / HPW;
+  const int tok0 = blockIdx.x / parts * toks, part = blockIdx.x % parts;
+  const int heads = a.hq + 2 * a.hkv, turns = (heads + HPW - 1) / HPW, all = min(toks, a.n - tok0) * turns;
   int turn = part * 8 + (threadIdx.x >> 5);
-  const bf16* row = a.qkv + (size_t)tok * a.ld + l * 8;
   uint4 lo8 = make_uint4(0u, 0u, 0u, 0u), hi8 = lo8;
   auto load = [&](int t) {
-    const int head = t * HPW + sub;
-    if (t < turns && head < heads) {
-      lo8 = ld_nc_v4(row + (size_t)head * HD);
-      hi8 = ld_nc_v4(row + (size_t)head * HD + HALF);
+    const int u = t >= turns, head = (t - u * turns) * HPW + sub;
+    if (t < all && head < heads) {
+      const bf16* src = a.qkv + (size_t)(tok0 + u) * a.ld + (size_t)head * HD + l * 8;
+      lo8 = ld_nc_v4(src);
+      hi8 = ld_nc_v4(src + HALF);
     }
   };
   load(turn);
-  const int pos = a.tok_pos[tok], seq = a.tok_seq[tok];
 
   // The angle in turns, in 64 bits: a 32-bit product of a position of 100000 and a frequency near one is off by several
   // thousandths of a radian.  Its fraction goes to sincospi, which needs no argument reduction of its own.
-  if (threadIdx.x < HALF) {
-    const int i = threadIdx.x;
-    int p = a.rope_pos ? a.rope_pos[tok] : pos;
-    if (a.rope_pos3) p = a.rope_pos3[(size_t)min((int)a.pair_axis[i], 2) * a.n + tok];
+  const int mine = threadIdx.x / HALF, tok1 = tok0 + mine;
+  if (mine < toks && tok1 < a.n) {
+    const int i = threadIdx.x % HALF;
+    int p = a.rope_pos ? a.rope_pos[tok1] : a.tok_pos[tok1];
+    if (a.rope_pos3) p = a.rope_pos3[(size_t)min((int)a.pair_axis[i], 2) * a.n + tok1];
     double t = (double)p * (double)a.inv_freq[i] * 0.15915494309189535;
     t -= rint(t);
-    sincospif((float)(2.0 * t), &sh_s[i], &sh_c[i]);
+    sincospif((float)(2.0 * t), &sh_s[mine][i], &sh_c[mine][i]);
   }
-  int page = -1;
-  if (pos >= 0 && pos / kKv8Page < a.bt_cols && seq >= 0 && seq < a.n_seq) page = a.block_table[(size_t)seq * a.bt_ld + pos / kKv8Page];
-  const bool stored = page >= 0 && page < a.n_pages;
-  if (!stored && part == 0 && threadIdx.x == 0) atomicExch(a.status, (int)B2_ERR_BOUNDS);
+  if (threadIdx.x >= 254 && tok0 + (int)threadIdx.x - 254 < a.n && (int)threadIdx.x - 254 < toks) {
+    const int u = threadIdx.x - 254, pos = a.tok_pos[tok0 + u], seq = a.tok_seq[tok0 + u];
+    int page = -1;
+    if (pos >= 0 && pos / kKv8Page < a.bt_cols && seq >= 0 && seq < a.n_seq) page = a.block_table[(size_t)seq * a.bt_ld + pos / kKv8Page];
+    if (page >= a.n_pages) page = -1;
+    if (page < 0 && part == 0) atomicExch(a.status, (int)B2_ERR_BOUNDS);
+    sh_page[u] = page;
+    sh_slot[u] = pos % kKv8Page;
+  }
   __syncthreads();
-  float c[8], s[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) { c[i] = sh_c[l * 8 + i]; s[i] = sh_s[l * 8 + i]; }
 
-  for (; turn < turns; turn += 8 * parts) {
-    const int head = turn * HPW + sub;
+  for (; turn < all; turn += 8 * parts) {
+    const int u = turn >= turns, head = (turn - u * turns) * HPW + sub, tok = tok0 + u, page = sh_page[u];
+    const bool stored = page >= 0;
     float lo[8], hi[8];
     unpack8(lo8, lo);
     unpack8(hi8, hi);
     load(turn + 8 * parts);
     if (head < a.hq + a.hkv) {
+      const float4* c4 = reinterpret_cast<const float4*>(&sh_c[u][l * 8]);
+      const float4* s4 = reinterpret_cast<const float4*>(&sh_s[u][l * 8]);
+      const float4 cv[2] = {c4[0], c4[1]}, sv[2] = {s4[0], s4[1]};
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float x = lo[i], y = hi[i];
-        lo[i] = x * c[i] - y * s[i];
-        hi[i] = y * c[i] + x * s[i];
+        const float x = lo[i], y = hi[i], c = (&cv[i >> 2].x)[i & 3], s = (&sv[i >> 2].x)[i & 3];
+        lo[i] = x * c - y * s;
+        hi[i] = y * c + x * s;
       }
     }
     if (head < a.hq) {
@@ -109,7 +119,7 @@ __global__ void __launch_bounds__(256) kv8_store_kernel(const Kv8StoreArgs a, in
       *reinterpret_cast<uint4*>(dst) = pack8(lo);
       *reinterpret_cast<uint4*>(dst + HALF) = pack8(hi);
     }
-    if (turn * HPW + HPW <= a.hq) continue;            // q heads only, for the whole warp
+    if (head - sub + HPW <= a.hq) continue;            // q heads only, for the whole warp
     // the largest magnitude, compared as bits: a NaN's are above an infinity's, so neither is lost
     uint32_t mx = 0;
 #pragma unroll
@@ -118,7 +128,7 @@ __global__ void __launch_bounds__(256) kv8_store_kernel(const Kv8StoreArgs a, in
     for (int o = LPH / 2; o > 0; o >>= 1) mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
     if (head >= heads || head < a.hq || !stored) continue;
     const bool is_v = head >= a.hq + a.hkv;
-    const int kvh = head - a.hq - (is_v ? a.hkv : 0), slot = pos % kKv8Page;
+    const int kvh = head - a.hq - (is_v ? a.hkv : 0), slot = sh_slot[u];
     const float scale = fmaxf(__fdiv_rn(__uint_as_float(mx), FMT == KV8_INT8 ? 127.f : 448.f), kKv8MinScale);
     const bool finite = mx < 0x7f800000u;
     uint32_t clo[2] = {0u, 0u}, chi[2] = {0u, 0u};
@@ -136,8 +146,9 @@ __global__ void __launch_bounds__(256) kv8_store_kernel(const Kv8StoreArgs a, in
   }
 }
 
-// Pages [n_out] of the pool as bf16 pages [n_out][2][hkv][16][hd]; slots from n_tokens on are zeros.  A CTA expands a page of a KV
-// head, a thread eight codes of K and eight of V, so that a warp's stores are whole lines.
+// Pages [n_out] of the pool as bf16 pages [n_out][2][hkv][16][hd], code * scale rounded once; slots from n_tokens on are zeros.  A CTA
+// expands a page of a KV head, a thread eight codes of K and eight of V, so that a warp's stores are whole lines.  Bound by memory: 65536
+// tokens of 8 heads of 128 68 us (407 MB, 5.95 TB/s, 0.92 of a copy's rate; 72 with blocks of 256 threads over pages and heads at large).
 template <int HD, int FMT>
 __global__ void __launch_bounds__(2 * HD) kv8_read_kernel(const Kv8ReadArgs a) {
   pdl_wait();
@@ -190,11 +201,14 @@ B2_API int b2_kv8_store(const Kv8StoreArgs* args, int hd, int fmt, cudaStream_t 
   const int hpw = 32 / (hd / 16), turns = (a.hq + 2 * a.hkv + hpw - 1) / hpw;
   // few tokens: a CTA for eight turns, so that no warp has two; many: a CTA for a token, whose sines and cosines are taken once
   const int most = (turns + 7) / 8, parts = (long)a.n * most <= 148 * 4 ? most : 1;
-  const long blocks = (long)a.n * parts;
+  // two tokens a CTA where that leaves every SM one: 2048 tokens of 64 + 16 heads (two and a half turns a warp) 17.1 us instead of 19.5,
+  // 4000 of 24 + 8 (one turn a warp) 17.8 instead of 21.3; 48 tokens 3.4 instead of 2.5
+  const int toks = parts == 1 && a.n >= 2 * 148 ? 2 : 1;
+  const long blocks = ((long)a.n + toks - 1) / toks * parts;
   if (blocks > 0x7fffffffl) return B2_ERR_ARG;
   auto k = hd == 128 ? (fmt == KV8_INT8 ? kv8_store_kernel<128, KV8_INT8> : kv8_store_kernel<128, KV8_FP8>)
                      : (fmt == KV8_INT8 ? kv8_store_kernel<64, KV8_INT8> : kv8_store_kernel<64, KV8_FP8>);
-  return launch(k, dim3((unsigned)blocks), 256, st, a, parts);
+  return launch(k, dim3((unsigned)blocks), 256, st, a, parts, toks);
 }
 
 B2_API int b2_kv8_read(const Kv8ReadArgs* args, int hd, int fmt, cudaStream_t st) {

@@ -133,6 +133,21 @@ def test_store_skips_and_reports_what_is_out_of_range():
     _check_stored(q[good], pool, hq, hkv, hd, "int8", [pos[i] for i in good], [0, 0], bt, qkv[good], lambda i: float(pos[good[i]]))
 
 
+@pytest.mark.parametrize("hq,hkv,hd,n", [(6, 1, 128, 297), (64, 8, 128, 301), (5, 3, 64, 650)])
+def test_store_of_many_tokens_some_of_them_nowhere(hq, hkv, hd, n):
+    """An odd number of tokens, where blocks take two; slots 96 to 111 have no page, one token no sequence."""
+    pos, seq = list(range(n)), [0] * n
+    pages = (n + PAGE - 1) // PAGE
+    bt = torch.randperm(pages).to(torch.int32).view(1, -1)
+    bt[0, 6] = pages
+    seq[n - 2] = 1
+    qkv = bf(torch.randn(n, (hq + 2 * hkv) * hd))
+    q, pool, st = _store(hq, hkv, hd, "int8", pos, seq, bt, pages, qkv)
+    assert st == 4
+    good = [i for i in range(n) if i // PAGE != 6 and i != n - 2]
+    _check_stored(q[good], pool, hq, hkv, hd, "int8", [pos[i] for i in good], [0] * len(good), bt, qkv[good], lambda i: float(good[i]))
+
+
 # ---------------------------------------------------------------------------------------------------------------- read
 @pytest.mark.parametrize("fmt", FMTS)
 @pytest.mark.parametrize("hkv,hd,n", [(8, 128, 1), (2, 64, 16), (1, 128, 17), (3, 64, 100), (2, 128, 333)])

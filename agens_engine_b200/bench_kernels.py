@@ -5,7 +5,7 @@ is taken with CUDA events on the launching stream after warm-up; the L2 is flush
 a buffer larger than L2 (256 MiB).  Roofline denominators come from ``MEASURED_PEAKS.json`` when present.
 
     python -m agens_engine_b200.bench_kernels gemv [--m 1] [--small]
-    python -m agens_engine_b200.bench_kernels attn
+    python -m agens_engine_b200.bench_kernels attn | kv8
     python -m agens_engine_b200.bench_kernels gemm
 """
 from __future__ import annotations
@@ -264,6 +264,60 @@ def bench_attn(args):
     print(json.dumps({"peaks": pk, "timing": "CUDA events, median of 10, L2 flushed; split kernel + merge kernel"}))
 
 
+def _kv8_case(ctx: int, rows: int, seqs: int, fmt: str, dev, hq=64, hkv=8, hd=128):
+    """``seqs`` sequences of ``ctx`` tokens in 8-bit pages and ``rows`` new rows at the end of each; a call and its K/V bytes."""
+    from .ops import kv8 as K
+    n_pages = (ctx + 15) // 16
+    g = torch.Generator(device=dev).manual_seed(ctx + rows)
+    pool = K.make_pool(seqs * n_pages, hkv, hd, dev)
+    pool[..., :32 * hd] = torch.randint(0, 120, (*pool.shape[:2], 32 * hd), device=dev, generator=g, dtype=torch.uint8)
+    pool[..., 32 * hd:].view(torch.float32).fill_(0.01)
+    bt = torch.randperm(seqs * n_pages, device=dev, generator=g).to(torch.int32).view(seqs, n_pages)
+    q = torch.randn(seqs * rows, hq * hd, device=dev, generator=g).to(torch.bfloat16)
+    i = lambda v: torch.tensor(v, dtype=torch.int32, device=dev)
+    idx = (i([s * rows for s in range(seqs)]), i([rows] * seqs), i([ctx - rows + r for _ in range(seqs) for r in range(rows)]), i([s for s in range(seqs) for _ in range(rows)]))
+    st = torch.zeros(1, dtype=torch.int32, device=dev)
+    return (lambda: K.attn_decode8(q, pool, fmt, bt, *idx, hq, hkv, hd, status=st)), seqs * ctx * hkv * (2 * hd + 8), st
+
+
+def bench_kv8(args):
+    """8-bit KV cache of the 32B shape (64 q / 8 kv heads x 128): attention of decode steps and verify blocks at several lengths, reading
+    65536 tokens back and storing 2048; CUDA events, L2 flushed."""
+    from .ops import basic, kv8 as K
+    dev = "cuda:0"
+    pk = peaks()
+    flush = L2Flusher(dev)
+    for seqs, ctx, rows in ([(1, 2560, 1)] if args.small else [(1, 2560, 1), (1, 32768, 1), (1, 131072, 1), (24, 5000, 1), (4, 9000, 6), (1, 32768, 8)]):
+        for fmt in K.FORMATS:
+            fn, nbytes, st = _kv8_case(ctx, rows, seqs, fmt, dev)
+            med, _ = time_cuda(fn, iters=10, warmup=3, flush=flush)
+            print(json.dumps(dict(op="attend", fmt=fmt, seqs=seqs, ctx=ctx, rows=rows, us=round(med, 1), kv_gbs=round(nbytes / med / 1e3, 1),
+                                  frac_hbm_single_read=round(nbytes / med / 1e3 / pk["hbm_gbs"], 3), status=int(st.item()))), flush=True)
+    n = 1024 if args.small else 65536
+    pool = K.make_pool(n // 16, 8, 128, dev)
+    pages = torch.randperm(n // 16, device=dev).to(torch.int32)
+    for fmt in K.FORMATS:
+        med, _ = time_cuda(lambda: K.kv_read8(pool, fmt, pages), iters=10, warmup=3, flush=flush)
+        print(json.dumps(dict(op="read", fmt=fmt, tokens=n, us=round(med, 1), gbs=round(n * 8 * (264 + 512) / med / 1e3, 1))), flush=True)
+        rows = min(n, 2048)
+        qkv = torch.randn(rows, 80 * 128, device=dev).to(torch.bfloat16)
+        q = torch.empty(rows, 64 * 128, dtype=torch.bfloat16, device=dev)
+        pos, seq = torch.arange(rows, dtype=torch.int32, device=dev), torch.zeros(rows, dtype=torch.int32, device=dev)
+        inv = basic.rope_inv_freq(128, 1e6, dev)
+        med, _ = time_cuda(lambda: K.rope_kvstore8(qkv, 64, 8, 128, inv, pos, seq, pages[None, :], pool, fmt, q), iters=10, warmup=3, flush=flush)
+        print(json.dumps(dict(op="store", fmt=fmt, tokens=rows, us=round(med, 1), gbs=round(rows * (144 * 256 + 8 * 264) / med / 1e3, 1))), flush=True)
+    print(json.dumps({"peaks": pk, "timing": "CUDA events, median of 10, L2 flushed; split kernel + join kernel"}))
+
+
+def profile_kv8(args):
+    """A few plain launches of the attention over 8-bit pages (int8) for a profiler capture: ``--rows`` rows at ``--ctx`` tokens."""
+    fn, nbytes, st = _kv8_case(args.ctx, args.rows, 1, "int8", "cuda:0")
+    for _ in range(3):
+        fn()
+    torch.cuda.synchronize()
+    print("profile_kv8 done, status", int(st.item()), "bytes", nbytes)
+
+
 def profile_attn(args):
     """A few plain launches for a profiler capture: by default a 256-row prefill chunk at an 8K context (CTA-shared
     ring); ``--rows 1 --ctx 32768`` is one decode row over 134 MB of K/V (64-key splits, per-warp ring)."""
@@ -369,7 +423,7 @@ def profile_step(args):
 
 def main(argv=None):
     ap = argparse.ArgumentParser()
-    ap.add_argument("what", choices=["gemv", "bf16", "attn", "gemm", "profile_gemv", "mm", "profile_mm", "profile_attn", "profile_attn_tc", "profile_gemm", "profile_misc", "profile_step"])
+    ap.add_argument("what", choices=["gemv", "bf16", "attn", "gemm", "profile_gemv", "mm", "profile_mm", "profile_attn", "profile_attn_tc", "profile_gemm", "profile_misc", "profile_step", "kv8", "profile_kv8"])
     ap.add_argument("--layers", type=int, default=0)
     ap.add_argument("--bits", type=int, default=4)
     ap.add_argument("--m", type=int, default=1)
@@ -391,6 +445,10 @@ def main(argv=None):
         profile_mm(args)
     elif args.what == "attn":
         bench_attn(args)
+    elif args.what == "kv8":
+        bench_kv8(args)
+    elif args.what == "profile_kv8":
+        profile_kv8(args)
     elif args.what == "profile_attn":
         profile_attn(args)
     elif args.what == "profile_attn_tc":

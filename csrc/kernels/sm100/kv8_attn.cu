@@ -29,7 +29,7 @@
 //
 // What bounds it, and what it measured (B200, 64 q and 8 KV heads of 128, join included).  Decode: the copies.  One sequence of 131072
 // keys 56 us (277 MB: 4.97 TB/s; the same loop with its copies alone 48 us), 24 sequences of 2000 to 4001 in fp8 36 us (155 MB, 4.3 TB/s;
-// 30 us), one of 700 7.2 us: launch, one page's latency, join.  Verify blocks (4 sequences of 4500 to 9001, 6 rows each, int8): 54 us for
+// 30 us), one of 700 7.2 us: launch, one page's latency, join.  Verify blocks (4 sequences of 5626 to 9001, 6 rows each, int8): 54 us for
 // 63 MB, the chain of products, weights and conversions of two warps a scheduler (0.34 instructions a cycle, half of the stalls are
 // results of the instruction before); sixteen columns an item, since twenty-four took 59 and eight convert all of K and V twice as often.
 // Tried and slower: codes in registers instead of shared memory (24 sequences 53 us), pages converted once for 64 columns by all warps

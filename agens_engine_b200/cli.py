@@ -232,11 +232,12 @@ def cmd_plan(ns):
     from .serve import budget as B
     mc = _model_config(cfg)
     kv = B.kv_cache_plan(mc, cfg.wctx, cfg.max_batch, cfg.tp, cfg.split_keys)
+    kw = {} if mc.kv_cache == "bf16" else dict(allow_host_tier=kv["host_tier"], split_keys=kv["split_keys"])
     rep = H.plan(budget_gib=cfg.budget_gib, gpu_free_gib=ns.gpu_free_gib, weights_bytes=mc.weight_bytes(cfg.tp) + kv["extra_bytes"],
                  kv_bytes_per_token=mc.kv_bytes_per_token(cfg.tp), page_size=mc.page_size, max_batch=cfg.max_batch,
                  sessions=cfg.max_convs, prefill_chunk=ns.plan_prefill_chunk, d_model=mc.d_model, ffn=mc.ffn, q_dim=mc.q_dim,
                  kv_dim=mc.kv_dim, vocab=mc.vocab, n_heads=mc.n_heads, head_dim=mc.head_dim, tp=cfg.tp, wctx=cfg.wctx,
-                 host_avail_gib=ns.host_avail_gib, allow_host_tier=kv["host_tier"], split_keys=kv["split_keys"])
+                 host_avail_gib=ns.host_avail_gib, **kw)
     for line in rep.get("lines", []):
         print(line)
     print(json.dumps({k: v for k, v in rep.items() if k != "lines"}, indent=1))

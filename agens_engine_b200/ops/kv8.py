@@ -188,7 +188,8 @@ def attn_decode8(q: torch.Tensor, pool: torch.Tensor, fmt: str, block_table: tor
     ``[n_tok, hq * hd]`` (RoPE applied).  Group ``g`` is the ``grp_cnt[g]`` (at most 32) rows from ``grp_tok0[g]`` on, all of one
     sequence in ascending order of ``tok_pos``, whose K and V are in the pool already; row i sees the slots up to ``tok_pos[i]``, of
     the slots from the group's first on those whose bit its ``tree_mask`` (int32 ``[n_tok]``) has.  A row that sees nothing
-    (``tok_pos`` -1 in a group of its own, an empty mask) gives zeros; rows of no group are left as they were in ``out``.
+    (``tok_pos`` -1 in a group of its own, an empty mask) gives zeros; rows of no group are left as they were in ``out``, which does
+    not overlap ``q``.
 
     ``split_keys`` (a multiple of 16, at most 2048; default :func:`split_keys_for` the table's size) cuts every sequence into
     splits that are joined at the end; a row's bits depend on its own position and on ``split_keys`` only.  ``max_ctx`` (default:

@@ -71,23 +71,26 @@ def _format(fmt: str) -> int:
     return f
 
 
-def _check_pool(pool: torch.Tensor, dev: int) -> int:
-    """Head size of a pool's pages."""
-    if not (pool.dtype is _U8 and pool.dim() == 3 and pool.is_contiguous() and pool.data_ptr() % 16 == 0):
+def _check_pool(pool: torch.Tensor, dev: int):
+    """Pages, KV heads, head size and address of a pool."""
+    shape, at = pool.shape, pool.data_ptr()
+    if not (pool.dtype is _U8 and len(shape) == 3 and pool.is_contiguous() and at % 16 == 0):
         _fail("the pool is a contiguous uint8 tensor [pages, hkv, 32 * hd + 128]")
-    pages, _, size = pool.shape
+    pages, hkv, size = shape
     hd = _HD_OF.get(size)
-    if hd is None or pages == 0:
-        _fail(f"a pool of {tuple(pool.shape)} holds no pages of head_dim 64 or 128")
+    if not (hd and pages):
+        _fail(f"a pool of {tuple(shape)} holds no pages of head_dim 64 or 128")
     if pool.get_device() != dev:
         _fail("all tensors on one device")
-    return hd
+    return pages, hkv, hd, at
 
 
 def _check_heads(pool: torch.Tensor, dev: int, hkv: int, hd: int):
-    got = _check_pool(pool, dev)
-    if got != hd or pool.shape[1] != hkv:
-        _fail(f"the pool's pages are of {pool.shape[1]} KV heads of {got}")
+    """Pages and address of a pool for ``hkv`` KV heads of ``hd``."""
+    pages, heads, size, at = _check_pool(pool, dev)
+    if size != hd or heads != hkv:
+        _fail(f"the pool's pages are of {heads} KV heads of {size}")
+    return pages, at
 
 
 def _check_index(t: torch.Tensor, n: int, dev: int, name: str) -> int:
@@ -96,30 +99,27 @@ def _check_index(t: torch.Tensor, n: int, dev: int, name: str) -> int:
     return t.data_ptr()
 
 
-def _check_rows(t: torch.Tensor, n: int, width: int, dev: int, name: str, align: int) -> int:
-    """Distance of two rows of a bf16 [n, width] tensor."""
+def _check_rows(t: torch.Tensor, n: int, width: int, dev: int, name: str):
+    """Distance of two rows of a bf16 [n, width] tensor, and its address."""
+    at = t.data_ptr()
     if not (t.dtype is _BF16 and t.shape == (n, width) and t.get_device() == dev):
         _fail(f"{name}: bf16 [{n}, {width}] on the device of the rows")
-    if t.is_contiguous():
-        ld = width
-    else:
-        ld, unit = t.stride()
-        if unit != 1:
-            ld = 1
-    if ld % align or t.data_ptr() % (2 * align):
-        _fail(f"{name}: rows of unit stride that start on {2 * align}-byte boundaries")
-    return ld
+    ld, unit = (width, 1) if t.is_contiguous() else t.stride()
+    if ld % 8 or at % 16 or unit != 1:
+        _fail(f"{name}: rows of unit stride that start on 16-byte boundaries")
+    return ld, at
 
 
 def _check_table(bt: torch.Tensor, dev: int):
-    """Sequences, pages of a sequence and distance of two rows of a block table."""
-    if not (bt.dtype is _I32 and bt.dim() == 2 and bt.get_device() == dev):
+    """Sequences, pages of a sequence, distance of two rows and address of a block table."""
+    shape = bt.shape
+    if not (bt.dtype is _I32 and len(shape) == 2 and bt.get_device() == dev):
         _fail("block_table: int32 [sequences, pages] on the device of the rows")
-    seqs, cols = bt.shape
+    seqs, cols = shape
     ld, unit = (cols, 1) if bt.is_contiguous() else bt.stride()
     if cols == 0 or unit != 1:
         _fail("block_table: rows of unit stride, at least one page each")
-    return seqs, cols, ld
+    return seqs, cols, ld, bt.data_ptr()
 
 
 _BF16, _I32, _U8, _F32 = torch.bfloat16, torch.int32, torch.uint8, torch.float32
@@ -133,7 +133,7 @@ def _launch(name: str, dev: int, *args):
     if dev < 0:
         _fail("tensors on a CUDA device")
     fn = getattr(_lib.cuda_lib(), name)
-    if torch.cuda.current_device() == dev:
+    if torch._C._cuda_getDevice() == dev:
         rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
     else:
         with torch.cuda.device(dev):
@@ -154,10 +154,10 @@ def rope_kvstore8(qkv: torch.Tensor, hq: int, hkv: int, hd: int, inv_freq: torch
     n = qkv.shape[0]
     if hq < 1 or hkv < 1:
         _fail("hq and hkv are positive")
-    _check_heads(pool, dev, hkv, hd)
-    ld = _check_rows(qkv, n, (hq + 2 * hkv) * hd, dev, "qkv", 8)
-    ldq = _check_rows(q_out, n, hq * hd, dev, "q_out", 8)
-    seqs, cols, bt_ld = _check_table(block_table, dev)
+    n_pages, at_pool = _check_heads(pool, dev, hkv, hd)
+    ld, at_qkv = _check_rows(qkv, n, (hq + 2 * hkv) * hd, dev, "qkv")
+    ldq, at_q = _check_rows(q_out, n, hq * hd, dev, "q_out")
+    seqs, cols, bt_ld, at_bt = _check_table(block_table, dev)
     at_pos, at_seq = _check_index(tok_pos, n, dev, "tok_pos"), _check_index(tok_seq, n, dev, "tok_seq")
     at_rope = 0 if rope_pos is None else _check_index(rope_pos, n, dev, "rope_pos")
     if not (inv_freq.dtype is _F32 and inv_freq.numel() == hd // 2 and inv_freq.is_contiguous() and inv_freq.get_device() == dev
@@ -174,8 +174,8 @@ def rope_kvstore8(qkv: torch.Tensor, hq: int, hkv: int, hd: int, inv_freq: torch
         status = torch.zeros(1, dtype=_I32, device=qkv.device)
     at_status = _check_index(status, 1, dev, "status")
     if n:
-        a = _store_args(qkv.data_ptr(), ld, n, hq, hkv, inv_freq.data_ptr(), at_pos, at_rope, at_rope3, at_axis, at_seq, seqs, block_table.data_ptr(), bt_ld,
-                         cols, pool.data_ptr(), pool.shape[0], q_out.data_ptr(), ldq, at_status)
+        a = _store_args(at_qkv, ld, n, hq, hkv, inv_freq.data_ptr(), at_pos, at_rope, at_rope3, at_axis, at_seq, seqs, at_bt, bt_ld, cols, at_pool, n_pages,
+                        at_q, ldq, at_status)
         _launch("b2_kv8_store", dev, a, hd, f)
     return status
 
@@ -199,17 +199,16 @@ def attn_decode8(q: torch.Tensor, pool: torch.Tensor, fmt: str, block_table: tor
     n = q.shape[0]
     if hkv < 1 or hq < 1 or hq % hkv:
         _fail("hq is a multiple of hkv")
-    _check_heads(pool, dev, hkv, hd)
-    ldq = _check_rows(q, n, hq * hd, dev, "q", 8)
-    seqs, cols, bt_ld = _check_table(block_table, dev)
+    n_pages, at_pool = _check_heads(pool, dev, hkv, hd)
+    ldq, at_q = _check_rows(q, n, hq * hd, dev, "q")
+    seqs, cols, bt_ld, at_bt = _check_table(block_table, dev)
     n_groups = grp_tok0.numel()
     at_tok0, at_cnt = _check_index(grp_tok0, n_groups, dev, "grp_tok0"), _check_index(grp_cnt, n_groups, dev, "grp_cnt")
     at_pos, at_seq = _check_index(tok_pos, n, dev, "tok_pos"), _check_index(tok_seq, n, dev, "tok_seq")
     at_mask = 0 if tree_mask is None else _check_index(tree_mask, n, dev, "tree_mask")
     if out is None:
-        out, ldo = torch.empty(n, hq * hd, dtype=_BF16, device=q.device), hq * hd
-    else:
-        ldo = _check_rows(out, n, hq * hd, dev, "out", 8)
+        out = torch.empty(n, hq * hd, dtype=_BF16, device=q.device)
+    ldo, at_out = _check_rows(out, n, hq * hd, dev, "out")
     if max_ctx is None:
         max_ctx = cols * PAGE
     elif not 0 < max_ctx <= cols * PAGE:
@@ -230,8 +229,8 @@ def attn_decode8(q: torch.Tensor, pool: torch.Tensor, fmt: str, block_table: tor
         if part is None and slots:
             part = torch.empty(slots * (hd + 2), dtype=_F32, device=q.device)
         at_o = part.data_ptr() if slots else 0
-        a = _attn_args(q.data_ptr(), ldq, pool.data_ptr(), pool.shape[0], block_table.data_ptr(), bt_ld, cols, seqs, at_tok0, at_cnt, n_groups, at_pos, at_seq, n,
-                        at_mask, hq, hkv, _LOG2E / math.sqrt(hd), out.data_ptr(), ldo, at_status, split_keys, splits, at_o, at_o + 4 * slots * hd)
+        a = _attn_args(at_q, ldq, at_pool, n_pages, at_bt, bt_ld, cols, seqs, at_tok0, at_cnt, n_groups, at_pos, at_seq, n, at_mask, hq, hkv,
+                       _LOG2E / math.sqrt(hd), at_out, ldo, at_status, split_keys, splits, at_o, at_o + 4 * slots * hd)
         _launch("b2_kv8_attn", dev, a, hd, f)
     return out
 
@@ -241,8 +240,8 @@ def kv_read8(pool: torch.Tensor, fmt: str, pages: torch.Tensor, n_tokens: Option
     """The named pages (int32 ``[n]``, a row of a block table or any list) as bf16 pages ``[n, 2, hkv, 16, hd]``, the layout of the
     bf16 pool.  Slots from ``n_tokens`` on (counted over the list) are zeros and are not read; default: every slot."""
     f, dev = _format(fmt), pool.get_device()
-    hd = _check_pool(pool, dev)
-    n, hkv = pages.numel(), pool.shape[1]
+    n_pages, hkv, hd, at_pool = _check_pool(pool, dev)
+    n = pages.numel()
     at_pages = _check_index(pages, n, dev, "pages")
     if n_tokens is None:
         n_tokens = n * PAGE
@@ -256,5 +255,5 @@ def kv_read8(pool: torch.Tensor, fmt: str, pages: torch.Tensor, n_tokens: Option
         status = torch.zeros(1, dtype=_I32, device=pool.device)
     at_status = _check_index(status, 1, dev, "status")
     if n:
-        _launch("b2_kv8_read", dev, _read_args(pool.data_ptr(), pool.shape[0], hkv, at_pages, n, n_tokens, out.data_ptr(), at_status), hd, f)
+        _launch("b2_kv8_read", dev, _read_args(at_pool, n_pages, hkv, at_pages, n, n_tokens, out.data_ptr(), at_status), hd, f)
     return out

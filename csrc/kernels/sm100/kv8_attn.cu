@@ -29,12 +29,12 @@
 //
 // What bounds it, and what it measured (B200, 64 q and 8 KV heads of 128, join included).  Decode: the copies.  One sequence of 131072
 // keys 56 us (277 MB: 4.97 TB/s; the same loop with its copies alone 48 us), 24 sequences of 2000 to 4001 in fp8 36 us (155 MB, 4.3 TB/s;
-// 30 us), one of 700 7.2 us: launch, one page's latency, join.  Verify blocks (4 sequences of 5626 to 9001, 6 rows each, int8): 54 us for
-// 63 MB, the chain of products, weights and conversions of two warps a scheduler (0.34 instructions a cycle, half of the stalls are
-// results of the instruction before); sixteen columns an item, since twenty-four took 59 and eight convert all of K and V twice as often.
+// 30 us), one of 700 7.2 us: launch, one page's latency, join.  Verify blocks (4 sequences of 5626 to 9001, 6 rows each, int8): 49 us for
+// 63 MB, the chain of products, weights and conversions of two warps a scheduler (0.40 instructions a cycle; 620 of them a pair of pages
+// and 750 an item of four pairs); sixteen columns an item: twenty-four were 7 % slower and eight convert all of K and V twice as often.
 // Tried and slower: codes in registers instead of shared memory (24 sequences 53 us), pages converted once for 64 columns by all warps
-// together (verify 66 us, a barrier every pair of pages), bulk copies of four rows (41 and 63 us: they arrive later), tcgen05 products
-// with V converted into shared memory (54 and 56 us, 77 for 131072 keys: with eight columns the products are all issue and latency,
+// together (verify 66 us when this took 54, a barrier every pair of pages), bulk copies of four rows (41 and 63 us: they arrive later), tcgen05
+// products with V converted into shared memory (54 and 56 us, 77 for 131072 keys: with eight columns the products are all issue and latency,
 // and rows of verify blocks must not differ from decode), joining in the last CTA of a row (45 us).
 #include <algorithm>
 #include <type_traits>
@@ -194,6 +194,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_attn_kernel(
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float sh_m[kWarps][COLS], sh_l[kWarps][COLS];
   __shared__ int sh_at[kWarps];
+  __shared__ long sh_to[COLS];           // a column's first part, or its place in the output if it has one split
+  __shared__ int sh_ns[COLS];            // its splits, 0 behind the last column
   pdl_wait();
   pdl_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -288,6 +290,16 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_attn_kernel(
     send(rd ^ flip, 1);
 
     if (!same_q) {
+      if (threadIdx.x < COLS) {
+        const int col = col0 + threadIdx.x;
+        int ns = 0;
+        if (col < cnt * gq) {
+          const int tok = tok0 + col / gq, head = kvh * gq + col % gq;
+          ns = cnt == 1 ? cur.ns : splits_of(min(a.tok_pos[tok], last), a.split_keys);
+          sh_to[threadIdx.x] = ns == 1 ? (long)tok * a.ldo + (long)head * HD : ((long)tok * a.hq + head) * a.max_splits;
+        }
+        sh_ns[threadIdx.x] = ns;
+      }
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         const int col = col0 + n * 8 + g;
@@ -539,15 +551,9 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_attn_kernel(
     __syncthreads();
 #pragma unroll
     for (int i = threadIdx.x; i < COLS * (HD / 4); i += kWarps * 32) {
-      const int c = i / (HD / 4), d = i % (HD / 4) * 4, col = col0 + c;
-      if (col >= cnt * gq) continue;
-      int tok = tok0, head = kvh * gq + col, ns = cur.ns;
-      if (cnt > 1) {
-        const int row = col / gq;
-        tok += row; head -= row * gq;
-        ns = splits_of(min(a.tok_pos[tok], last), a.split_keys);
-        if (split >= ns) continue;
-      }
+      const int c = i / (HD / 4), d = i % (HD / 4) * 4, ns = sh_ns[c];
+      if (split >= ns) continue;
+      const long to = sh_to[c];
       float M = sh_m[0][c];
 #pragma unroll
       for (int w = 1; w < kWarps; ++w) M = fmaxf(M, sh_m[w][c]);
@@ -565,9 +571,9 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_attn_kernel(
         uint2 v;
         *reinterpret_cast<__nv_bfloat162*>(&v.x) = __floats2bfloat162_rn(__fmul_rn(x.x, inv), __fmul_rn(x.y, inv));
         *reinterpret_cast<__nv_bfloat162*>(&v.y) = __floats2bfloat162_rn(__fmul_rn(x.z, inv), __fmul_rn(x.w, inv));
-        *reinterpret_cast<uint2*>(a.out + (size_t)tok * a.ldo + (size_t)head * HD + d) = v;
+        *reinterpret_cast<uint2*>(a.out + to + d) = v;
       } else {
-        const size_t slot = ((size_t)tok * a.hq + head) * a.max_splits + split;
+        const long slot = to + split;
         *reinterpret_cast<float4*>(a.part_o + slot * HD + d) = x;
         if (d == 0) *reinterpret_cast<float2*>(a.part_ml + slot * 2) = make_float2(M, L);
       }

@@ -106,8 +106,11 @@ def test_packed_arguments_are_the_structures_bytes(cls):
 
 
 def test_splits_for_a_context():
-    assert [K.split_keys_for(n) for n in (1, 700, 7040, 7041, 8000, 16000, 131072, 131073, 1 << 19, 1 << 20)] == [128, 128, 128, 256, 256, 512, 512, 1024, 2048, 2048]
-    assert [K.split_keys_for(4000, h) for h in (2, 8, 16, 1000)] == [128, 128, 256, 512]
+    sizes = (1, 700, 7040, 7041, 8000, 16000, 28160, 28161, 131072, 196608, 196609, 262145, 1 << 20)
+    assert [K.split_keys_for(n) for n in sizes] == [128, 128, 128, 256, 256, 512, 512, 768, 768, 768, 1024, 2048, 2048]
+    assert [K.split_keys_for(4000, h) for h in (2, 8, 16, 55, 56, 1000)] == [128, 128, 256, 512, 768, 768]
+    assert [K.split_keys_for(n, 1) for n in (50000, 131072, 131073, 300000)] == [256, 512, 768, 2048]
+    assert all(K.split_keys_for(n, h) % 16 == 0 and K.split_keys_for(n, h) <= K.MAX_SPLIT for n in range(1, 10 ** 6, 7919) for h in (1, 8, 512))
     assert K.part_floats(3, 8, 128, 256, 256) == 0 and K.part_floats(3, 8, 128, 257, 256) == 3 * 8 * 2 * 130 and K.part_floats(1, 2, 64, 100, 16) == 2 * 7 * 66
 
 

@@ -28,10 +28,10 @@
 // passes kGrow = 2^14, a quarter of fp16's range, which leaves the accumulators alone for nearly all pages.
 //
 // What bounds it, and what it measured (B200, 64 q and 8 KV heads of 128, join included).  Decode: the copies.  One sequence of 131072
-// keys 56 us (277 MB: 4.97 TB/s; the same loop with its copies alone 48 us), 24 sequences of 2000 to 4001 in fp8 36 us (155 MB, 4.3 TB/s;
-// 30 us), one of 700 7.2 us: launch, one page's latency, join.  Verify blocks (4 sequences of 5626 to 9001, 6 rows each, int8): 49 us for
+// keys 54 us (277 MB: 5.1 TB/s; the same loop with its copies alone 48 us), 24 sequences of 2000 to 4001 in fp8 34.7 us (155 MB, 4.5 TB/s;
+// 30 us), one of 700 7.2 us: launch, one page's latency, join.  Verify blocks (4 sequences of 5626 to 9001, 6 rows each, int8): 47.6 us for
 // 63 MB, the chain of products, weights and conversions of two warps a scheduler (0.40 instructions a cycle; 620 of them a pair of pages
-// and 750 an item of four pairs); sixteen columns an item: twenty-four were 7 % slower and eight convert all of K and V twice as often.
+// and 700 an item of six pairs, three or four items a CTA); sixteen columns an item: twenty-four were 7 % slower and eight convert all of K and V twice as often.
 // Tried and slower: codes in registers instead of shared memory (24 sequences 53 us), pages converted once for 64 columns by all warps
 // together (verify 66 us when this took 54, a barrier every pair of pages), bulk copies of four rows (41 and 63 us: they arrive later), tcgen05
 // products with V converted into shared memory (54 and 56 us, 77 for 131072 keys: with eight columns the products are all issue and latency,
@@ -192,10 +192,11 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_attn_kernel(
   // a warp's results of an item go over the pair of pages that it used last, which is not refilled before they have been read
   static_assert(COLS * LDO * 4 <= PAIR, "a tile of results fits a pair of pages");
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ float sh_m[kWarps][COLS], sh_l[kWarps][COLS];
-  __shared__ int sh_at[kWarps];
-  __shared__ long sh_to[COLS];           // a column's first part, or its place in the output if it has one split
-  __shared__ int sh_ns[COLS];            // its splits, 0 behind the last column
+  __shared__ __align__(16) float sh_m[COLS][kWarps], sh_l[COLS][kWarps];
+  __shared__ __align__(16) int sh_at[kWarps];
+  // a column's first part, or its place in the output if it has one split; its splits, 0 behind the last column
+  struct __align__(16) Target { long to; int ns; };
+  __shared__ Target sh_to[COLS];
   pdl_wait();
   pdl_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -292,13 +293,13 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_attn_kernel(
     if (!same_q) {
       if (threadIdx.x < COLS) {
         const int col = col0 + threadIdx.x;
-        int ns = 0;
+        Target x = {0, 0};
         if (col < cnt * gq) {
           const int tok = tok0 + col / gq, head = kvh * gq + col % gq;
-          ns = cnt == 1 ? cur.ns : splits_of(min(a.tok_pos[tok], last), a.split_keys);
-          sh_to[threadIdx.x] = ns == 1 ? (long)tok * a.ldo + (long)head * HD : ((long)tok * a.hq + head) * a.max_splits;
+          x.ns = cnt == 1 ? cur.ns : splits_of(min(a.tok_pos[tok], last), a.split_keys);
+          x.to = x.ns == 1 ? (long)tok * a.ldo + (long)head * HD : ((long)tok * a.hq + head) * a.max_splits;
         }
-        sh_ns[threadIdx.x] = ns;
+        sh_to[threadIdx.x] = x;
       }
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
@@ -539,7 +540,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_attn_kernel(
       float x = l[n];
       x = __fadd_rn(x, __shfl_xor_sync(0xffffffffu, x, 1));
       x = __fadd_rn(x, __shfl_xor_sync(0xffffffffu, x, 2));
-      if (t == 0) { sh_m[warp][n * 8 + g] = m[n]; sh_l[warp][n * 8 + g] = x; }
+      if (t == 0) { sh_m[n * 8 + g][warp] = m[n]; sh_l[n * 8 + g][warp] = x; }
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
 #pragma unroll
@@ -549,21 +550,23 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_attn_kernel(
       }
     }
     __syncthreads();
+    const int4 at = *reinterpret_cast<const int4*>(sh_at);
 #pragma unroll
     for (int i = threadIdx.x; i < COLS * (HD / 4); i += kWarps * 32) {
-      const int c = i / (HD / 4), d = i % (HD / 4) * 4, ns = sh_ns[c];
+      const int c = i / (HD / 4), d = i % (HD / 4) * 4;
+      const Target target = sh_to[c];
+      const int ns = target.ns;
+      const long to = target.to;
       if (split >= ns) continue;
-      const long to = sh_to[c];
-      float M = sh_m[0][c];
-#pragma unroll
-      for (int w = 1; w < kWarps; ++w) M = fmaxf(M, sh_m[w][c]);
+      const float4 ms = *reinterpret_cast<const float4*>(sh_m[c]), ls = *reinterpret_cast<const float4*>(sh_l[c]);
+      const float M = fmaxf(fmaxf(fmaxf(ms.x, ms.y), ms.z), ms.w);
       float L = 0.f;
       float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
-        const float f = ex2(__fadd_rn(sh_m[w][c], -M));
-        const float4 y = *reinterpret_cast<const float4*>(smem + sh_at[w] + (c * LDO + d) * 4);
-        L = __fmaf_rn(sh_l[w][c], f, L);
+        const float f = ex2(__fadd_rn((&ms.x)[w], -M));
+        const float4 y = *reinterpret_cast<const float4*>(smem + (&at.x)[w] + (c * LDO + d) * 4);
+        L = __fmaf_rn((&ls.x)[w], f, L);
         x.x = __fmaf_rn(y.x, f, x.x); x.y = __fmaf_rn(y.y, f, x.y); x.z = __fmaf_rn(y.z, f, x.z); x.w = __fmaf_rn(y.w, f, x.w);
       }
       if (ns == 1) {

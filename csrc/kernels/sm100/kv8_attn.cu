@@ -1,12 +1,12 @@
 // Attention of new tokens over 8-bit key-value pages (format: kv8.cuh): decode steps, verify blocks (causal or tree mask)
 // and short prefill chunks.  Counterpart in the reference: the INT8 KV of its dense layers, which expands tiles to bf16 and
-// attends to those (kernels/m1/m1_dense8.cu:65-126); here the codes go straight into the products.
+// attends to those (kernels/m1/m1_dense8.cu:65-126); here the codes become operands in registers.
 //
 //     o = sum_j p_j vs_j vc_j / sum_j p_j,    p_j = 2^(s_j - m),    s_j = log2(e) / sqrt(hd) * ks_j * (q . kc_j)
 //
-// over the keys j that the row sees.  One pass with a running reference m.  The int8 codes kc go into an integer product with q in
-// sixteen bits; e4m3's, and all vc, become fp16 numbers (exactly: both formats fit).  The scales stay in fp32: ks multiplies the
-// finished product, vs the weight before it is rounded.
+// over the keys j that the row sees.  One pass with a running reference m.  The codes kc and vc become fp16 numbers (exactly: both
+// formats fit), q's too, times a power of two of its column.  The scales stay in fp32: ks multiplies the finished product, vs the
+// weight before it is rounded.
 //
 // Split.  A sequence's keys are cut every split_keys keys, a constant of the engine; one CTA of four warps takes the keys of one
 // (group, KV head, columns, split), page i of them on warp i % 4, and joins its warps in shared memory.  Rows with one split are
@@ -14,9 +14,8 @@
 // own position alone, so a row has the same bits in a decode step, a verify block or any batch.
 //
 // Products.  The group's rows times the q heads of a KV head are the columns, eight to a tile, so that a single decode row with
-// eight q heads wastes nothing.  S = q K^T takes q as A (its rows are the columns; for int8 the two bytes of eight columns) and K's
-// bytes as B just as they lie in shared memory; its result is, lane for lane, the B operand of O^T = V^T P^T, whose A are V's bytes
-// as fp16.  The order of channels inside a product and of keys inside a page is free, and chosen so that every lane reads sixteen
+// eight q heads wastes nothing.  S = q K^T takes q as A (its rows are the columns, eight of sixteen where there are no more) and
+// K's bytes as fp16 as B; its result is, lane for lane, the B operand of O^T = V^T P^T, whose A are V's bytes as fp16.  The order of channels inside a product and of keys inside a page is free, and chosen so that every lane reads sixteen
 // bytes of a row at a time and nothing has to be moved between lanes or registers.
 //
 // Loads.  Every warp copies its own pages, two at a time, into one of two places in shared memory (cp.async, no barrier but the
@@ -71,17 +70,21 @@ __device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
   const __half2 v = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
 }
-// D(16x8, s32) = A(16x32, s8, row) * B(32x8, u8, col) + C
-__device__ __forceinline__ void mma_s8u8(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, int c0, int c1, int c2, int c3) {
-  asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
-               : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
-               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(c0), "r"(c1), "r"(c2), "r"(c3));
-}
 // Taken off here and not from the finished sums (64 instructions a pair of pages less, 1 % of the time): the accumulators truncate,
 // and 1152 in every term cost a flat row of 131072 keys half of its last bf16 digit.
 __device__ __forceinline__ uint32_t minus_1152(uint32_t two) {
   const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&two), __half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480)));
   return *reinterpret_cast<const uint32_t*>(&v);
+}
+// The four channels of a K word as fp16 pairs (0, 1) and (2, 3)
+template <int FMT>
+__device__ __forceinline__ void k_pairs(uint32_t w, uint32_t& x, uint32_t& y) {
+  if (FMT == KV8_INT8) {
+    x = minus_1152(__byte_perm(w, 0x64646464u, 0x4140));               // 0x64xx is 1024 + xx
+    y = minus_1152(__byte_perm(w, 0x64646464u, 0x4342));
+  } else {
+    e4m3_pairs(w, x, y);
+  }
 }
 // Of two rows' words: pairs (row a, row b) of bytes 2 * HI and 2 * HI + 1
 template <int FMT, int HI>
@@ -184,8 +187,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_attn_kernel(
   constexpr int KC = HD / 64;            // 16-byte pieces of a K row per lane
   constexpr int VW = HD / 32;            // words of a V row per lane
   constexpr int MT = HD / 16;            // channel tiles of V^T P^T
-  constexpr int QM = FMT == KV8_INT8 ? NT : 1;            // A tiles of q: two bytes of eight columns, or sixteen columns in fp16
-  constexpr int QK = FMT == KV8_INT8 ? HD / 32 : HD / 16; // k-steps of q K^T
+  constexpr int QK = HD / 16;            // k-steps of q K^T
   constexpr int COLS = NT * 8;
   constexpr int LDO = HD + 4;
   constexpr int BLK = kv8_block_bytes(HD), PAIR = 2 * BLK;
@@ -272,13 +274,13 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_attn_kernel(
   };
 
   // q, every column scaled by a power of two; qs undoes it on the scores and brings the softmax scale.
-  // int8: sixteen bits of fixed point, the largest value in [2^14, 2^15), as two signed bytes (hi * 256 + lo): K's bytes then feed the
-  // product as they are, and the sums are exact.  What is lost is at most 2^-15 of the column's largest value.  The 128 in K's
-  // bytes comes off again with the accumulators' start, -128 * sum(q).
-  // e4m3: fp16 with the largest value in [2^10, 2^11), where a bf16 number stays exact down to 2^-24 of that.
-  uint32_t qa[QM][QK][4];
+  // The largest value lies in [2^10, 2^11): a bf16 number keeps its eight digits down to 2^-27 of that (fp16's step there is 2^-24), and
+  // sums of 128 products with codes up to 448 stay below 2^28.  int8 keys once went into an integer product as they are, with q as two
+  // bytes of fixed point: 4 to 6 % less time (131072 keys 54.2 us instead of 56.1, the verify block 47.6 instead of 50.6), but a channel
+  // below 2^-7 of the largest one lost digits, and with a channel of K as much larger the result was off by up to a tenth.  A third byte
+  // of q mends that too and takes longer (58.3 and 52.7).
+  uint32_t qa[QK][4];
   float qs[NT];
-  int q0[NT];
 
   send(rd, 0);
   for (bool same_q = false; item < item_end; ++item) {
@@ -319,37 +321,19 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_attn_kernel(
           }
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const uint32_t e = min((FMT == KV8_INT8 ? 268u : 264u) - (top >> 23), 253u);
+        const uint32_t e = min(264u - (top >> 23), 253u);
         const float up = __uint_as_float(e << 23);
         qs[n] = __fmul_rn(__uint_as_float((254u - e) << 23), a.scale_log2);
         if (top >= 0x7f800000u) qs[n] = __uint_as_float(0x7fffffffu);           // an infinity or a NaN in q: a column of NaN
-        int sum = 0;
 #pragma unroll
         for (int c = 0; c < KC; ++c)
 #pragma unroll
-          for (int w = 0; w < 4; ++w) {                // four channels of a K word
+          for (int w = 0; w < 4; ++w) {                // four channels of a K word; rows g and g + 8 of the tile: columns g and g + 8
             const uint32_t a0 = (&raw[c][w >> 1].x)[2 * (w & 1)], a1 = (&raw[c][w >> 1].x)[2 * (w & 1) + 1];
-            const float f0 = __uint_as_float(a0 << 16) * up, f1 = __uint_as_float(a0 & 0xffff0000u) * up;
-            const float f2 = __uint_as_float(a1 << 16) * up, f3 = __uint_as_float(a1 & 0xffff0000u) * up;
-            if constexpr (FMT == KV8_INT8) {           // rows g and g + 8 of the tile: hi and lo
-              // 32640 would need hi = 128: it becomes 32639
-              const int i0 = min(__float2int_rn(f0), 32639), i1 = min(__float2int_rn(f1), 32639);
-              const int i2 = min(__float2int_rn(f2), 32639), i3 = min(__float2int_rn(f3), 32639);
-              sum += i0 + i1 + i2 + i3;
-              const int w2 = c * 2 + (w >> 1), half = 2 * (w & 1);
-              qa[n][w2][half] = __byte_perm(__byte_perm(i0 + 128, i1 + 128, 0x0051), __byte_perm(i2 + 128, i3 + 128, 0x0051), 0x5410);
-              qa[n][w2][half + 1] = __byte_perm(__byte_perm(i0, i1, 0x0040), __byte_perm(i2, i3, 0x0040), 0x5410);
-            } else {                                   // rows g and g + 8 of the tile: columns g and g + 8
-              qa[0][c * 4 + w][n] = pack_half(f0, f1);
-              qa[0][c * 4 + w][2 + n] = pack_half(f2, f3);
-              if (NT == 1) qa[0][c * 4 + w][1] = qa[0][c * 4 + w][3] = 0u;
-            }
+            qa[c * 4 + w][n] = pack_half(__uint_as_float(a0 << 16) * up, __uint_as_float(a0 & 0xffff0000u) * up);
+            qa[c * 4 + w][2 + n] = pack_half(__uint_as_float(a1 << 16) * up, __uint_as_float(a1 & 0xffff0000u) * up);
+            if (NT == 1) qa[c * 4 + w][1] = qa[c * 4 + w][3] = 0u;
           }
-        if constexpr (FMT == KV8_INT8) {
-          sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-          sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-          q0[n] = -128 * sum;
-        }
       }
     }
     same_q = true;
@@ -371,42 +355,21 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_attn_kernel(
       float s[2][NT][4];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        if constexpr (FMT == KV8_INT8) {
-          int x[NT][2][4];                         // (hi, hi, lo, lo) of keys 4t + 2r, 4t + 2r + 1
 #pragma unroll
-          for (int r = 0; r < 2; ++r)
+        for (int r = 0; r < 2; ++r) {
+          float x[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int c = 0; c < KC; ++c) {
-              const uint4 k = ring.k(stage + h * BLK, r, c);
+          for (int c = 0; c < KC; ++c) {
+            const uint4 k = ring.k(stage + h * BLK, r, c);
 #pragma unroll
-              for (int n = 0; n < NT; ++n) {
-                int (&y)[4] = x[n][r];
-                if (c == 0) mma_s8u8(y, qa[n][0], k.x, k.y, 0, 0, q0[n], q0[n]);
-                else mma_s8u8(y, qa[n][2 * c], k.x, k.y, y[0], y[1], y[2], y[3]);
-                mma_s8u8(y, qa[n][2 * c + 1], k.z, k.w, y[0], y[1], y[2], y[3]);
-              }
+            for (int w = 0; w < 4; ++w) {
+              uint32_t b0, b1;
+              k_pairs<FMT>((&k.x)[w], b0, b1);
+              mma_f16_16816(x, qa[c * 4 + w], b0, b1);
             }
-#pragma unroll
-          for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) s[h][n][j] = __int2float_rn(x[n][j >> 1][j & 1] * 256 + x[n][j >> 1][2 + (j & 1)]);
-        } else {
-#pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            float x[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int c = 0; c < KC; ++c) {
-              const uint4 k = ring.k(stage + h * BLK, r, c);
-#pragma unroll
-              for (int w = 0; w < 4; ++w) {
-                uint32_t b0, b1;
-                e4m3_pairs((&k.x)[w], b0, b1);
-                mma_f16_16816(x, qa[0][c * 4 + w], b0, b1);
-              }
-            }
-#pragma unroll
-            for (int n = 0; n < NT; ++n) { s[h][n][2 * r] = x[2 * n]; s[h][n][2 * r + 1] = x[2 * n + 1]; }
           }
+#pragma unroll
+          for (int n = 0; n < NT; ++n) { s[h][n][2 * r] = x[2 * n]; s[h][n][2 * r + 1] = x[2 * n + 1]; }
         }
       }
       float vs[2][4];

@@ -1,0 +1,31 @@
+"""Attention over 8-bit pages where numbers of very different size meet, or that are none."""
+import pytest
+import torch
+
+from tests.kv8_reference import FMTS, Cache
+from tests.test_kv8_gpu import _attend, _check_attend, _groups, bf
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("hq,hkv,hd", [(16, 2, 128), (8, 2, 64)])
+@pytest.mark.parametrize("factor", [30.0, 200.0])
+@pytest.mark.parametrize("rows", [1, 5])
+def test_channels_of_very_different_size(hq, hkv, hd, fmt, factor, rows):
+    """One channel of q `factor` times the others; another one of K as much larger, q as much smaller there, so that it counts as any
+    other.  A score has to come from all digits of q: the bound takes its error as 2^-17 of sum |q k|, no part of the largest channel."""
+    n = 700
+    g = torch.Generator().manual_seed(int(factor) + hd)
+    k = torch.randn(n, hkv, hd, generator=g)
+    v = torch.randn(n, hkv, hd, generator=g)
+    q = torch.randn(rows, hq, hd, generator=g)
+    k[..., 9] *= factor
+    q[..., 9] /= factor
+    q[..., 40] *= factor
+    k[..., 40] *= 0.02                                        # codes of 0 to 3 where the large channel is: the others decide
+    c = Cache([n], hkv, hd, fmt, k=[k], v=[v])
+    pos, seq, g0, gc = _groups([n], [rows])
+    q = bf(q.reshape(rows, hq * hd))
+    out = _attend(c, q, hq, pos, seq, g0, gc)
+    _check_attend(c, q, hq, out, pos, seq, g0, gc)

@@ -322,9 +322,9 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_attn_kernel(
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
         const uint32_t e = min(264u - (top >> 23), 253u);
-        const float up = __uint_as_float(e << 23);
+        // an infinity or a NaN in q: every score is NaN; those of keys that are not seen become -infinity like any other
+        const float up = top >= 0x7f800000u ? __uint_as_float(0x7fffffffu) : __uint_as_float(e << 23);
         qs[n] = __fmul_rn(__uint_as_float((254u - e) << 23), a.scale_log2);
-        if (top >= 0x7f800000u) qs[n] = __uint_as_float(0x7fffffffu);           // an infinity or a NaN in q: a column of NaN
 #pragma unroll
         for (int c = 0; c < KC; ++c)
 #pragma unroll

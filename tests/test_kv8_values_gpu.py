@@ -29,3 +29,27 @@ def test_channels_of_very_different_size(hq, hkv, hd, fmt, factor, rows):
     q = bf(q.reshape(rows, hq * hd))
     out = _attend(c, q, hq, pos, seq, g0, gc)
     _check_attend(c, q, hq, out, pos, seq, g0, gc)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+def test_rows_that_see_nothing_are_zeros_whatever_their_q_holds(fmt, bad):
+    """Padded rows (position -1) and rows with an empty mask, of one split and of two, with q that is no number: zeros, and their
+    neighbours do not notice."""
+    hq, hkv, hd = 8, 2, 64
+    lens, new = [24, 40, 9], [24, 1, 9]
+    c = Cache(lens, hkv, hd, fmt, seed=3)
+    pos, seq, g0, gc = _groups(lens, new)
+    pos[24] = -1
+    mask = [(1 << r + 1) - 1 for cnt in new for r in range(cnt)]
+    empty = [0, 7, 20, 23, 24, 25, 33]                        # 20 and 23 lie in the second split of sixteen keys
+    for t in empty:
+        mask[t] = 0
+    q = bf(torch.randn(len(pos), hq * hd))
+    out = _attend(c, q, hq, pos, seq, g0, gc, mask, split_keys=16)
+    assert bool((out[empty] == 0).all())
+    q[empty] = bad
+    again = _attend(c, q, hq, pos, seq, g0, gc, mask, split_keys=16)
+    assert bool((again[empty] == 0).all())
+    assert torch.equal(again, out)
+    _check_attend(c, q, hq, out, pos, seq, g0, gc, mask)

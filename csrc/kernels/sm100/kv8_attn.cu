@@ -66,6 +66,9 @@ constexpr float kNoRef = -3.4028234e38f;    // m before the first key
 constexpr float kGrow = 16384.f;              // what a weight may reach before m follows
 
 __device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
+// The square root of 2^(m - to).  Sums of p are brought from m to another reference in two such steps: beside rows of V near the largest
+// numbers, m of rows of zeros lies more than 126 lower, and 2^(m - to) is no number, while their p (as much larger) still count.
+__device__ __forceinline__ float ex2_half(float m, float to) { return ex2(__fmul_rn(0.5f, __fadd_rn(m, -to))); }
 __device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
   const __half2 v = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
@@ -445,9 +448,10 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_attn_kernel(
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
           float f = 1.f;
-          if (top > kGrow) { f = ex2(__fadd_rn(m[n], -mx)); m[n] = mx; }
+          float half = 1.f;
+          if (top > kGrow) { half = ex2_half(m[n], mx); f = __fmul_rn(half, half); m[n] = mx; }
           if (i == 0) continue;                     // nothing has been added up
-          l[n] = __fmul_rn(l[n], f);
+          l[n] = __fmul_rn(__fmul_rn(l[n], half), half);
           const float f0 = __shfl_sync(0xffffffffu, f, 8 * t), f1 = __shfl_sync(0xffffffffu, f, 8 * t + 4);
 #pragma unroll
           for (int k = 0; k < MT; ++k) {
@@ -527,9 +531,9 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_attn_kernel(
       float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
-        const float f = ex2(__fadd_rn((&ms.x)[w], -M));
+        const float half = ex2_half((&ms.x)[w], M), f = __fmul_rn(half, half);
         const float4 y = *reinterpret_cast<const float4*>(smem + (&at.x)[w] + (c * LDO + d) * 4);
-        L = __fmaf_rn((&ls.x)[w], f, L);
+        L = __fmaf_rn(__fmul_rn((&ls.x)[w], half), half, L);
         x.x = __fmaf_rn(y.x, f, x.x); x.y = __fmaf_rn(y.y, f, x.y); x.z = __fmaf_rn(y.z, f, x.z); x.w = __fmaf_rn(y.w, f, x.w);
       }
       if (ns == 1) {
@@ -585,8 +589,8 @@ __global__ void __launch_bounds__(512) kv8_join_kernel(const Kv8AttnArgs a, int 
       Vec y[kJoin];
 #pragma unroll
       for (int j = 0; j < kJoin; ++j) y[j] = po[min(j, n - 1) * 32];        // past the end: the last part again, with the weight zero
-      const float m = warp_max(part.x), M2 = fmaxf(M, m), f = lane < n ? ex2(__fadd_rn(part.x, -m)) : 0.f;
-      float z[PER], l = warp_sum(__fmul_rn(part.y, f));
+      const float m = warp_max(part.x), M2 = fmaxf(M, m), half = lane < n ? ex2_half(part.x, m) : 0.f, f = __fmul_rn(half, half);
+      float z[PER], l = warp_sum(__fmul_rn(__fmul_rn(part.y, half), half));
 #pragma unroll
       for (int d = 0; d < PER; ++d) z[d] = 0.f;
 #pragma unroll
@@ -595,9 +599,9 @@ __global__ void __launch_bounds__(512) kv8_join_kernel(const Kv8AttnArgs a, int 
 #pragma unroll
         for (int d = 0; d < PER; ++d) z[d] = __fmaf_rn((&y[j].x)[d], fj, z[d]);
       }
-      const float old = ex2(__fadd_rn(M, -M2)), add = ex2(__fadd_rn(m, -M2));
+      const float old_half = ex2_half(M, M2), add_half = ex2_half(m, M2), old = __fmul_rn(old_half, old_half), add = __fmul_rn(add_half, add_half);
       M = M2;
-      L = __fmaf_rn(l, add, __fmul_rn(L, old));
+      L = __fmaf_rn(__fmul_rn(l, add_half), add_half, __fmul_rn(__fmul_rn(L, old_half), old_half));
 #pragma unroll
       for (int d = 0; d < PER; ++d) x[d] = __fmaf_rn(z[d], add, __fmul_rn(x[d], old));
     }
@@ -608,14 +612,14 @@ __global__ void __launch_bounds__(512) kv8_join_kernel(const Kv8AttnArgs a, int 
       __syncthreads();
       if (warp == 0)
         for (int v = 1; v < warps; ++v) M = fmaxf(M, sh_m[v]);
-      const float own = ex2(__fadd_rn(sh_m[0], -M));
+      const float own_half = ex2_half(sh_m[0], M), own = __fmul_rn(own_half, own_half);
       if (warp == 0) {
-        L = __fmul_rn(L, own);
+        L = __fmul_rn(__fmul_rn(L, own_half), own_half);
 #pragma unroll
         for (int d = 0; d < PER; ++d) x[d] = __fmul_rn(x[d], own);
         for (int v = 1; v < warps; ++v) {
-          const float f = ex2(__fadd_rn(sh_m[v], -M));
-          L = __fmaf_rn(sh_l[v], f, L);
+          const float half = ex2_half(sh_m[v], M), f = __fmul_rn(half, half);
+          L = __fmaf_rn(__fmul_rn(sh_l[v], half), half, L);
 #pragma unroll
           for (int d = 0; d < PER; ++d) x[d] = __fmaf_rn(sh_x[v][lane * PER + d], f, x[d]);
         }

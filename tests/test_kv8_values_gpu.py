@@ -53,3 +53,25 @@ def test_rows_that_see_nothing_are_zeros_whatever_their_q_holds(fmt, bad):
     assert bool((again[empty] == 0).all())
     assert torch.equal(again, out)
     _check_attend(c, q, hq, out, pos, seq, g0, gc, mask)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("big", [1.0, 1e15, 1e25])
+@pytest.mark.parametrize("split", [128, 768])
+def test_rows_of_zeros_beside_large_values_keep_their_weight(fmt, big, split):
+    """Some pages' V are zeros (the least scale there is), the others' are as large as `big`: what the zeros weigh stays in the sum,
+    whichever warp or split has them, and in whichever order they come."""
+    hq, hkv, hd = 8, 2, 64
+    n = 640
+    g = torch.Generator().manual_seed(8)
+    k = [torch.randn(n, hkv, hd, generator=g) for _ in range(3)]
+    v = [torch.randn(n, hkv, hd, generator=g) * big for _ in range(3)]
+    page = torch.arange(n) // 16
+    v[0][page % 4 == 1] = 0                                   # all of one warp's
+    v[1][(page >= 8) & (page < 24)] = 0                       # whole splits
+    v[2][page < 20] = 0                                       # zeros first, then large ones
+    c = Cache([n] * 3, hkv, hd, fmt, k=k, v=v)
+    pos, seq, g0, gc = _groups([n] * 3, [1, 4, 1])
+    q = bf(torch.randn(len(pos), hq * hd))
+    out = _attend(c, q, hq, pos, seq, g0, gc, split_keys=split)
+    _check_attend(c, q, hq, out, pos, seq, g0, gc)

@@ -723,10 +723,16 @@ class DenseModel:
         K8.rope_kvstore8(qkv, cfg.n_heads, cfg.n_kv_heads, cfg.head_dim, self.inv_freq, pos, seqv, self.block_table, self.kv[li], self.kv8, q,
                          status=self.status, **kw)
         if T < A.PREFILL_TC_MIN_TOKENS:
-            g0, gc, _, _ = A.prefill_groups(T, pos0, seq, self.dev)
-            part = self.part8 if T <= self.max_rows else None
-            return K8.attn_decode8(q, self.kv[li], self.kv8, self.block_table, g0, gc, pos, seqv, cfg.n_heads, cfg.n_kv_heads, cfg.head_dim,
-                                   split_keys=self.split8, part=part, status=self.status)
+            # as many rows at a time as the steps' workspace holds for the splits that there are (a row's bits do not depend on it)
+            ctx, a = pos0 + T, torch.empty_like(q)
+            need = K8.part_floats(8, cfg.n_heads, cfg.head_dim, ctx, self.split8)
+            step = T if need == 0 else min(T, self.part8.numel() // need * 8)
+            for r in range(0, T, step):
+                n = min(step, T - r)
+                g0, gc, _, _ = A.prefill_groups(n, pos0 + r, seq, self.dev)
+                K8.attn_decode8(q[r:r + n], self.kv[li], self.kv8, self.block_table, g0, gc, pos[r:], seqv[r:], cfg.n_heads, cfg.n_kv_heads,
+                                cfg.head_dim, split_keys=self.split8, max_ctx=ctx, part=self.part8, status=self.status, out=a[r:r + n])
+            return a
         used = (pos0 + T + cfg.page_size - 1) // cfg.page_size
         K8.kv_read8(self.kv[li], self.kv8, self.block_table[seq, :used], n_tokens=pos0 + T, out=self._stage[:used], status=self.status)
         return A.attn_prefill(q, self._stage, self._stage_table, 0, pos0, cfg.n_heads, cfg.n_kv_heads, cfg.head_dim, status=self.status,

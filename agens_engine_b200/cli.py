@@ -107,6 +107,7 @@ def build_model(cfg: EngineConfig, **kw):
     With ``--budget-gib`` the load is planned first (``serve/budget.py``): the KV pool gets the pages the plan grants,
     the context is clamped to what the pool plus the host tier can hold, the host tier is switched on when the plan
     says so, every rank takes the minimum, the process's allocator is capped at the budget, and the plan is printed.
+    ``together``: sequences that decode together, where ``max_seqs`` counts slots of parked ones too.
     Reference: crates/agens-cli/src/m1.rs:905-974, plan.rs:182-241, tp.rs:77-90."""
     import torch
     rank, world = int(os.environ.get("RANK", "0")), int(os.environ.get("WORLD_SIZE", "1"))
@@ -115,6 +116,7 @@ def build_model(cfg: EngineConfig, **kw):
     kw.setdefault("prefill_chunk", cfg.prefill_chunk)
     kw.setdefault("split_keys", cfg.split_keys)
     kw.setdefault("kv_cache", cfg.kv_cache)
+    together = kw.pop("together", kw["max_seqs"])
     # long contexts: at most 1024 attention splits per (row, head), so that the split partials stay near 1 GB at 256K
     want = (kw["max_ctx"] + 1023) // 1024
     while kw["split_keys"] < want:
@@ -129,13 +131,16 @@ def build_model(cfg: EngineConfig, **kw):
         dist.init_process_group("nccl", device_id=torch.device(dev))
         ctrl = D.control_group()
     dep = ledger = None
+    if cfg.kv_cache != "bf16":
+        from .serve import budget as B
+        kw["kv_split"] = B.kv_cache_plan(_model_config(cfg), kw["max_ctx"], together, world)["split_keys"]
     if cfg.budget_gib > 0:
         from .serve import budget as B
         mc = _model_config(cfg)
         free, _total = torch.cuda.mem_get_info(local)
         dep = B.plan_deployment(mc, cfg.budget_gib, kw["max_ctx"], cfg.max_batch, kw["max_seqs"], kw["prefill_chunk"], tp=world,
                                 gpu_free_gib=free / B.GiB, dual_layout=os.environ.get("B200E_STEP", "auto") != "0",
-                                split_keys=kw["split_keys"])
+                                split_keys=kw["split_keys"], together=together)
         if world > 1:
             import torch.distributed as dist
 
@@ -516,7 +521,7 @@ def cmd_serve(ns):
     if cfg.mode == "personal":
         cfg.max_batch = 1
     # slots beyond the running batch hold finished conversations and prompt-prefix snapshots
-    m, rank, world, ctrl = build_model(cfg, max_seqs=max(cfg.max_batch, 1) + max(0, min(cfg.max_convs, 64)))
+    m, rank, world, ctrl = build_model(cfg, max_seqs=max(cfg.max_batch, 1) + max(0, min(cfg.max_convs, 64)), together=max(cfg.max_batch, 1))
     if rank == 0:
         print("config: " + json.dumps(dataclasses.asdict(cfg)), flush=True)
     if world > 1 and rank > 0:

@@ -33,17 +33,22 @@ M_ROWS = 128         # most token rows of one step (64 decode rows or 128 verify
 class DenseModel:
     def __init__(self, cfg: ModelConfig, device="cuda:0", max_seqs: int = 1, max_ctx: int = 4096,
                  n_pages: Optional[int] = None, split_keys: int = 64, prefill_chunk: int = 256,
-                 lm_rows: Optional[int] = None, kv_cache: Optional[str] = None):
+                 lm_rows: Optional[int] = None, kv_cache: Optional[str] = None, kv_split: Optional[int] = None):
         """``kv_cache``: "bf16" (default: what the config says), or "int8" / "fp8": 8-bit pages (``ops/kv8.py``), half the bytes.  A
-        model with 8-bit pages runs its steps on the per-op kernels and does not tier its KV to the host."""
+        model with 8-bit pages runs its steps on the per-op kernels and does not tier its KV to the host.  ``kv_split``: keys of one
+        attention split over 8-bit pages, which a row's bits depend on.  Default: ``kv8.split_keys_for`` with every slot decoding; where
+        slots also hold parked sequences, its value for those that decode together gives short contexts more CTAs."""
         if kv_cache is not None and kv_cache != cfg.kv_cache:
             cfg = dataclasses.replace(cfg, kv_cache=kv_cache)
         if cfg.kv_cache not in ("bf16", *K8.FORMATS):
             raise ValueError(f"kv_cache: bf16, {' or '.join(K8.FORMATS)}, got {cfg.kv_cache!r}")
         if cfg.kv_cache != "bf16" and (cfg.page_size != K8.PAGE or cfg.head_dim not in (64, 128)):
             raise ValueError(f"an 8-bit KV cache has pages of {K8.PAGE} tokens and heads of 64 or 128")
+        if kv_split is not None and (cfg.kv_cache == "bf16" or not K8.PAGE <= kv_split <= K8.MAX_SPLIT or kv_split % K8.PAGE):
+            raise ValueError(f"kv_split: a multiple of {K8.PAGE} up to {K8.MAX_SPLIT}, of an 8-bit KV cache")
         self.cfg, self.dev = cfg, torch.device(device)
         self.kv8 = cfg.kv_cache if cfg.kv_cache != "bf16" else None
+        self.split8 = (kv_split or K8.split_keys_for(max_ctx, max_seqs * cfg.n_kv_heads)) if self.kv8 else None
         self.lm_rows = lm_rows or cfg.vocab          # rows of the (possibly vocab-sharded, padded) lm_head
         self.max_seqs, self.max_ctx, self.split_keys = max_seqs, max_ctx, split_keys
         self.prefill_chunk = prefill_chunk
@@ -136,7 +141,6 @@ class DenseModel:
         M = self.max_rows = min(M_ROWS, max(M_GEMV, 8 * self.max_seqs))
         if self.kv8:
             self.kv = [K8.make_pool(self.n_pages, cfg.n_kv_heads, cfg.head_dim, dev) for _ in range(cfg.n_layers)]
-            self.split8 = K8.split_keys_for(self.max_ctx, self.max_seqs * cfg.n_kv_heads)
             # bf16 copy of one sequence's pages of one layer: what the prefill attention of a long chunk reads
             self._stage = torch.empty(self.pages_per_seq, 2, cfg.n_kv_heads, cfg.page_size, cfg.head_dim, dtype=torch.bfloat16, device=dev)
             self._stage_table = torch.arange(self.pages_per_seq, dtype=torch.int32, device=dev).view(1, -1)

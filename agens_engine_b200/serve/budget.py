@@ -81,6 +81,7 @@ class Deployment:
     host_tier: bool
     resident_window_tokens: int
     host_pages: int
+    split_keys: int            # keys per attention split that the plan counts partial results for
     fits: bool
     lines: List[str]
     plan: dict
@@ -88,7 +89,8 @@ class Deployment:
 
 def kv_cache_plan(cfg, wctx: int, max_batch: int, tp: int = 1, split_keys: int = 64) -> dict:
     """What the KV cache's format means for a plan: bytes beside the pool, keys per attention split, whether pages may be tiered.  With
-    8-bit pages (``cfg.kv_cache``) one sequence's pages of one layer are held in bf16 for prefill and pages stay on the GPU."""
+    8-bit pages (``cfg.kv_cache``) one sequence's pages of one layer are held in bf16 for prefill, pages stay on the GPU, and the split
+    size is that of ``max_batch`` sequences decoding together: the model is built with it (``DenseModel(kv_split=)``)."""
     if cfg.kv_cache == "bf16":
         return {"extra_bytes": 0, "split_keys": split_keys, "host_tier": True}
     from ..ops.kv8 import split_keys_for
@@ -97,13 +99,14 @@ def kv_cache_plan(cfg, wctx: int, max_batch: int, tp: int = 1, split_keys: int =
 
 def plan_deployment(cfg, budget_gib: float, wctx: int, max_batch: int, sessions: int, prefill_chunk: int, tp: int = 1,
                     gpu_free_gib: Optional[float] = None, host_avail_gib: float = -1.0, allow_host_tier: bool = True,
-                    weights_bytes: Optional[int] = None, dual_layout: bool = False, split_keys: int = 64) -> Deployment:
+                    weights_bytes: Optional[int] = None, dual_layout: bool = False, split_keys: int = 64,
+                    together: Optional[int] = None) -> Deployment:
     """Runs the planner for one rank of a ``tp``-way deployment of the architecture ``cfg`` (the full model's config).
     ``weights_bytes``: measured bytes when the weights are already on the device, else the architecture's estimate
     plus 0.6 GiB of CUDA context; ``dual_layout`` doubles the quantised linears (the step kernel's second layout, which a model
-    with an 8-bit KV cache does not have)."""
+    with an 8-bit KV cache does not have); ``together``: sequences that decode together (default: ``max_batch``)."""
     from . import host as H
-    kv = kv_cache_plan(cfg, wctx, max_batch, tp, split_keys)
+    kv = kv_cache_plan(cfg, wctx, together or max_batch, tp, split_keys)
     if weights_bytes is None:
         lin = cfg.weight_bytes(tp) - cfg.vocab * cfg.d_model * 2
         weights_bytes = cfg.weight_bytes(tp) + (lin if dual_layout and cfg.kv_cache == "bf16" else 0) + int(0.6 * GiB)
@@ -123,7 +126,7 @@ def plan_deployment(cfg, budget_gib: float, wctx: int, max_batch: int, sessions:
     host = p["tier"] == "host"
     window = int(p["resident_window_pages"]) * ps
     return Deployment(budget_bytes=int(p["budget_bytes"]), n_pages=n_pages, max_ctx=max_ctx, host_tier=host,
-                      resident_window_tokens=window, host_pages=int(p["host_pages"]), fits=bool(p["fits"]), lines=list(p["lines"]),
+                      resident_window_tokens=window, host_pages=int(p["host_pages"]), split_keys=int(kv["split_keys"]), fits=bool(p["fits"]), lines=list(p["lines"]),
                       plan=p)
 
 

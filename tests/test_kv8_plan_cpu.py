@@ -1,0 +1,69 @@
+"""What a deployment plans for an 8-bit key-value cache and what its model is built with, without a GPU."""
+import dataclasses
+
+import pytest
+import torch
+
+from agens_engine_b200 import cli
+from agens_engine_b200.models import config as C
+from agens_engine_b200.models.dense import DenseModel
+from agens_engine_b200.ops import kv8 as K
+from agens_engine_b200.serve import budget as B
+
+
+class Built(Exception):
+    pass
+
+
+def _serve(monkeypatch, argv):
+    """Runs `serve` up to the model's construction: its arguments, and the deployment that was planned (None without a budget)."""
+    got, plan = {}, []
+
+    def init(mc, dev, seed, **kw):
+        got.update(kw)
+        raise Built
+    real = B.plan_deployment
+    monkeypatch.setattr(DenseModel, "random_init", staticmethod(init))
+    monkeypatch.setattr(torch.cuda, "mem_get_info", lambda d=None: (170 << 30, 180 << 30))
+    monkeypatch.setattr(B, "cap_process", lambda *a: None)
+    monkeypatch.setattr(B, "plan_deployment", lambda *a, **kw: plan.append(real(*a, **kw)) or plan[-1])
+    with pytest.raises(Built):
+        cli.main(["serve", "--random", "dense-32b", *argv])
+    return got, plan[0] if plan else None
+
+
+@pytest.mark.parametrize("wctx", [4096, 8192, 40000, 131072])
+@pytest.mark.parametrize("mode,batch", [("personal", 1), ("server", 8), ("server", 1)])
+def test_the_servers_split_is_the_planned_one(monkeypatch, mode, batch, wctx):
+    """Sequences that decode together count, not the slots that hold parked ones."""
+    argv = ["--kv-cache", "int8", "--mode", mode, "--wctx", str(wctx), "--max-batch", str(batch)]
+    got, _ = _serve(monkeypatch, argv)
+    assert got["max_seqs"] > batch and got["kv_split"] == K.split_keys_for(wctx, 8 * batch)
+    budgeted, dep = _serve(monkeypatch, argv + ["--budget-gib", "100"])
+    assert budgeted["kv_split"] == dep.split_keys == got["kv_split"]
+
+
+def test_short_contexts_of_one_conversation_get_short_splits(monkeypatch):
+    got = [_serve(monkeypatch, ["--kv-cache", "fp8", "--mode", "personal", "--wctx", str(n)])[0]["kv_split"] for n in (4096, 8192, 20000, 65536)]
+    assert got == [128, 256, 512, 768]
+
+
+def test_bf16_models_are_built_as_before(monkeypatch):
+    got, _ = _serve(monkeypatch, ["--mode", "personal", "--wctx", "8192"])
+    assert got == dict(max_seqs=65, max_ctx=8192, prefill_chunk=256, split_keys=64, kv_cache="bf16")
+
+
+def test_a_plan_names_its_split():
+    k8 = dataclasses.replace(C.dense_32b(seed=0), kv_cache="int8")
+    plan = lambda batch, slots, tp=1, **kw: B.plan_deployment(k8, 100, 8192, batch, slots, 2048, tp=tp, gpu_free_gib=170, host_avail_gib=64, **kw).split_keys
+    assert plan(1, 65) == plan(1, 1) == plan(8, 72, together=1) == 256 and plan(8, 72) == 768 and plan(8, 72, tp=8) == 256
+    assert B.plan_deployment(C.dense_32b(seed=0), 100, 8192, 1, 1, 2048, gpu_free_gib=170, host_avail_gib=64, split_keys=64).split_keys == 64
+
+
+def test_a_model_takes_its_split_and_refuses_others():
+    cfg = C.oracle_tiny()
+    for bad in (0, 24, 4096, -16):
+        with pytest.raises(ValueError, match="kv_split"):
+            DenseModel(cfg, "cpu", kv_cache="int8", kv_split=bad)
+    with pytest.raises(ValueError, match="kv_split"):
+        DenseModel(cfg, "cpu", kv_split=128)

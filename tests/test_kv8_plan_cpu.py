@@ -67,3 +67,26 @@ def test_a_model_takes_its_split_and_refuses_others():
             DenseModel(cfg, "cpu", kv_cache="int8", kv_split=bad)
     with pytest.raises(ValueError, match="kv_split"):
         DenseModel(cfg, "cpu", kv_split=128)
+
+
+@pytest.mark.parametrize("wctx", [100, 8192, 131072])
+@pytest.mark.parametrize("batch,slots,rows", [(1, 65, 128), (8, 72, 128), (1, 1, 32), (2, 6, 48), (20, 20, 128)])
+def test_a_plan_counts_the_workspace_that_the_model_has(wctx, batch, slots, rows):
+    """The model's step workspace holds eight rows a slot, parked ones included; the planner counts eight a sequence of the batch."""
+    k8 = dataclasses.replace(C.dense_32b(seed=0), kv_cache="int8")
+    plan = lambda n, c=k8: B.plan_deployment(c, 100, wctx, batch, n, 2048, gpu_free_gib=170, host_avail_gib=64)
+    dep, least = plan(slots), plan(batch)
+    beyond = dep.plan["fixed_bytes"] - least.plan["fixed_bytes"]
+    floats = K.part_floats(rows, 64, 128, wctx, dep.split_keys)
+    assert beyond + dep.plan["scratch"]["attention_partials"] >= 4 * floats
+    assert beyond == 4 * K.part_floats(rows - min(128, max(32, 8 * batch)), 64, 128, wctx, dep.split_keys)
+    assert plan(slots, C.dense_32b(seed=0)).plan["fixed_bytes"] == plan(batch, C.dense_32b(seed=0)).plan["fixed_bytes"]
+
+
+def test_the_plan_command_counts_the_servers_slots(capsys):
+    def pages(convs):
+        assert cli.main(["plan", "--random", "dense-32b", "--budget-gib", "64", "--wctx", "131072", "--max-batch", "1", "--max-convs", str(convs),
+                         "--kv-cache", "int8", "--host-avail-gib", "8"]) == 0
+        return int([line for line in capsys.readouterr().out.splitlines() if "KV pool" in line][0].split("KV pool ")[1].split()[0])
+    page = 64 * 8 * (32 * 128 + 128)
+    assert abs((pages(0) - pages(64)) - 4 * K.part_floats(96, 64, 128, 131072, 768) / page) <= 1

@@ -22,7 +22,8 @@ from .dense import DenseModel, M_GEMV
 
 class MtpHead(DenseModel):
     """One-layer model with its own paged KV; ``embed``, ``final_norm`` weights for the head and ``lm_head`` are the
-    target's tensors (shared, not copied).  Beside a tensor-parallel target the head runs unsharded on the leader's GPU
+    target's tensors (shared, not copied).  Its KV pages have the target's format and split size (``kv_cache`` and ``kv_split`` say
+    otherwise), beside a tensor-parallel target too.  Beside a tensor-parallel target the head runs unsharded on the leader's GPU
     (the target's hidden rows are replicated on every rank); the target's lm_head is a vocabulary shard there, so the
     head carries its own full one (``own_lm_head``; reference: the MTP head under TP, kernels/m1/m1_mtp.cu:503-524)."""
 
@@ -33,6 +34,9 @@ class MtpHead(DenseModel):
         kw.setdefault("max_seqs", target.max_seqs)
         kw.setdefault("max_ctx", target.max_ctx)
         kw.setdefault("split_keys", target.split_keys)
+        kw.setdefault("kv_cache", target.cfg.kv_cache)
+        if kw["kv_cache"] != "bf16" and target.split8:
+            kw.setdefault("kv_split", target.split8)
         lm_rows = (cfg.vocab + 31) // 32 * 32 if self.own_lm_head else target.lm_rows
         super().__init__(cfg, target.dev, lm_rows=lm_rows, **kw)
         self.embed = target.embed

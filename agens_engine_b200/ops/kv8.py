@@ -38,7 +38,7 @@ def make_pool(n_pages: int, hkv: int, hd: int, device) -> torch.Tensor:
     return torch.zeros(n_pages, hkv, block_bytes(hd), dtype=torch.uint8, device=device)
 
 
-@functools.lru_cache(maxsize=None)
+@functools.lru_cache(maxsize=256)
 def split_keys_for(max_ctx: int, heads: int = 8) -> int:
     """Keys of one attention split for ``heads`` pairs of a sequence and a KV head with contexts of up to ``max_ctx`` tokens: the least of
     128, 256, 512 that makes no more splits than CTAs run at once, else 768, and more where a context had over 256 of them.  A

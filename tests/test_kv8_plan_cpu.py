@@ -90,3 +90,10 @@ def test_the_plan_command_counts_the_servers_slots(capsys):
         return int([line for line in capsys.readouterr().out.splitlines() if "KV pool" in line][0].split("KV pool ")[1].split()[0])
     page = 64 * 8 * (32 * 128 + 128)
     assert abs((pages(0) - pages(64)) - 4 * K.part_floats(96, 64, 128, 131072, 768) / page) <= 1
+
+
+def test_split_sizes_of_many_contexts_are_not_kept():
+    """A caller whose context grows by one a step looks up another one every step."""
+    for n in range(1, 3000):
+        K.split_keys_for(n, 3)
+    assert K.split_keys_for.cache_info().currsize <= 256

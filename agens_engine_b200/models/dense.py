@@ -370,10 +370,12 @@ class DenseModel:
         torch.cuda.current_stream(self.dev).synchronize()
         delta = self.rope_delta.get(seq, 0)
         self.free_seq(seq)
-        return {"len": n, "kv": host_kv, "rope_delta": delta}
+        return {"len": n, "kv": host_kv, "rope_delta": delta, "kv_cache": self.cfg.kv_cache}
 
     def unpark(self, seq: int, blob: Dict[str, object]):
-        """Restores a parked sequence into the (free) slot ``seq``."""
+        """Restores a parked sequence into the (free) slot ``seq`` of a model with the same KV format."""
+        if blob.get("kv_cache", self.cfg.kv_cache) != self.cfg.kv_cache:         # int8 and fp8 pages have the same shape
+            raise ValueError(f"the sequence was parked with KV cache {blob['kv_cache']}, this model has {self.cfg.kv_cache}")
         self.new_seq(seq)
         n = int(blob["len"])
         if blob.get("rope_delta"):

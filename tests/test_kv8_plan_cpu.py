@@ -97,3 +97,14 @@ def test_split_sizes_of_many_contexts_are_not_kept():
     for n in range(1, 3000):
         K.split_keys_for(n, 3)
     assert K.split_keys_for.cache_info().currsize <= 256
+
+
+def test_a_parked_sequence_goes_back_to_its_own_format_only():
+    """int8 and fp8 pages have the same shape: the format goes with a parked sequence, and nothing is touched before it is looked at."""
+    import types
+    touched = []
+    m = types.SimpleNamespace(cfg=dataclasses.replace(C.oracle_tiny(), kv_cache="int8"), new_seq=touched.append)
+    for other in ("fp8", "bf16"):
+        with pytest.raises(ValueError, match="parked"):
+            DenseModel.unpark(m, 0, {"len": 3, "kv": torch.zeros(2, 1, 2, 2176, dtype=torch.uint8), "rope_delta": 0, "kv_cache": other})
+    assert touched == []

@@ -75,3 +75,19 @@ def test_rows_of_zeros_beside_large_values_keep_their_weight(fmt, big, split):
     q = bf(torch.randn(len(pos), hq * hd))
     out = _attend(c, q, hq, pos, seq, g0, gc, split_keys=split)
     _check_attend(c, q, hq, out, pos, seq, g0, gc)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("power", [98, 40, -50])
+def test_scores_of_large_times_small(fmt, power):
+    """K of 2^98 against q of 2^-98 and the other way round: the scores are ordinary numbers, and nothing on the way to them is not."""
+    hq, hkv, hd = 8, 2, 128
+    g = torch.Generator().manual_seed(abs(power))
+    n = 300
+    k = torch.randn(n, hkv, hd, generator=g) * 2.0 ** power
+    v = torch.randn(n, hkv, hd, generator=g)
+    c = Cache([n], hkv, hd, fmt, k=[k], v=[v])
+    pos, seq, g0, gc = _groups([n], [3])
+    q = bf(torch.randn(3, hq * hd, generator=g) * 2.0 ** -power)
+    out = _attend(c, q, hq, pos, seq, g0, gc)
+    _check_attend(c, q, hq, out, pos, seq, g0, gc)

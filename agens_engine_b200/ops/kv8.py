@@ -44,9 +44,9 @@ def split_keys_for(max_ctx: int, heads: int = 8) -> int:
     128, 256, 512 that makes no more splits than CTAs run at once, else 768, and more where a context had over 256 of them.  A
     constant of the engine, since a row's bits depend on it.
 
-    Small splits spread a short context over the GPU (700 tokens, 8 KV heads: 7.2 us with 128, 9.1 with 512), large ones cost less
-    between their keys: 24 sequences of 2000 to 4001 34.7 us with 768, 35.9 with 512, 39.8 with 1024; 131072 tokens 54.0, 55.7, 54.9;
-    verify blocks of 4 x 6 rows at 5626 to 9001 47.6, 49.1, 46.9."""
+    Small splits spread a short context over the GPU (700 tokens, 8 KV heads: 7.3 us with 128, 8.3 with 256, 9.9 with 512), large ones cost
+    less between their keys: 24 sequences of 2000 to 4001 34.7 us with 768, 36.1 with 512, 40.0 with 1024; 131072 tokens 57.1, 57.9, 58.2;
+    verify blocks of 4 x 6 rows at 5626 to 9001 51.0, 51.0, 49.2."""
     s = next((s for s in (128, 256, 512) if heads * -(-max_ctx // s) <= 444), 768)
     return next((t for t in (128, 256, 512, 768, 1024) if t >= s and t * 256 >= max_ctx), MAX_SPLIT)
 
@@ -149,7 +149,8 @@ def rope_kvstore8(qkv: torch.Tensor, hq: int, hkv: int, hd: int, inv_freq: torch
     """Rotates q and k of the fused rows ``qkv`` (bf16 ``[n, (hq + 2 * hkv) * hd]``), writes q to ``q_out`` (bf16 ``[n, hq * hd]``) and
     quantises k and v into slot ``tok_pos[i]`` of sequence ``tok_seq[i]``.  The 8-bit form of ``basic.rope_kvstore`` and, with
     ``rope_pos3`` (int32 ``[3, n]``) and ``pair_axis`` (uint8 ``[hd / 2]``), of ``basic.rope_kvstore_m``; angles are taken in
-    64 bits.  Two rows of a call must not name the same slot.  Returns the status word."""
+    64 bits.  Two rows of a call must not name the same slot, and ``q_out`` does not overlap ``qkv``.  A row without a slot (position -1, a
+    page that is not there) is not stored and reported; its q is written.  Returns the status word."""
     f, dev = _format(fmt), qkv.get_device()
     n = qkv.shape[0]
     if hq < 1 or hkv < 1:
@@ -189,7 +190,7 @@ def attn_decode8(q: torch.Tensor, pool: torch.Tensor, fmt: str, block_table: tor
     sequence in ascending order of ``tok_pos``, whose K and V are in the pool already; row i sees the slots up to ``tok_pos[i]``, of
     the slots from the group's first on those whose bit its ``tree_mask`` (int32 ``[n_tok]``) has.  A row that sees nothing
     (``tok_pos`` -1 in a group of its own, an empty mask) gives zeros; rows of no group are left as they were in ``out``, which does
-    not overlap ``q``.
+    not overlap ``q``.  K's rows may be as large as 2^100: scores are formed in fp32.
 
     ``split_keys`` (a multiple of 16, at most 2048; default :func:`split_keys_for` the table's size) cuts every sequence into
     splits that are joined at the end; a row's bits depend on its own position and on ``split_keys`` only.  ``max_ctx`` (default:

@@ -23,16 +23,16 @@
 //
 // Range.  The weights reach the second product as fp16 numbers p_j vs_j: what is rounded is each key's contribution relative to the
 // largest one, whatever the size of V, and a key that has weight but no V (a row of zeros has the least scale) cannot push the
-// others out of fp16's range.  m begins as the largest contribution of a warp's first pair of pages and is raised only when a weight
+// others out of fp16's range.  Scores are formed in fp32 from up to 2^27 times ks: K's rows may be as large as 2^100.  m begins as the largest contribution of a warp's first pair of pages and is raised only when a weight
 // passes kGrow = 2^14, a quarter of fp16's range, which leaves the accumulators alone for nearly all pages.
 //
 // What bounds it, and what it measured (B200, 64 q and 8 KV heads of 128, join included).  Decode: the copies.  One sequence of 131072
-// keys 54 us (277 MB: 5.1 TB/s; the same loop with its copies alone 48 us), 24 sequences of 2000 to 4001 in fp8 34.7 us (155 MB, 4.5 TB/s;
-// 30 us), one of 700 7.2 us: launch, one page's latency, join.  Verify blocks (4 sequences of 5626 to 9001, 6 rows each, int8): 47.6 us for
-// 63 MB, the chain of products, weights and conversions of two warps a scheduler (0.40 instructions a cycle; 620 of them a pair of pages
-// and 700 an item of six pairs, three or four items a CTA); sixteen columns an item: twenty-four were 7 % slower and eight convert all of K and V twice as often.
+// keys 57 us in int8, 55.5 in fp8 (277 MB: 4.9 and 5.0 TB/s; the same loop with its copies alone 48 us), 24 sequences of 2000 to 4001 in fp8 34.7 us
+// (155 MB, 4.5 TB/s; 30 us), one of 700 7.3 us: launch, one page's latency, join.  Verify blocks (4 sequences of 5626 to 9001, 6 rows each, int8): 51 us
+// for 63 MB, the chain of products, weights and conversions of two warps a scheduler (0.42 instructions a cycle; 680 of them a pair of pages and 700 an
+// item of six pairs, three or four items a CTA); sixteen columns an item: twenty-four were 7 % slower and eight convert all of K and V twice as often.
 // Tried and slower: codes in registers instead of shared memory (24 sequences 53 us), pages converted once for 64 columns by all warps
-// together (verify 66 us when this took 54, a barrier every pair of pages), bulk copies of four rows (41 and 63 us: they arrive later), tcgen05
+// together (verify 66 us when this took 54; a barrier every pair of pages), bulk copies of four rows (41 and 63 us: they arrive later), tcgen05
 // products with V converted into shared memory (54 and 56 us, 77 for 131072 keys: with eight columns the products are all issue and latency,
 // and rows of verify blocks must not differ from decode), joining in the last CTA of a row (45 us).
 #include <algorithm>
@@ -559,8 +559,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_attn_kernel(
 // at once and added in order.  `warps` of them share a (row, q head); block b is warp b % 16's, the warps' sums are added in order.
 // With warps == 1 (rows of at most sixteen splits) a CTA has four (row, q head)s.  Neither choice changes a row's bits:
 //     o = sum_s o_s 2^(m_s - M) / sum_s l_s 2^(m_s - M),    M = max_s m_s
-// Bound by latency: a warp's loads, the exchange and the launch.  256 splits of 64 heads add 4 us to the kernel before (attention over
-// 131072 keys in all: 57 us, 59 with a head's parts loaded one after the other; over 700 keys 7.9 and 9.3).
+// Bound by latency: a warp's loads, the exchange and the launch.  171 splits of 64 heads (131072 keys) add 3 to 6 us to the kernel before,
+// two to six splits 1.6 to 2.5; with a head's parts loaded one after the other it was 2 us more at 256 splits.
 template <int HD>
 __global__ void __launch_bounds__(512) kv8_join_kernel(const Kv8AttnArgs a, int rows_at_once, int warps) {
   constexpr int PER = HD / 32;

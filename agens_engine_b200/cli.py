@@ -237,7 +237,7 @@ def cmd_plan(ns):
     from .serve import budget as B
     mc = _model_config(cfg)
     slots = max(cfg.max_batch, 1) + max(0, min(cfg.max_convs, 64))                   # what `serve` builds
-    kv = B.kv_cache_plan(mc, cfg.wctx, cfg.max_batch, cfg.tp, cfg.split_keys, more_rows=B.step_rows(slots) - B.step_rows(cfg.max_batch))
+    kv = B.kv_cache_plan(mc, cfg.wctx, cfg.max_batch, cfg.tp, cfg.split_keys, slots=slots)
     kw = {} if mc.kv_cache == "bf16" else dict(allow_host_tier=kv["host_tier"], split_keys=kv["split_keys"])
     rep = H.plan(budget_gib=cfg.budget_gib, gpu_free_gib=ns.gpu_free_gib, weights_bytes=mc.weight_bytes(cfg.tp) + kv["extra_bytes"],
                  kv_bytes_per_token=mc.kv_bytes_per_token(cfg.tp), page_size=mc.page_size, max_batch=cfg.max_batch,

@@ -87,20 +87,18 @@ class Deployment:
     plan: dict
 
 
-def step_rows(seqs: int) -> int:
-    """Rows of the largest step of a model with ``seqs`` slots (``DenseModel.max_rows``)."""
-    from ..models.dense import M_GEMV, M_ROWS
-    return min(M_ROWS, max(M_GEMV, 8 * seqs))
-
-
-def kv_cache_plan(cfg, wctx: int, max_batch: int, tp: int = 1, split_keys: int = 64, more_rows: int = 0) -> dict:
+def kv_cache_plan(cfg, wctx: int, max_batch: int, tp: int = 1, split_keys: int = 64, slots: int = 0, counted: int = 0) -> dict:
     """What the KV cache's format means for a plan: bytes beside the pool, keys per attention split, whether pages may be tiered.  With
     8-bit pages (``cfg.kv_cache``) one sequence's pages of one layer are held in bf16 for prefill, pages stay on the GPU, and the split
-    size is that of ``max_batch`` sequences decoding together: the model is built with it (``DenseModel(kv_split=)``).  ``more_rows``: rows
-    of its largest step beyond those whose partial results the planner counts itself."""
+    size is that of ``max_batch`` sequences decoding together: the model is built with it (``DenseModel(kv_split=)``).  ``slots``:
+    sequence slots of the model, whose largest step has eight rows for each; ``counted``: for how many the planner counts partial results
+    itself."""
     if cfg.kv_cache == "bf16":
         return {"extra_bytes": 0, "split_keys": split_keys, "host_tier": True}
+    from ..models.dense import M_GEMV, M_ROWS
     from ..ops.kv8 import part_floats, split_keys_for
+    rows = lambda seqs: min(M_ROWS, max(M_GEMV, 8 * seqs))               # DenseModel.max_rows
+    more_rows = max(0, rows(slots) - rows(counted or max_batch))
     split = split_keys_for(wctx, max_batch * (cfg.n_kv_heads // tp))
     extra = wctx * (cfg.kv_dim // tp) * 4 + 4 * part_floats(more_rows, cfg.n_heads // tp, cfg.head_dim, wctx, split)
     return {"extra_bytes": extra, "split_keys": split, "host_tier": False}
@@ -115,7 +113,7 @@ def plan_deployment(cfg, budget_gib: float, wctx: int, max_batch: int, sessions:
     plus 0.6 GiB of CUDA context; ``sessions``: slots of the model; ``dual_layout`` doubles the quantised linears (the step kernel's second layout, which a model
     with an 8-bit KV cache does not have); ``together``: sequences that decode together (default: ``max_batch``)."""
     from . import host as H
-    kv = kv_cache_plan(cfg, wctx, together or max_batch, tp, split_keys, more_rows=max(0, step_rows(sessions) - step_rows(max_batch)))
+    kv = kv_cache_plan(cfg, wctx, together or max_batch, tp, split_keys, slots=sessions, counted=max_batch)
     if weights_bytes is None:
         lin = cfg.weight_bytes(tp) - cfg.vocab * cfg.d_model * 2
         weights_bytes = cfg.weight_bytes(tp) + (lin if dual_layout and cfg.kv_cache == "bf16" else 0) + int(0.6 * GiB)

@@ -190,7 +190,7 @@ def attn_decode8(q: torch.Tensor, pool: torch.Tensor, fmt: str, block_table: tor
     sequence in ascending order of ``tok_pos``, whose K and V are in the pool already; row i sees the slots up to ``tok_pos[i]``, of
     the slots from the group's first on those whose bit its ``tree_mask`` (int32 ``[n_tok]``) has.  A row that sees nothing
     (``tok_pos`` -1 in a group of its own, an empty mask) gives zeros; rows of no group are left as they were in ``out``, which does
-    not overlap ``q``.  K's rows may be as large as 2^100: scores are formed in fp32.
+    not overlap ``q``.  Rows of K and V may be as large as 2^100: scores and weights are fp32 numbers.
 
     ``split_keys`` (a multiple of 16, at most 2048; default :func:`split_keys_for` the table's size) cuts every sequence into
     splits that are joined at the end; a row's bits depend on its own position and on ``split_keys`` only.  ``max_ctx`` (default:

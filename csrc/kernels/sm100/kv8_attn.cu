@@ -13,28 +13,32 @@
 // finished there, the others leave (o, m, l) per split to kv8_join_kernel.  What a row adds up and in which order depends on its
 // own position alone, so a row has the same bits in a decode step, a verify block or any batch.
 //
-// Products.  The group's rows times the q heads of a KV head are the columns, eight to a tile, so that a single decode row with
-// eight q heads wastes nothing.  S = q K^T takes q as A (its rows are the columns, eight of sixteen where there are no more) and
-// K's bytes as fp16 as B; its result is, lane for lane, the B operand of O^T = V^T P^T, whose A are V's bytes as fp16.  The order of channels inside a product and of keys inside a page is free, and chosen so that every lane reads sixteen
-// bytes of a row at a time and nothing has to be moved between lanes or registers.
+// Products.  The group's rows times the q heads of a KV head are the columns, eight to a tile, so that a single decode row with eight
+// q heads wastes nothing.  S = q K^T takes q as A (its rows are the columns, eight of sixteen where there are no more) and K's bytes
+// as fp16 as B; its result is, lane for lane, the B operand of O^T = V^T P^T, whose A are V's bytes as fp16.  The order of channels
+// inside a product and of keys inside a page is free, and chosen so that every lane reads sixteen bytes of a row at a time and nothing
+// has to be moved between lanes or registers.
 //
 // Loads.  Every warp copies its own pages, two at a time, into one of two places in shared memory (cp.async, no barrier but the
 // warp's) and runs ahead into the CTA's next item, whose page numbers were fetched an item earlier.
 //
 // Range.  The weights reach the second product as fp16 numbers p_j vs_j: what is rounded is each key's contribution relative to the
-// largest one, whatever the size of V, and a key that has weight but no V (a row of zeros has the least scale) cannot push the
-// others out of fp16's range.  Scores are formed in fp32 from up to 2^27 times ks: K's rows may be as large as 2^100.  m begins as the largest contribution of a warp's first pair of pages and is raised only when a weight
-// passes kGrow = 2^14, a quarter of fp16's range, which leaves the accumulators alone for nearly all pages.
+// largest one, whatever the size of V, and a key that has weight but no V (a row of zeros has the least scale) cannot push the others
+// out of fp16's range.  Scores are formed in fp32 from up to 2^27 times ks, and weights of keys are lost below 2^-126 times the power
+// of two of V's scale: rows of K and V may be as large as 2^100.  m begins as the largest contribution of a warp's first pair of pages
+// and is raised only when a weight passes kGrow = 2^14, a quarter of fp16's range, which leaves the accumulators alone for nearly all
+// pages.
 //
 // What bounds it, and what it measured (B200, 64 q and 8 KV heads of 128, join included).  Decode: the copies.  One sequence of 131072
-// keys 57 us in int8, 55.5 in fp8 (277 MB: 4.9 and 5.0 TB/s; the same loop with its copies alone 48 us), 24 sequences of 2000 to 4001 in fp8 34.7 us
-// (155 MB, 4.5 TB/s; 30 us), one of 700 7.3 us: launch, one page's latency, join.  Verify blocks (4 sequences of 5626 to 9001, 6 rows each, int8): 51 us
-// for 63 MB, the chain of products, weights and conversions of two warps a scheduler (0.42 instructions a cycle; 680 of them a pair of pages and 700 an
-// item of six pairs, three or four items a CTA); sixteen columns an item: twenty-four were 7 % slower and eight convert all of K and V twice as often.
-// Tried and slower: codes in registers instead of shared memory (24 sequences 53 us), pages converted once for 64 columns by all warps
-// together (verify 66 us when this took 54; a barrier every pair of pages), bulk copies of four rows (41 and 63 us: they arrive later), tcgen05
-// products with V converted into shared memory (54 and 56 us, 77 for 131072 keys: with eight columns the products are all issue and latency,
-// and rows of verify blocks must not differ from decode), joining in the last CTA of a row (45 us).
+// keys 57 us in int8, 55.5 in fp8 (277 MB: 4.9 and 5.0 TB/s; the same loop with its copies alone 48 us), 24 sequences of 2000 to 4001
+// in fp8 34.7 us (155 MB, 4.5 TB/s; 30 us), one of 700 7.3 us: launch, one page's latency, join.  Verify blocks (4 sequences of 5626
+// to 9001, 6 rows each, int8): 51 us for 63 MB, the chain of products, weights and conversions of two warps a scheduler (0.42
+// instructions a cycle; 680 of them a pair of pages and 700 an item of six pairs, three or four items a CTA); sixteen columns an item:
+// twenty-four were 7 % slower and eight convert all of K and V twice as often. Tried and slower: codes in registers instead of shared
+// memory (24 sequences 53 us), pages converted once for 64 columns by all warps together (verify 66 us when this took 54; a barrier
+// every pair of pages), bulk copies of four rows (41 and 63 us: they arrive later), tcgen05 products with V converted into shared
+// memory (54 and 56 us, 77 for 131072 keys: with eight columns the products are all issue and latency, and rows of verify blocks must
+// not differ from decode), joining in the last CTA of a row (45 us).
 #include <algorithm>
 #include <type_traits>
 

@@ -236,8 +236,8 @@ def cmd_plan(ns):
     cfg = EngineConfig.resolve(ns)
     from .serve import budget as B
     mc = _model_config(cfg)
-    slots = max(cfg.max_batch, 1) + max(0, min(cfg.max_convs, 64))                   # what `serve` builds
-    kv = B.kv_cache_plan(mc, cfg.wctx, cfg.max_batch, cfg.tp, cfg.split_keys, slots=slots)
+    together = 1 if cfg.mode == "personal" else max(cfg.max_batch, 1)                # as `serve` builds it
+    kv = B.kv_cache_plan(mc, cfg.wctx, together, cfg.tp, cfg.split_keys, slots=together + max(0, min(cfg.max_convs, 64)), counted=cfg.max_batch)
     kw = {} if mc.kv_cache == "bf16" else dict(allow_host_tier=kv["host_tier"], split_keys=kv["split_keys"])
     rep = H.plan(budget_gib=cfg.budget_gib, gpu_free_gib=ns.gpu_free_gib, weights_bytes=mc.weight_bytes(cfg.tp) + kv["extra_bytes"],
                  kv_bytes_per_token=mc.kv_bytes_per_token(cfg.tp), page_size=mc.page_size, max_batch=cfg.max_batch,

@@ -108,3 +108,14 @@ def test_a_parked_sequence_goes_back_to_its_own_format_only():
         with pytest.raises(ValueError, match="parked"):
             DenseModel.unpark(m, 0, {"len": 3, "kv": torch.zeros(2, 1, 2, 2176, dtype=torch.uint8), "rope_delta": 0, "kv_cache": other})
     assert touched == []
+
+
+@pytest.mark.parametrize("mode,split", [("personal", 256), ("server", 768)])
+def test_the_plan_command_takes_the_servers_split(monkeypatch, mode, split):
+    """A personal server decodes one conversation at a time, whatever --max-batch says."""
+    from agens_engine_b200.serve import host as H
+    got = {}
+    monkeypatch.setattr(H, "plan", lambda **kw: got.update(kw) or {"lines": []})
+    argv = ["--random", "dense-32b", "--budget-gib", "64", "--wctx", "8192", "--kv-cache", "int8", "--mode", mode]
+    assert cli.main(["plan", *argv]) == 0
+    assert got["split_keys"] == split == _serve(monkeypatch, argv[2:])[0]["kv_split"]

@@ -115,7 +115,9 @@ def test_the_plan_command_takes_the_servers_split(monkeypatch, mode, split):
     """A personal server decodes one conversation at a time, whatever --max-batch says."""
     from agens_engine_b200.serve import host as H
     got = {}
-    monkeypatch.setattr(H, "plan", lambda **kw: got.update(kw) or {"lines": []})
+    real = H.plan
+    monkeypatch.setattr(H, "plan", lambda **kw: got.update(kw) or real(**kw))
     argv = ["--random", "dense-32b", "--budget-gib", "64", "--wctx", "8192", "--kv-cache", "int8", "--mode", mode]
     assert cli.main(["plan", *argv]) == 0
-    assert got["split_keys"] == split == _serve(monkeypatch, argv[2:])[0]["kv_split"]
+    assert got["split_keys"] == split
+    assert split == _serve(monkeypatch, argv[2:])[0]["kv_split"]

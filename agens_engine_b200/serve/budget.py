@@ -81,10 +81,10 @@ class Deployment:
     host_tier: bool
     resident_window_tokens: int
     host_pages: int
-    split_keys: int            # keys per attention split that the plan counts partial results for
     fits: bool
     lines: List[str]
     plan: dict
+    split_keys: int = 64       # keys per attention split that the plan counts partial results for
 
 
 def kv_cache_plan(cfg, wctx: int, max_batch: int, tp: int = 1, split_keys: int = 64, slots: int = 0, counted: int = 0) -> dict:
@@ -110,8 +110,8 @@ def plan_deployment(cfg, budget_gib: float, wctx: int, max_batch: int, sessions:
                     together: Optional[int] = None) -> Deployment:
     """Runs the planner for one rank of a ``tp``-way deployment of the architecture ``cfg`` (the full model's config).
     ``weights_bytes``: measured bytes when the weights are already on the device, else the architecture's estimate
-    plus 0.6 GiB of CUDA context; ``sessions``: slots of the model; ``dual_layout`` doubles the quantised linears (the step kernel's second layout, which a model
-    with an 8-bit KV cache does not have); ``together``: sequences that decode together (default: ``max_batch``)."""
+    plus 0.6 GiB of CUDA context; ``sessions``: slots of the model; ``dual_layout`` doubles the quantised linears (the
+    step kernel's second layout, which a model with an 8-bit KV cache does not have); ``together``: sequences that decode together (default: ``max_batch``)."""
     from . import host as H
     kv = kv_cache_plan(cfg, wctx, together or max_batch, tp, split_keys, slots=sessions, counted=max_batch)
     if weights_bytes is None:
@@ -133,8 +133,8 @@ def plan_deployment(cfg, budget_gib: float, wctx: int, max_batch: int, sessions:
     host = p["tier"] == "host"
     window = int(p["resident_window_pages"]) * ps
     return Deployment(budget_bytes=int(p["budget_bytes"]), n_pages=n_pages, max_ctx=max_ctx, host_tier=host,
-                      resident_window_tokens=window, host_pages=int(p["host_pages"]), split_keys=int(kv["split_keys"]), fits=bool(p["fits"]), lines=list(p["lines"]),
-                      plan=p)
+                      resident_window_tokens=window, host_pages=int(p["host_pages"]), fits=bool(p["fits"]), lines=list(p["lines"]),
+                      plan=p, split_keys=int(kv["split_keys"]))
 
 
 def agree_min(dep: Deployment, all_reduce_min: Callable[[List[int]], List[int]]) -> Deployment:
